@@ -127,6 +127,31 @@ int inferlab_cuda_pool_create(int32_t device, uint32_t dtype, uint64_t num_block
                               uint32_t block_tokens, uint32_t kv_heads, uint32_t head_dim,
                               InferlabCudaKvPool** pool, char* error, size_t error_capacity);
 
+/*
+ * A pool whose K and V rows are held in 4 bits: every 64 dims of a row share an
+ * f16 pair (scale, zero) and a code c in 0..15 stands for zero + (c - 8) *
+ * scale, with scale = f16((max - min) / 15), zero = f16(min + 8 * scale), c =
+ * clamp(rint((x - zero) / scale) + 8, 0, 15): 4.5 bits a value against 16.
+ * `dtype` (INFERLAB_KV_F16 or INFERLAB_KV_BF16) is the row type: rows are
+ * rounded to it before they are quantised, read back in it, and queries and
+ * outputs of the attention entries are in it (or fp32). block_tokens must be a
+ * multiple of 16, head_dim 64 or 128. No counterpart in the reference.
+ * One arena (InferlabCudaPoolInfo.key_arena; value_arena is NULL, element_bytes
+ * 0, block_bytes covers K and V) of [num_blocks][kv_heads][block_tokens / 16]
+ * tiles. A tile holds 16 tokens of one kv-head: key codes [16][D / 2] bytes, key
+ * pairs [16][D / 64] (scale, zero), value codes, value pairs. A code row is made
+ * of 32-bit words of 8 consecutive dims (dim 8 u + n in bits 4 n .. 4 n + 3);
+ * word u of a key row lies at byte (u % 4) * D / 8 + (u / 4) * 4, of a value row
+ * at (u % 8) * D / 16 + (u / 8) * 4, where for D = 128 and slots t with t / 2
+ * odd u % 8 is replaced by (u % 8) ^ 4.
+ * inferlab_cuda_kv_append, _kv_append_rotary, _kv_gather, _kv_gather_rows,
+ * _output_project, _pages_copy and inferlab_cuda_kv4_* take such a pool; the
+ * other entries return an error for it.
+ */
+int inferlab_cuda_pool_create_kv4(int32_t device, uint32_t dtype, uint64_t num_blocks,
+                                  uint32_t block_tokens, uint32_t kv_heads, uint32_t head_dim,
+                                  InferlabCudaKvPool** pool, char* error, size_t error_capacity);
+
 /* Frees the arenas (after synchronising the device). NULL is a no-op. */
 void inferlab_cuda_pool_destroy(InferlabCudaKvPool* pool);
 
@@ -161,6 +186,67 @@ int inferlab_cuda_kv_append(InferlabCudaKvPool* pool, const void* key_rows, cons
                             const int32_t* positions, uint64_t rows, const int32_t* block_tables,
                             uint32_t max_blocks_per_seq, void* stream, char* error,
                             size_t error_capacity);
+
+/*
+ * One call of inferlab_cuda_kv_append_rotary. Row r of queries (q_heads heads;
+ * q_heads 0 and NULL for none), key_rows and value_rows (kv_heads heads) starts
+ * r * stride elements into its array, its heads' head_dim elements one after
+ * another, so the three may be views of one projection output. All rows have
+ * row_dtype (INFERLAB_KV_FP32 or the pool's type).
+ */
+typedef struct InferlabCudaRotaryAppend {
+    const void* queries;
+    const void* key_rows;
+    const void* value_rows;
+    uint32_t row_dtype;
+    uint32_t q_heads;
+    uint64_t query_stride;
+    uint64_t key_stride;
+    uint64_t value_stride;
+    const float* cos_sin;           /* [cos_sin_positions][rotary_dim]: cosines, then sines */
+    uint64_t cos_sin_positions;
+    uint32_t rotary_dim;            /* even, <= head_dim; 0: no rotation */
+    uint32_t interleaved;           /* pairs (2i, 2i+1) instead of (i, i + rotary_dim / 2) */
+    const int32_t* row_sequences;   /* [rows]; -1: a padded row, skipped */
+    const int32_t* positions;       /* [rows] */
+    uint64_t rows;
+    const int32_t* block_tables;    /* [num_seqs][max_blocks_per_seq] */
+    uint32_t num_seqs;
+    uint32_t max_blocks_per_seq;
+    void* q_out;                    /* [rows][q_heads][head_dim] of q_out_dtype */
+    uint32_t q_out_dtype;           /* INFERLAB_KV_FP32 or the pool's type */
+    uint32_t reserved;
+} InferlabCudaRotaryAppend;
+
+/*
+ * inferlab_cuda_kv_append with the position rotation applied on the way: each
+ * pair (a, b) of the first rotary_dim dims of every Q and K head becomes
+ * (a cos - b sin, b cos + a sin) by row positions[r] of cos_sin, in fp32,
+ * rounded once; Q goes to q_out, K and V to the pool (any pool). Padded rows
+ * (sequence -1) are skipped: neither the pool nor q_out is written, no error.
+ * A row whose sequence, position or block id is bad, or whose position lies
+ * behind the table of angles, is reported through the pool's error word and
+ * skipped whole. K/V values that the pool cannot hold as finite numbers (for
+ * a 4-bit pool, as a group with finite f16 scale and zero) are reported
+ * ("attention input must be finite") and that row is skipped whole. q_out must
+ * not overlap the input rows. Two rows of one call with the same sequence and
+ * position leave an unspecified one of the two, in a 4-bit pool possibly a
+ * mixture. No counterpart in the reference (its positions are learned vectors).
+ */
+int inferlab_cuda_kv_append_rotary(InferlabCudaKvPool* pool, const InferlabCudaRotaryAppend* call,
+                                   void* stream, char* error, size_t error_capacity);
+
+/*
+ * Reads rows back: row r of keys_out / values_out [rows][kv_heads][head_dim]
+ * (the pool's type; a 4-bit pool's row type, saturating) is the pool's row at
+ * position positions[r] of sequence row_sequences[r]. Padded rows (sequence -1)
+ * and bad ones (reported through the error word) are left as they were.
+ */
+int inferlab_cuda_kv_gather_rows(InferlabCudaKvPool* pool, const int32_t* row_sequences,
+                                 const int32_t* positions, uint64_t rows,
+                                 const int32_t* block_tables, uint32_t num_seqs,
+                                 uint32_t max_blocks_per_seq, void* keys_out, void* values_out,
+                                 void* stream, char* error, size_t error_capacity);
 
 /*
  * The Q/K/V projection beside attention, with the K/V rows appended in the
@@ -395,6 +481,44 @@ int inferlab_cuda_paged_prefill(InferlabCudaKvPool* pool, const void* queries, u
                                 uint32_t q_heads, uint32_t max_query_count,
                                 uint64_t total_queries, float* out, void* stream, char* error,
                                 size_t error_capacity);
+
+/*
+ * Attention over a 4-bit pool (inferlab_cuda_pool_create_kv4). No counterpart
+ * in the reference.
+ * _kv4_decode: one query token per sequence at position context_lens[i] - 1,
+ * like inferlab_cuda_paged_decode; context_lens[i] 0 is a slot of the batch that
+ * holds no sequence: its output row is zero, no error.
+ * _kv4_prefill: several query tokens per segment, causal among themselves,
+ * like inferlab_cuda_paged_prefill (drafted tokens, prompt chunks, prompts); a
+ * segment of count 0 has no rows.
+ * queries and out are [..][q_heads][head_dim] of query_dtype: the pool's row
+ * type, or fp32 (queries rounded to the row type on load, as the reference's
+ * 16-bit modes do). Scores, softmax statistics and sums are fp32.
+ * max_context_len bounds every context (start + count for segments); a context
+ * over it, over the table's width, or negative is reported through the pool's
+ * error word and its rows are zero. Long contexts are split across CTAs and
+ * merged in split order inside the launch. workspace:
+ * inferlab_cuda_kv4_workspace_size bytes, initialised once with
+ * inferlab_cuda_paged_decode_workspace_init; launches that may overlap (other
+ * streams, graphs replayed side by side) need one each.
+ */
+size_t inferlab_cuda_kv4_workspace_size(const InferlabCudaKvPool* pool, uint32_t num_seqs,
+                                        uint32_t q_heads, uint32_t max_query_count,
+                                        uint32_t max_context_len);
+int inferlab_cuda_kv4_decode(InferlabCudaKvPool* pool, const void* queries, uint32_t query_dtype,
+                             const int32_t* block_tables, uint32_t max_blocks_per_seq,
+                             const int32_t* context_lens, uint32_t num_seqs, uint32_t q_heads,
+                             uint32_t max_context_len, void* out, void* workspace,
+                             size_t workspace_bytes, void* stream, char* error,
+                             size_t error_capacity);
+int inferlab_cuda_kv4_prefill(InferlabCudaKvPool* pool, const void* queries, uint32_t query_dtype,
+                              const int32_t* block_tables, uint32_t max_blocks_per_seq,
+                              const int32_t* query_starts, const int32_t* query_counts,
+                              const int32_t* query_offsets, uint32_t num_segments, uint32_t q_heads,
+                              uint32_t max_query_count, uint64_t total_queries,
+                              uint32_t max_context_len, void* out, void* workspace,
+                              size_t workspace_bytes, void* stream, char* error,
+                              size_t error_capacity);
 
 /* ---- Block ownership (host metadata over the device pool) -------------------
  *

@@ -65,6 +65,34 @@ class InferlabCudaPoolInfo(ctypes.Structure):
     ]
 
 
+class InferlabCudaRotaryAppend(ctypes.Structure):
+    """One call of inferlab_cuda_kv_append_rotary."""
+
+    _fields_ = [
+        ("queries", c_vp),
+        ("key_rows", c_vp),
+        ("value_rows", c_vp),
+        ("row_dtype", ctypes.c_uint32),
+        ("q_heads", ctypes.c_uint32),
+        ("query_stride", ctypes.c_uint64),
+        ("key_stride", ctypes.c_uint64),
+        ("value_stride", ctypes.c_uint64),
+        ("cos_sin", c_vp),
+        ("cos_sin_positions", ctypes.c_uint64),
+        ("rotary_dim", ctypes.c_uint32),
+        ("interleaved", ctypes.c_uint32),
+        ("row_sequences", c_vp),
+        ("positions", c_vp),
+        ("rows", ctypes.c_uint64),
+        ("block_tables", c_vp),
+        ("num_seqs", ctypes.c_uint32),
+        ("max_blocks_per_seq", ctypes.c_uint32),
+        ("q_out", c_vp),
+        ("q_out_dtype", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
 class InferlabPagedCacheStats(ctypes.Structure):
     """worker/cpp/inferlab_runtime.h:7-31."""
 
@@ -89,6 +117,9 @@ SIGNATURES = {
     "inferlab_cuda_pool_create": (ctypes.c_int, [
         ctypes.c_int32, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32,
         ctypes.c_uint32, ctypes.POINTER(c_vp), c_err, c_sz]),
+    "inferlab_cuda_pool_create_kv4": (ctypes.c_int, [
+        ctypes.c_int32, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32,
+        ctypes.c_uint32, ctypes.POINTER(c_vp), c_err, c_sz]),
     "inferlab_cuda_pool_destroy": (None, [c_vp]),
     "inferlab_cuda_peer_buffer_bytes": (ctypes.c_uint64, [ctypes.c_uint32, ctypes.c_uint64,
                                                           ctypes.c_uint32]),
@@ -110,6 +141,20 @@ SIGNATURES = {
     "inferlab_cuda_pool_synchronize": (ctypes.c_int, [c_vp, c_vp, ctypes.c_uint32, c_err, c_sz]),
     "inferlab_cuda_kv_append": (ctypes.c_int, [
         c_vp, c_vp, c_vp, ctypes.c_uint32, c_vp, c_vp, ctypes.c_uint64, c_vp, ctypes.c_uint32,
+        c_vp, c_err, c_sz]),
+    "inferlab_cuda_kv_append_rotary": (ctypes.c_int, [
+        c_vp, ctypes.POINTER(InferlabCudaRotaryAppend), c_vp, c_err, c_sz]),
+    "inferlab_cuda_kv_gather_rows": (ctypes.c_int, [
+        c_vp, c_vp, c_vp, ctypes.c_uint64, c_vp, ctypes.c_uint32, ctypes.c_uint32, c_vp, c_vp,
+        c_vp, c_err, c_sz]),
+    "inferlab_cuda_kv4_workspace_size": (c_sz, [
+        c_vp, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32]),
+    "inferlab_cuda_kv4_decode": (ctypes.c_int, [
+        c_vp, c_vp, ctypes.c_uint32, c_vp, ctypes.c_uint32, c_vp, ctypes.c_uint32,
+        ctypes.c_uint32, ctypes.c_uint32, c_vp, c_vp, c_sz, c_vp, c_err, c_sz]),
+    "inferlab_cuda_kv4_prefill": (ctypes.c_int, [
+        c_vp, c_vp, ctypes.c_uint32, c_vp, ctypes.c_uint32, c_vp, c_vp, c_vp, ctypes.c_uint32,
+        ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_uint32, c_vp, c_vp, c_sz,
         c_vp, c_err, c_sz]),
     "inferlab_cuda_kv_gather": (ctypes.c_int, [
         c_vp, c_vp, ctypes.c_uint64, c_vp, c_vp, c_vp, c_err, c_sz]),

@@ -237,7 +237,7 @@ int decode_step_host(InferlabCudaKvPool* pool, const float* queries, const float
                      std::size_t error_capacity) {
     return ilb::protect(error, error_capacity, [&] {
         using namespace ilb;
-        auto& p = checked_pool(pool);
+        auto& p = checked_wide_pool(pool, "decode step does not read a 4-bit pool");
         if (num_seqs == 0) return;
         if (queries == nullptr || block_tables == nullptr || context_lens == nullptr ||
             out == nullptr) {

@@ -5,6 +5,7 @@
 #include "pool.cuh"
 
 struct InferlabCudaPeerExchange;
+struct InferlabCudaRotaryAppend;
 
 namespace ilb {
 
@@ -59,5 +60,15 @@ void launch_kv_append(InferlabCudaKvPool& pool, const void* key_rows, const void
                       const std::int32_t* positions, std::uint64_t rows,
                       const std::int32_t* block_tables, std::uint32_t max_blocks,
                       cudaStream_t stream);
+
+// Launches the rotary append (see inferlab_cuda_kv_append_rotary), any pool;
+// the pool's device must be current. padded_rows: sequence -1 marks a padded
+// row instead of being an error.
+void launch_rotary_append(InferlabCudaKvPool& pool, const InferlabCudaRotaryAppend& call,
+                          bool padded_rows, cudaStream_t stream);
+
+// The first `tokens` rows of a table of a 4-bit pool, widened to its row type.
+void launch_kv4_gather(InferlabCudaKvPool& pool, const std::int32_t* block_table,
+                       std::uint64_t tokens, void* keys_out, void* values_out, cudaStream_t stream);
 
 }  // namespace ilb

@@ -1,0 +1,99 @@
+// kv4.cuh - the packed 4-bit pool: what a code stands for and where it lies.
+//
+// Every 64 dims of one token's K or V row of one kv-head share a pair of f16
+// numbers (scale, zero); a code c in 0..15 stands for zero + (c - 8) * scale.
+// A row is quantised from values x already rounded to the pool's 16-bit row
+// type:
+//   scale = f16((max - min) / 15)     zero = f16(min + 8 * scale)
+//   c = clamp(rint((x - zero) * (1 / scale)) + 8, 0, 15), 8 where scale is 0.
+// Codes counted from 8 keep sum p (c - 8) a sum of either sign, so that the
+// fp32 accumulators of a long, flat softmax do not grow far beyond the output.
+//
+// One arena [num_blocks][kv_heads][block_tokens / 16][tile]. A tile is 16
+// tokens of one kv-head in one contiguous run, so one bulk copy moves it:
+//   key codes   [16][D / 2] bytes, key pairs   [16][D / 64] (scale, zero),
+//   value codes [16][D / 2] bytes, value pairs [16][D / 64] (scale, zero).
+// D = 128: 2304 bytes (144 a token against 512 in 16 bits), D = 64: 1152.
+//
+// A code row is made of 32-bit words of 8 consecutive dims (dim 8 w + n in
+// bits 4n..4n+3). The words are ordered for the attention's mma fragments, so
+// that a lane reads its part of a row with one load:
+//   keys:   lane t of four holds, for every 32 dims, dims 8t .. 8t+7;
+//           word (w, t) (dims 32 w + 8 t ..) lies at t * D / 8 + 4 w bytes.
+//   values: lane g of eight holds, for every 64 dims, dims 8g .. 8g+7;
+//           word (w, g) (dims 64 w + 8 g ..) lies at g' * D / 16 + 4 w bytes,
+//           g' = g, but g ^ 4 in tokens 2, 3 of every four when D is 128: four
+//           token rows read by four lanes then fall on different banks.
+#pragma once
+
+#include "common.cuh"
+
+namespace ilb {
+namespace kv4 {
+
+constexpr int kGroup = 64;       // dims that share a (scale, zero) pair
+constexpr int kTileTokens = 16;
+
+__host__ __device__ constexpr int code_bytes(int d) { return kTileTokens * (d / 2); }
+__host__ __device__ constexpr int pair_bytes(int d) { return kTileTokens * (d / kGroup) * 4; }
+__host__ __device__ constexpr int half_tile_bytes(int d) { return code_bytes(d) + pair_bytes(d); }
+__host__ __device__ constexpr int tile_bytes(int d) { return 2 * half_tile_bytes(d); }
+
+// Byte of the word that holds dims 8 unit .. 8 unit + 7 of token slot `t`.
+__device__ __forceinline__ int key_word(int d, int t, int unit) {
+    return t * (d / 2) + (unit & 3) * (d / 8) + (unit >> 2) * 4;
+}
+__device__ __forceinline__ int value_word(int d, int t, int unit) {
+    const int chunk = (unit & 7) ^ (d == 128 ? ((t >> 1) & 1) * 4 : 0);
+    return half_tile_bytes(d) + t * (d / 2) + chunk * (d / 16) + (unit >> 3) * 4;
+}
+// Byte of the (scale, zero) pair of group `g` of token slot `t`; value = 0 / 1.
+__device__ __forceinline__ int pair_at(int d, int t, int g, int value) {
+    return value * half_tile_bytes(d) + code_bytes(d) + (t * (d / kGroup) + g) * 4;
+}
+
+__device__ __forceinline__ float2 load_pair(const unsigned char* tile, int at) {
+    return __half22float2(*reinterpret_cast<const __half2*>(tile + at));
+}
+
+// A code's value, fp32 with one rounding per operation.
+__device__ __forceinline__ float code_value(std::uint32_t word, int n, float2 pair) {
+    const float c = static_cast<float>((word >> (4 * n)) & 15u) - 8.0f;
+    return __fadd_rn(__fmul_rn(c, pair.x), pair.y);
+}
+
+// Quantises the 8 dims of this lane's unit; the 8 lanes of an aligned octet
+// hold the 64 dims of one group. Returns the word of codes and the pair;
+// `bad` reports a non-finite value or a pair outside f16.
+__device__ __forceinline__ std::uint32_t quantise(const float (&x)[8], __half2& pair, bool& bad) {
+    float low = x[0], high = x[0];
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        finite &= isfinite(x[i]);
+        low = fminf(low, x[i]);
+        high = fmaxf(high, x[i]);
+    }
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) {
+        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, off));
+        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, off));
+    }
+    const __half scale_h = __float2half_rn(__fdiv_rn(__fsub_rn(high, low), 15.0f));
+    const float scale = __half2float(scale_h);
+    const __half zero_h = __float2half_rn(__fadd_rn(low, 8.0f * scale));
+    const float zero = __half2float(zero_h);
+    bad = !finite || !isfinite(scale) || !isfinite(zero);
+    pair = __halves2half2(scale_h, zero_h);
+    const float inverse = scale > 0.0f ? __frcp_rn(scale) : 0.0f;
+    std::uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int c = __float2int_rn(__fmul_rn(__fsub_rn(x[i], zero), inverse)) + 8;
+        word |= static_cast<std::uint32_t>(min(max(c, 0), 15)) << (4 * i);
+    }
+    return word;
+}
+
+}  // namespace kv4
+}  // namespace ilb

@@ -6,11 +6,13 @@
 // write) stays on the host; only block ids cross to the device.
 #include "common.cuh"
 #include "internal.cuh"
+#include "kv4.cuh"
 #include "pool.cuh"
 
 #include "../../include/inferlab_attention.h"
 
 #include <memory>
+#include <utility>
 #include <type_traits>
 
 namespace ilb {
@@ -147,6 +149,65 @@ void launch_kv_append(InferlabCudaKvPool& pool, const void* key_rows, const void
 
 }  // namespace ilb
 
+namespace ilb {
+namespace {
+
+// Frees what a half-made pool holds when a later allocation throws.
+struct PoolDeleter {
+    void operator()(InferlabCudaKvPool* p) const {
+        if (p->key_arena != nullptr) cudaFree(p->key_arena);
+        if (p->value_arena != nullptr) cudaFree(p->value_arena);
+        if (p->error_word != nullptr) cudaFree(p->error_word);
+        if (p->error_host != nullptr) cudaFreeHost(p->error_host);
+        delete p;
+    }
+};
+
+// The pool's device memory, zero-filled, once its geometry is set (one arena
+// when value_arena_bytes is 0); returns the finished pool.
+InferlabCudaKvPool* allocate_pool(std::unique_ptr<InferlabCudaKvPool, PoolDeleter> owned,
+                                  std::size_t value_arena_bytes) {
+    cuda_check(cudaMalloc(&owned->key_arena, owned->arena_bytes), "cudaMalloc key arena");
+    if (value_arena_bytes != 0) {
+        cuda_check(cudaMalloc(&owned->value_arena, value_arena_bytes), "cudaMalloc value arena");
+    }
+    cuda_check(cudaMalloc(&owned->error_word, kPoolWordBytes), "cudaMalloc error word");
+    cuda_check(cudaMallocHost(&owned->error_host, 16), "cudaMallocHost");
+    cuda_check(cudaMemset(owned->key_arena, 0, owned->arena_bytes), "cudaMemset");
+    if (value_arena_bytes != 0) cuda_check(cudaMemset(owned->value_arena, 0, value_arena_bytes), "cudaMemset");
+    cuda_check(cudaMemset(owned->error_word, 0, kPoolWordBytes), "cudaMemset");
+    cuda_check(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
+    return owned.release();
+}
+
+// The checks every pool shares; returns the pool with its geometry set.
+std::unique_ptr<InferlabCudaKvPool, PoolDeleter> checked_geometry(std::uint64_t num_blocks,
+                                                                  std::uint32_t block_tokens,
+                                                                  std::uint32_t kv_heads,
+                                                                  std::uint32_t head_dim) {
+    if (num_blocks == 0 || block_tokens == 0 || kv_heads == 0 || head_dim == 0) {
+        throw std::runtime_error("paged KV cache dimensions must be positive");
+    }
+    if (num_blocks > 0x7FFFFFFFull) {
+        throw std::runtime_error("paged KV num_blocks must fit a 32-bit block id");
+    }
+    std::unique_ptr<InferlabCudaKvPool, PoolDeleter> owned(new InferlabCudaKvPool);
+    owned->block_tokens = block_tokens;
+    owned->kv_heads = kv_heads;
+    owned->head_dim = head_dim;
+    owned->num_blocks = num_blocks;
+    return owned;
+}
+
+void check_device(std::int32_t device) {
+    int count = 0;
+    cuda_check(cudaGetDeviceCount(&count), "cudaGetDeviceCount");
+    if (device < 0 || device >= count) throw std::runtime_error("CUDA device index out of range");
+}
+
+}  // namespace
+}  // namespace ilb
+
 extern "C" int inferlab_cuda_pool_create(std::int32_t device, std::uint32_t dtype,
                                          std::uint64_t num_blocks, std::uint32_t block_tokens,
                                          std::uint32_t kv_heads, std::uint32_t head_dim,
@@ -157,42 +218,52 @@ extern "C" int inferlab_cuda_pool_create(std::int32_t device, std::uint32_t dtyp
         if (pool == nullptr) throw std::runtime_error("paged KV pool output pointer is null");
         *pool = nullptr;
         if (dtype > 2) throw std::runtime_error("paged KV dtype must be 0 (FP32), 1 (FP16), or 2 (BF16)");
-        if (num_blocks == 0 || block_tokens == 0 || kv_heads == 0 || head_dim == 0) {
-            throw std::runtime_error("paged KV cache dimensions must be positive");
-        }
-        if (num_blocks > 0x7FFFFFFFull) {
-            throw std::runtime_error("paged KV num_blocks must fit a 32-bit block id");
-        }
-        int count = 0;
-        cuda_check(cudaGetDeviceCount(&count), "cudaGetDeviceCount");
-        if (device < 0 || device >= count) throw std::runtime_error("CUDA device index out of range");
+        auto owned = checked_geometry(num_blocks, block_tokens, kv_heads, head_dim);
+        check_device(device);
         DeviceGuard guard(device);
-        auto owned = std::make_unique<InferlabCudaKvPool>();
         owned->device = device;
         owned->dtype = dtype;
         owned->element_bytes = dtype == kFp32 ? 4 : 2;
-        owned->block_tokens = block_tokens;
-        owned->kv_heads = kv_heads;
-        owned->head_dim = head_dim;
-        owned->num_blocks = num_blocks;
         const char* overflow = "paged KV pool size overflows";
         owned->block_bytes = checked_mul(
             checked_mul(checked_mul(block_tokens, kv_heads, overflow), head_dim, overflow),
             owned->element_bytes, overflow);
         owned->arena_bytes = checked_mul(owned->block_bytes, num_blocks, overflow);
-        cuda_check(cudaMalloc(&owned->key_arena, owned->arena_bytes), "cudaMalloc key arena");
-        const cudaError_t second = cudaMalloc(&owned->value_arena, owned->arena_bytes);
-        if (second != cudaSuccess) {
-            cudaFree(owned->key_arena);
-            cuda_check(second, "cudaMalloc value arena");
+        const std::size_t value_bytes = owned->arena_bytes;
+        *pool = allocate_pool(std::move(owned), value_bytes);
+    });
+}
+
+extern "C" int inferlab_cuda_pool_create_kv4(std::int32_t device, std::uint32_t dtype,
+                                             std::uint64_t num_blocks, std::uint32_t block_tokens,
+                                             std::uint32_t kv_heads, std::uint32_t head_dim,
+                                             InferlabCudaKvPool** pool, char* error,
+                                             std::size_t error_capacity) {
+    return ilb::protect(error, error_capacity, [&] {
+        using namespace ilb;
+        if (pool == nullptr) throw std::runtime_error("paged KV pool output pointer is null");
+        *pool = nullptr;
+        if (dtype != kF16 && dtype != kBf16) {
+            throw std::runtime_error("4-bit paged KV row dtype must be 1 (FP16) or 2 (BF16)");
         }
-        cuda_check(cudaMalloc(&owned->error_word, ilb::kPoolWordBytes), "cudaMalloc error word");
-        cuda_check(cudaMallocHost(&owned->error_host, 16), "cudaMallocHost");
-        cuda_check(cudaMemset(owned->key_arena, 0, owned->arena_bytes), "cudaMemset");
-        cuda_check(cudaMemset(owned->value_arena, 0, owned->arena_bytes), "cudaMemset");
-        cuda_check(cudaMemset(owned->error_word, 0, ilb::kPoolWordBytes), "cudaMemset");
-        cuda_check(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
-        *pool = owned.release();
+        auto owned = checked_geometry(num_blocks, block_tokens, kv_heads, head_dim);
+        if (block_tokens % kv4::kTileTokens != 0) {
+            throw std::runtime_error("4-bit paged KV block_tokens must be a multiple of 16");
+        }
+        if (head_dim != 64 && head_dim != 128) {
+            throw std::runtime_error("4-bit paged KV head_dim must be 64 or 128");
+        }
+        check_device(device);
+        DeviceGuard guard(device);
+        owned->device = device;
+        owned->dtype = dtype;
+        owned->element_bytes = 0;
+        owned->kv_bits = 4;
+        const char* overflow = "paged KV pool size overflows";
+        owned->block_bytes = checked_mul(checked_mul(block_tokens / kv4::kTileTokens, kv_heads, overflow),
+                                         kv4::tile_bytes(static_cast<int>(head_dim)), overflow);
+        owned->arena_bytes = checked_mul(owned->block_bytes, num_blocks, overflow);
+        *pool = allocate_pool(std::move(owned), 0);
     });
 }
 
@@ -277,6 +348,21 @@ extern "C" int inferlab_cuda_kv_append(InferlabCudaKvPool* pool, const void* key
         if (rows > 0x7FFFFFFFull) throw std::runtime_error("paged KV append row count is too large");
         DeviceGuard guard(p.device);
         auto s = static_cast<cudaStream_t>(stream);
+        if (p.kv_bits != 0) {
+            InferlabCudaRotaryAppend call{};
+            call.key_rows = key_rows;
+            call.value_rows = value_rows;
+            call.row_dtype = row_dtype;
+            call.key_stride = call.value_stride = static_cast<std::uint64_t>(p.kv_heads) * p.head_dim;
+            call.row_sequences = row_sequences;
+            call.positions = positions;
+            call.rows = rows;
+            call.block_tables = block_tables;
+            call.num_seqs = 0x7FFFFFFFu;  // this entry is not told the table's height
+            call.max_blocks_per_seq = max_blocks_per_seq;
+            launch_rotary_append(p, call, false, s);
+            return;
+        }
         if (p.dtype == kFp32) {
             launch_append<float>(p, key_rows, value_rows, row_dtype, row_sequences, positions, rows,
                                  block_tables, max_blocks_per_seq, s);
@@ -304,6 +390,10 @@ extern "C" int inferlab_cuda_kv_gather(InferlabCudaKvPool* pool, const std::int3
         if (tokens > 0x7FFFFFFFull) throw std::runtime_error("paged KV gather is too long");
         DeviceGuard guard(p.device);
         auto s = static_cast<cudaStream_t>(stream);
+        if (p.kv_bits != 0) {
+            launch_kv4_gather(p, block_table, tokens, keys_out, values_out, s);
+            return;
+        }
         const std::size_t row_bytes = static_cast<std::size_t>(p.head_dim) * p.element_bytes;
         const auto* ka = static_cast<const unsigned char*>(p.key_arena);
         const auto* va = static_cast<const unsigned char*>(p.value_arena);

@@ -333,8 +333,7 @@ extern "C" int inferlab_cuda_pages_copy(InferlabCudaKvPool* pool, const int32_t*
         if (from == nullptr || to == nullptr) throw std::runtime_error("page manager argument is null");
         DeviceGuard guard(p.device);
         auto s = static_cast<cudaStream_t>(stream);
-        const std::size_t block_bytes =
-            static_cast<std::size_t>(p.kv_heads) * p.block_tokens * p.head_dim * p.element_bytes;
+        const std::size_t block_bytes = p.block_bytes;
         for (std::uint32_t i = 0; i < count; ++i) {
             if (from[i] < 0 || to[i] < 0 || static_cast<std::uint64_t>(from[i]) >= p.num_blocks ||
                 static_cast<std::uint64_t>(to[i]) >= p.num_blocks) {
@@ -343,6 +342,7 @@ extern "C" int inferlab_cuda_pages_copy(InferlabCudaKvPool* pool, const int32_t*
             // A block of one arena, all kv-heads, is one contiguous run.
             for (unsigned char* arena : {static_cast<unsigned char*>(p.key_arena),
                                          static_cast<unsigned char*>(p.value_arena)}) {
+                if (arena == nullptr) continue;  // a 4-bit pool keeps K and V in one arena
                 cuda_check(cudaMemcpyAsync(arena + static_cast<std::size_t>(to[i]) * block_bytes,
                                            arena + static_cast<std::size_t>(from[i]) * block_bytes,
                                            block_bytes, cudaMemcpyDeviceToDevice, s),

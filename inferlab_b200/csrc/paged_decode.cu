@@ -1156,7 +1156,7 @@ extern "C" int inferlab_cuda_paged_decode_exchange(InferlabCudaKvPool* pool, con
                                                    InferlabCudaPeerExchange* exchange, float* out, void* stream,
                                                    char* error, std::size_t error_capacity) {
     return ilb::protect(error, error_capacity, [&] {
-        auto& p = ilb::checked_pool(pool);
+        auto& p = ilb::checked_wide_pool(pool, "paged decode exchange does not read a 4-bit pool");
         ilb::validate_decode(p, queries, block_tables, max_blocks, context_lens, num_seqs, q_heads,
                              max_context_len);
         if (out == nullptr) throw std::runtime_error("paged decode pointer is null");
@@ -1199,7 +1199,7 @@ extern "C" std::size_t inferlab_cuda_paged_decode_workspace_size(const InferlabC
                                                                  std::uint32_t num_seqs,
                                                                  std::uint32_t q_heads,
                                                                  std::uint32_t max_context_len) {
-    if (pool == nullptr || num_seqs == 0 || q_heads == 0 || max_context_len == 0) return 0;
+    if (pool == nullptr || pool->kv_bits != 0 || num_seqs == 0 || q_heads == 0 || max_context_len == 0) return 0;
     try {
         const auto plan = ilb::full_plan(*pool, num_seqs, q_heads, max_context_len);
         return ilb::workspace_bytes_for(num_seqs, q_heads, pool->kv_heads, pool->head_dim, plan);
@@ -1241,7 +1241,7 @@ extern "C" int inferlab_cuda_paged_decode(InferlabCudaKvPool* pool, const float*
                                           void* stream, char* error, std::size_t error_capacity) {
     return ilb::protect(error, error_capacity, [&] {
         using namespace ilb;
-        auto& p = checked_pool(pool);
+        auto& p = checked_wide_pool(pool, "inferlab_cuda_kv4_decode reads a 4-bit pool");
         if (num_seqs == 0) return;
         validate_decode(p, queries, block_tables, max_blocks_per_seq, context_lens, num_seqs,
                         q_heads, max_context_len);
@@ -1261,7 +1261,7 @@ extern "C" int inferlab_cuda_paged_decode_partials(
     std::size_t error_capacity) {
     return ilb::protect(error, error_capacity, [&] {
         using namespace ilb;
-        auto& p = checked_pool(pool);
+        auto& p = checked_wide_pool(pool, "paged decode partials do not read a 4-bit pool");
         if (num_seqs == 0) return;
         validate_decode(p, queries, block_tables, max_blocks_per_seq, context_lens, num_seqs,
                         q_heads, max_context_len);

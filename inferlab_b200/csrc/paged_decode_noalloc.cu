@@ -67,7 +67,7 @@ extern "C" int inferlab_cuda_paged_decode_noalloc(InferlabCudaKvPool* pool, cons
                                                   std::size_t error_capacity) {
     return ilb::protect(error, error_capacity, [&] {
         using namespace ilb;
-        auto& p = checked_pool(pool);
+        auto& p = checked_wide_pool(pool, "paged decode without a workspace does not read a 4-bit pool");
         if (num_seqs == 0) return;
         check_decode_arguments(p, queries, block_tables, max_blocks_per_seq, context_lens,
                                num_seqs, q_heads, max_context_len);

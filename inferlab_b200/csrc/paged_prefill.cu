@@ -97,7 +97,7 @@ extern "C" int inferlab_cuda_paged_prefill(InferlabCudaKvPool* pool, const void*
                                            std::size_t error_capacity) {
     return ilb::protect(error, error_capacity, [&] {
         using namespace ilb;
-        auto& p = checked_pool(pool);
+        auto& p = checked_wide_pool(pool, "inferlab_cuda_kv4_prefill reads a 4-bit pool");
         if (num_segments == 0 || total_queries == 0) return;
         if (queries == nullptr || block_tables == nullptr || query_starts == nullptr ||
             query_counts == nullptr || query_offsets == nullptr || out == nullptr) {

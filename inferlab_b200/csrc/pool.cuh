@@ -16,6 +16,9 @@ struct InferlabCudaKvPool {
     std::uint32_t head_dim = 1;
     std::uint64_t num_blocks = 0;
     std::uint64_t block_bytes = 0;  // one block, all kv-heads, one arena
+    // 4: one packed 4-bit arena (kv4.cuh) in key_arena, value_arena null,
+    // dtype the 16-bit type rows are rounded to, element_bytes 0. Else 0.
+    std::uint32_t kv_bits = 0;
     std::uint64_t arena_bytes = 0;
     void* key_arena = nullptr;
     void* value_arena = nullptr;
@@ -51,6 +54,13 @@ inline InferlabCudaKvPool& checked_pool(InferlabCudaKvPool* pool) {
 inline const InferlabCudaKvPool& checked_pool(const InferlabCudaKvPool* pool) {
     if (pool == nullptr) throw std::runtime_error("paged KV pool pointer is null");
     return *pool;
+}
+
+// The pool of an entry that reads whole elements of the pool's type.
+inline InferlabCudaKvPool& checked_wide_pool(InferlabCudaKvPool* pool, const char* message) {
+    auto& p = checked_pool(pool);
+    if (p.kv_bits != 0) throw std::runtime_error(message);
+    return p;
 }
 
 // Bytes of one kv-head's block tile in one arena.

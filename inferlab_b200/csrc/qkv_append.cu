@@ -297,7 +297,7 @@ extern "C" int inferlab_cuda_qkv_project_append(
     return ilb::protect(error, error_capacity, [&] {
         using namespace ilb;
         using namespace ilb::qkv;
-        auto& p = checked_pool(pool);
+        auto& p = checked_wide_pool(pool, "projection does not append to a 4-bit pool");
         if (tokens == 0) return;
         if (hidden == nullptr || weights == nullptr || row_sequences == nullptr ||
             positions == nullptr || block_tables == nullptr || q_out == nullptr) {

@@ -1,0 +1,439 @@
+// rotary_append.cu - token rows into the paged pool with the position rotation
+// applied on the way, and rows read back.
+//   K8 rotary_append_kernel: Q rows rotated to q_out; K rows rotated, V rows
+//      as they are, rounded to the pool type (or quantised, kv4.cuh) and
+//      written at (table[pos / block_tokens], pos % block_tokens).
+//   K9 gather_rows_kernel: the rows at given (sequence, position) pairs, or of
+//      one sequence's first tokens, as [rows][kv_heads][head_dim].
+// The reference appends rows as the projection leaves them (PagedKvPool::append,
+// worker/cpp/inferlab_runtime.cpp:713-767; its positions are learned vectors
+// added to the hidden state) and has no quantised cache.
+//
+// Rotation of the pair (a, b) at a position with (cos, sin):
+// (a cos - b sin, b cos + a sin), each product and sum rounded to fp32 once,
+// then the result rounded once to the stored type. Pairs are (i, i + R / 2), or
+// (2 i, 2 i + 1) when interleaved, over the first R = rotary_dim dims.
+#include "common.cuh"
+#include "internal.cuh"
+#include "kv4.cuh"
+#include "pool.cuh"
+
+#include "../../include/inferlab_attention.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace ilb {
+namespace {
+
+struct AppendParams {
+    const void* queries;
+    const void* keys;
+    const void* values;
+    std::uint64_t q_stride, k_stride, v_stride;  // elements between token rows
+    std::uint32_t q_heads, kv_heads, head_dim;
+    const float* cos_sin;  // [positions][rotary_dim]: cosines, then sines
+    std::uint64_t cos_sin_positions;  // no limit without rotation
+    std::uint32_t rotary_dim;
+    bool interleaved;
+    bool padded_rows;  // sequence -1 is a padded row, not an error
+    const std::int32_t* row_sequences;
+    const std::int32_t* positions;
+    const std::int32_t* tables;
+    std::uint32_t num_seqs, max_blocks, block_tokens;
+    std::uint64_t num_blocks;
+    void* q_out;
+    unsigned char* key_arena;  // 4-bit pools: the packed arena
+    unsigned char* value_arena;
+    std::uint32_t* error_word;
+};
+
+// Where a row goes: block id and slot, or -1 when the row is to be skipped
+// (a padded row, sequence -1, without an error).
+struct Place {
+    std::int32_t block;
+    std::uint32_t slot;
+    std::int32_t position;
+};
+
+__device__ __forceinline__ Place find_place(std::int32_t seq, std::int32_t pos,
+                                            const std::int32_t* tables, std::uint32_t num_seqs,
+                                            std::uint32_t max_blocks, std::uint32_t block_tokens,
+                                            std::uint64_t num_blocks, std::uint64_t positions,
+                                            bool padded_rows, std::uint32_t& error) {
+    error = 0;
+    if (padded_rows && seq == -1) return Place{-1, 0, 0};
+    if (seq < 0 || static_cast<std::uint32_t>(seq) >= num_seqs || pos < 0 ||
+        static_cast<std::uint64_t>(pos) >= positions ||
+        static_cast<std::uint32_t>(pos) / block_tokens >= max_blocks) {
+        error = kErrPosition;
+        return Place{-1, 0, 0};
+    }
+    const std::int32_t block = tables[static_cast<std::size_t>(seq) * max_blocks +
+                                      static_cast<std::uint32_t>(pos) / block_tokens];
+    if (block < 0 || static_cast<std::uint64_t>(block) >= num_blocks) {
+        error = kErrBadBlock;
+        return Place{-1, 0, 0};
+    }
+    return Place{block, static_cast<std::uint32_t>(pos) % block_tokens, pos};
+}
+
+// Dim d of a head's row, rotated. `angles`: the position's [rotary_dim] row.
+template <typename RowT>
+__device__ __forceinline__ float rotated(const RowT* head, std::uint32_t d, const float* angles,
+                                         std::uint32_t rotary_dim, bool interleaved) {
+    const float x = Storage<RowT>::to_float(head[d]);
+    if (d >= rotary_dim) return x;
+    const std::uint32_t half = rotary_dim / 2;
+    const std::uint32_t pair = interleaved ? d / 2 : (d < half ? d : d - half);
+    const bool first = interleaved ? d % 2 == 0 : d < half;
+    const std::uint32_t other = interleaved ? (first ? d + 1 : d - 1) : (first ? d + half : d - half);
+    const float y = Storage<RowT>::to_float(head[other]);
+    const float c = angles[pair], s = angles[half + pair];
+    return first ? __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s))
+                 : __fadd_rn(__fmul_rn(x, c), __fmul_rn(y, s));
+}
+
+constexpr int kRowThreads = 256;
+
+// Any shape: one CTA per token row, elements (8-dim units in a 4-bit pool)
+// spread over its threads. The row is checked before any of it is written,
+// and the second pass finds it in L1.
+template <typename RowT, typename PoolT, typename OutT, bool kFourBit>
+__global__ void __launch_bounds__(kRowThreads) rotary_append_kernel(const AppendParams p) {
+    const std::size_t row = blockIdx.x;
+    std::uint32_t error = 0;
+    const Place place = find_place(p.row_sequences[row], p.positions[row], p.tables, p.num_seqs,
+                                   p.max_blocks, p.block_tokens, p.num_blocks, p.cos_sin_positions,
+                                   p.padded_rows, error);
+    if (error != 0 || place.block < 0) {
+        if (error != 0 && threadIdx.x == 0) flag_error(p.error_word, error);
+        return;
+    }
+    const float* angles = p.cos_sin + static_cast<std::size_t>(place.position) * p.rotary_dim;
+    const RowT* key_row = static_cast<const RowT*>(p.keys) + row * p.k_stride;
+    const RowT* value_row = static_cast<const RowT*>(p.values) + row * p.v_stride;
+    const std::uint32_t d = p.head_dim;
+
+    if constexpr (kFourBit) {
+        const std::uint32_t per_head = d / 8;
+        const std::uint32_t units = p.kv_heads * per_head;
+        const std::size_t tile_size = kv4::tile_bytes(d);
+        const std::size_t tiles_per_head = p.block_tokens / kv4::kTileTokens;
+        unsigned char* tile0 = p.key_arena +
+            (static_cast<std::size_t>(place.block) * p.kv_heads * tiles_per_head + place.slot / kv4::kTileTokens) * tile_size;
+        const int slot = static_cast<int>(place.slot % kv4::kTileTokens);
+        for (int pass = 0; pass < 2; ++pass) {
+            bool any_bad = false;
+            for (std::uint32_t first = 0; first < 2 * units; first += blockDim.x) {
+                // Whole octets are live or not (units is a multiple of 8).
+                const std::uint32_t at = first + threadIdx.x;
+                const bool live = at < 2 * units;
+                const bool is_value = live && at >= units;
+                const std::uint32_t unit = live ? (is_value ? at - units : at) : 0;
+                const std::uint32_t head = unit / per_head, u = unit % per_head;
+                float x[8];
+                const RowT* src = (is_value ? value_row : key_row) + static_cast<std::size_t>(head) * d;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float v = is_value ? Storage<RowT>::to_float(src[8 * u + i])
+                                             : rotated(src, 8 * u + i, angles, p.rotary_dim, p.interleaved);
+                    x[i] = Storage<PoolT>::to_float(Storage<PoolT>::from_float(v));
+                }
+                __half2 pair;
+                bool bad;
+                const std::uint32_t word = kv4::quantise(x, pair, bad);
+                any_bad |= live && bad;
+                if (pass == 1 && live) {
+                    unsigned char* tile = tile0 + head * tiles_per_head * tile_size;
+                    const int dd = static_cast<int>(d), uu = static_cast<int>(u);
+                    *reinterpret_cast<std::uint32_t*>(
+                        tile + (is_value ? kv4::value_word(dd, slot, uu) : kv4::key_word(dd, slot, uu))) = word;
+                    if (u % 8 == 0) {
+                        *reinterpret_cast<__half2*>(tile + kv4::pair_at(dd, slot, uu / 8, is_value)) = pair;
+                    }
+                }
+            }
+            if (pass == 0 && __syncthreads_or(any_bad)) {
+                if (threadIdx.x == 0) flag_error(p.error_word, kErrNonFinite);
+                return;
+            }
+        }
+    } else {
+        const std::size_t width = static_cast<std::size_t>(p.kv_heads) * d;
+        bool bad = false;
+        for (std::size_t i = threadIdx.x; i < width; i += blockDim.x) {
+            const std::uint32_t head = i / d, dim = i % d;
+            const float k = rotated(key_row + static_cast<std::size_t>(head) * d, dim, angles, p.rotary_dim, p.interleaved);
+            bad |= !isfinite(Storage<PoolT>::to_float(Storage<PoolT>::from_float(k)));
+            bad |= !isfinite(Storage<PoolT>::to_float(Storage<PoolT>::from_float(Storage<RowT>::to_float(value_row[i]))));
+        }
+        if (__syncthreads_or(bad)) {
+            if (threadIdx.x == 0) flag_error(p.error_word, kErrNonFinite);
+            return;
+        }
+        for (std::size_t i = threadIdx.x; i < width; i += blockDim.x) {
+            const std::uint32_t head = i / d, dim = i % d;
+            const std::size_t dst =
+                ((static_cast<std::size_t>(place.block) * p.kv_heads + head) * p.block_tokens + place.slot) * d + dim;
+            const float k = rotated(key_row + static_cast<std::size_t>(head) * d, dim, angles, p.rotary_dim, p.interleaved);
+            reinterpret_cast<PoolT*>(p.key_arena)[dst] = Storage<PoolT>::from_float(k);
+            reinterpret_cast<PoolT*>(p.value_arena)[dst] = Storage<PoolT>::from_float(Storage<RowT>::to_float(value_row[i]));
+        }
+    }
+    if (p.queries != nullptr) {
+        const RowT* q_row = static_cast<const RowT*>(p.queries) + row * p.q_stride;
+        const std::size_t width = static_cast<std::size_t>(p.q_heads) * d;
+        OutT* out = static_cast<OutT*>(p.q_out) + row * width;
+        for (std::size_t i = threadIdx.x; i < width; i += blockDim.x) {
+            out[i] = Storage<OutT>::from_float(rotated(q_row + i / d * d, static_cast<std::uint32_t>(i % d), angles,
+                                                       p.rotary_dim, p.interleaved));
+        }
+    }
+}
+
+struct GatherParams {
+    const unsigned char* key_arena;
+    const unsigned char* value_arena;
+    const std::int32_t* row_sequences;  // null: sequence 0, position = row
+    const std::int32_t* positions;
+    const std::int32_t* tables;
+    std::uint32_t num_seqs, max_blocks, block_tokens, kv_heads, head_dim;
+    std::uint64_t num_blocks;
+    void* keys_out;
+    void* values_out;
+    std::uint32_t* error_word;
+};
+
+// One CTA per row. Words of the pool's own element type are copied bit for
+// bit; a 4-bit pool's codes are widened and rounded to its row type T,
+// saturating at T's largest finite value.
+template <typename T, bool kFourBit>
+__global__ void __launch_bounds__(kRowThreads) gather_rows_kernel(const GatherParams p) {
+    const std::size_t row = blockIdx.x;
+    std::uint32_t error = 0;
+    const Place place = find_place(p.row_sequences != nullptr ? p.row_sequences[row] : 0,
+                                   p.positions != nullptr ? p.positions[row] : static_cast<std::int32_t>(row),
+                                   p.tables, p.num_seqs, p.max_blocks, p.block_tokens, p.num_blocks,
+                                   ~0ull, p.row_sequences != nullptr, error);
+    if (place.block < 0) {
+        if (error != 0 && threadIdx.x == 0) flag_error(p.error_word, error);
+        return;
+    }
+    const std::uint32_t d = p.head_dim;
+    const std::size_t width = static_cast<std::size_t>(p.kv_heads) * d;
+    T* keys = static_cast<T*>(p.keys_out) + row * width;
+    T* values = static_cast<T*>(p.values_out) + row * width;
+    if constexpr (kFourBit) {
+        const float most = std::is_same<T, __half>::value ? 65504.0f : 3.3895313892515355e38f;
+        const std::size_t tiles_per_head = p.block_tokens / kv4::kTileTokens;
+        const int slot = static_cast<int>(place.slot % kv4::kTileTokens);
+        for (std::size_t i = threadIdx.x; i < 2 * width / 8; i += blockDim.x) {
+            const bool is_value = i >= width / 8;
+            const std::size_t unit = is_value ? i - width / 8 : i;
+            const std::size_t head = unit / (d / 8);
+            const int u = static_cast<int>(unit % (d / 8)), dd = static_cast<int>(d);
+            const unsigned char* tile = p.key_arena +
+                ((static_cast<std::size_t>(place.block) * p.kv_heads + head) * tiles_per_head +
+                 place.slot / kv4::kTileTokens) * kv4::tile_bytes(dd);
+            const std::uint32_t word = *reinterpret_cast<const std::uint32_t*>(
+                tile + (is_value ? kv4::value_word(dd, slot, u) : kv4::key_word(dd, slot, u)));
+            const float2 pair = kv4::load_pair(tile, kv4::pair_at(dd, slot, u / 8, is_value));
+            T* out = (is_value ? values : keys) + unit * 8;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                out[n] = Storage<T>::from_float(fminf(fmaxf(kv4::code_value(word, n, pair), -most), most));
+            }
+        }
+    } else {
+        for (std::size_t i = threadIdx.x; i < width; i += blockDim.x) {
+            const std::size_t src =
+                ((static_cast<std::size_t>(place.block) * p.kv_heads + i / d) * p.block_tokens + place.slot) * d + i % d;
+            keys[i] = reinterpret_cast<const T*>(p.key_arena)[src];
+            values[i] = reinterpret_cast<const T*>(p.value_arena)[src];
+        }
+    }
+}
+
+template <typename RowT, typename PoolT, typename OutT>
+void launch_rotary(const AppendParams& a, std::uint64_t rows, bool four_bit, cudaStream_t s) {
+    const unsigned grid = static_cast<unsigned>(rows);
+    if constexpr (!std::is_same<PoolT, float>::value) {
+        if (four_bit) {
+            rotary_append_kernel<RowT, PoolT, OutT, true><<<grid, kRowThreads, 0, s>>>(a);
+            return;
+        }
+    }
+    rotary_append_kernel<RowT, PoolT, OutT, false><<<grid, kRowThreads, 0, s>>>(a);
+}
+
+template <typename PoolT>
+void select_rotary(const AppendParams& a, std::uint64_t rows, std::uint32_t row_dtype,
+                   std::uint32_t out_dtype, bool four_bit, cudaStream_t s) {
+    if constexpr (std::is_same<PoolT, float>::value) {
+        launch_rotary<float, float, float>(a, rows, false, s);
+    } else if (row_dtype == kFp32) {
+        if (out_dtype == kFp32) launch_rotary<float, PoolT, float>(a, rows, four_bit, s);
+        else launch_rotary<float, PoolT, PoolT>(a, rows, four_bit, s);
+    } else {
+        if (out_dtype == kFp32) launch_rotary<PoolT, PoolT, float>(a, rows, four_bit, s);
+        else launch_rotary<PoolT, PoolT, PoolT>(a, rows, four_bit, s);
+    }
+}
+
+void run_gather_rows(InferlabCudaKvPool& p, const std::int32_t* row_sequences,
+                     const std::int32_t* positions, std::uint64_t rows, const std::int32_t* tables,
+                     std::uint32_t num_seqs, std::uint32_t max_blocks, void* keys_out,
+                     void* values_out, cudaStream_t s) {
+    GatherParams g{};
+    g.key_arena = static_cast<const unsigned char*>(p.key_arena);
+    g.value_arena = static_cast<const unsigned char*>(p.value_arena);
+    g.row_sequences = row_sequences;
+    g.positions = positions;
+    g.tables = tables;
+    g.num_seqs = num_seqs;
+    g.max_blocks = max_blocks;
+    g.block_tokens = p.block_tokens;
+    g.kv_heads = p.kv_heads;
+    g.head_dim = p.head_dim;
+    g.num_blocks = p.num_blocks;
+    g.keys_out = keys_out;
+    g.values_out = values_out;
+    g.error_word = p.error_word;
+    const unsigned grid = static_cast<unsigned>(rows);
+    if (p.dtype == kFp32) {
+        gather_rows_kernel<float, false><<<grid, kRowThreads, 0, s>>>(g);
+    } else if (p.dtype == kF16) {
+        if (p.kv_bits != 0) gather_rows_kernel<__half, true><<<grid, kRowThreads, 0, s>>>(g);
+        else gather_rows_kernel<__half, false><<<grid, kRowThreads, 0, s>>>(g);
+    } else {
+        if (p.kv_bits != 0) gather_rows_kernel<__nv_bfloat16, true><<<grid, kRowThreads, 0, s>>>(g);
+        else gather_rows_kernel<__nv_bfloat16, false><<<grid, kRowThreads, 0, s>>>(g);
+    }
+    cuda_check(cudaGetLastError(), "gather rows launch");
+}
+
+bool overlaps(const void* a, std::size_t a_bytes, const void* b, std::size_t b_bytes) {
+    const auto a0 = reinterpret_cast<std::uintptr_t>(a), b0 = reinterpret_cast<std::uintptr_t>(b);
+    return a0 < b0 + b_bytes && b0 < a0 + a_bytes;
+}
+
+}  // namespace
+
+void launch_rotary_append(InferlabCudaKvPool& p, const InferlabCudaRotaryAppend& c,
+                          bool padded_rows, cudaStream_t stream) {
+    AppendParams a{};
+    a.queries = c.q_heads != 0 ? c.queries : nullptr;
+    a.keys = c.key_rows;
+    a.values = c.value_rows;
+    a.q_stride = c.query_stride;
+    a.k_stride = c.key_stride;
+    a.v_stride = c.value_stride;
+    a.q_heads = c.q_heads;
+    a.kv_heads = p.kv_heads;
+    a.head_dim = p.head_dim;
+    a.cos_sin = c.cos_sin;
+    a.cos_sin_positions = c.rotary_dim != 0 ? c.cos_sin_positions : ~0ull;
+    a.rotary_dim = c.rotary_dim;
+    a.interleaved = c.interleaved != 0;
+    a.padded_rows = padded_rows;
+    a.row_sequences = c.row_sequences;
+    a.positions = c.positions;
+    a.tables = c.block_tables;
+    a.num_seqs = c.num_seqs;
+    a.max_blocks = c.max_blocks_per_seq;
+    a.block_tokens = p.block_tokens;
+    a.num_blocks = p.num_blocks;
+    a.q_out = c.q_out;
+    a.key_arena = static_cast<unsigned char*>(p.key_arena);
+    a.value_arena = static_cast<unsigned char*>(p.value_arena);
+    a.error_word = p.error_word;
+    const bool four_bit = p.kv_bits != 0;
+    if (p.dtype == kFp32) {
+        select_rotary<float>(a, c.rows, c.row_dtype, c.q_out_dtype, four_bit, stream);
+    } else if (p.dtype == kF16) {
+        select_rotary<__half>(a, c.rows, c.row_dtype, c.q_out_dtype, four_bit, stream);
+    } else {
+        select_rotary<__nv_bfloat16>(a, c.rows, c.row_dtype, c.q_out_dtype, four_bit, stream);
+    }
+    cuda_check(cudaGetLastError(), "rotary append launch");
+}
+
+void launch_kv4_gather(InferlabCudaKvPool& p, const std::int32_t* block_table, std::uint64_t tokens,
+                       void* keys_out, void* values_out, cudaStream_t stream) {
+    const std::uint32_t blocks = static_cast<std::uint32_t>((tokens + p.block_tokens - 1) / p.block_tokens);
+    run_gather_rows(p, nullptr, nullptr, tokens, block_table, 1, blocks, keys_out, values_out, stream);
+}
+
+}  // namespace ilb
+
+extern "C" int inferlab_cuda_kv_append_rotary(InferlabCudaKvPool* pool,
+                                              const InferlabCudaRotaryAppend* call, void* stream,
+                                              char* error, std::size_t error_capacity) {
+    return ilb::protect(error, error_capacity, [&] {
+        using namespace ilb;
+        auto& p = checked_pool(pool);
+        if (call == nullptr) throw std::runtime_error("rotary append description is null");
+        const InferlabCudaRotaryAppend& c = *call;
+        if (c.rows == 0) return;
+        if (c.key_rows == nullptr || c.value_rows == nullptr || c.row_sequences == nullptr ||
+            c.positions == nullptr || c.block_tables == nullptr ||
+            (c.q_heads != 0 && (c.queries == nullptr || c.q_out == nullptr)) ||
+            (c.rotary_dim != 0 && c.cos_sin == nullptr)) {
+            throw std::runtime_error("rotary append pointer is null");
+        }
+        if (c.row_dtype != kFp32 && c.row_dtype != p.dtype) {
+            throw std::runtime_error("paged KV row dtype must be FP32 or the pool dtype");
+        }
+        if (c.q_heads != 0 && c.q_out_dtype != kFp32 && c.q_out_dtype != p.dtype) {
+            throw std::runtime_error("rotary append query output dtype must be FP32 or the pool dtype");
+        }
+        if (c.rotary_dim % 2 != 0 || c.rotary_dim > p.head_dim) {
+            throw std::runtime_error("rotary_dim must be even and at most head_dim");
+        }
+        if (c.num_seqs == 0 || c.max_blocks_per_seq == 0) throw std::runtime_error("paged KV block table is empty");
+        if (c.rows > 0x7FFFFFFFull) throw std::runtime_error("paged KV append row count is too large");
+        const std::uint64_t kv_width = static_cast<std::uint64_t>(p.kv_heads) * p.head_dim;
+        const std::uint64_t q_width = static_cast<std::uint64_t>(c.q_heads) * p.head_dim;
+        if (kv_width > 0x7FFFFFFFull || q_width > 0x7FFFFFFFull) throw std::runtime_error("rotary append rows are too wide");
+        if (c.q_heads != 0) {
+            // A dim's rotation reads its partner dim, which another thread may
+            // already have replaced if the output were the input.
+            const std::size_t in = c.row_dtype == kFp32 ? 4 : 2, out = c.q_out_dtype == kFp32 ? 4 : 2;
+            const std::size_t out_bytes = checked_mul(checked_mul(c.rows, q_width, "rotary append is too large"), out,
+                                                      "rotary append is too large");
+            const auto span = [&](std::uint64_t stride, std::uint64_t width) {
+                return (checked_mul(c.rows - 1, stride, "rotary append is too large") + width) * in;
+            };
+            if (overlaps(c.q_out, out_bytes, c.queries, span(c.query_stride, q_width)) ||
+                overlaps(c.q_out, out_bytes, c.key_rows, span(c.key_stride, kv_width)) ||
+                overlaps(c.q_out, out_bytes, c.value_rows, span(c.value_stride, kv_width))) {
+                throw std::runtime_error("rotary append query output overlaps its input rows");
+            }
+        }
+        DeviceGuard guard(p.device);
+        launch_rotary_append(p, c, true, static_cast<cudaStream_t>(stream));
+    });
+}
+
+extern "C" int inferlab_cuda_kv_gather_rows(InferlabCudaKvPool* pool, const std::int32_t* row_sequences,
+                                            const std::int32_t* positions, std::uint64_t rows,
+                                            const std::int32_t* block_tables, std::uint32_t num_seqs,
+                                            std::uint32_t max_blocks_per_seq, void* keys_out,
+                                            void* values_out, void* stream, char* error,
+                                            std::size_t error_capacity) {
+    return ilb::protect(error, error_capacity, [&] {
+        using namespace ilb;
+        auto& p = checked_pool(pool);
+        if (rows == 0) return;
+        if (row_sequences == nullptr || positions == nullptr || block_tables == nullptr ||
+            keys_out == nullptr || values_out == nullptr) {
+            throw std::runtime_error("paged KV gather pointer is null");
+        }
+        if (num_seqs == 0 || max_blocks_per_seq == 0) throw std::runtime_error("paged KV block table is empty");
+        if (rows > 0x7FFFFFFFull) throw std::runtime_error("paged KV gather is too long");
+        DeviceGuard guard(p.device);
+        run_gather_rows(p, row_sequences, positions, rows, block_tables, num_seqs, max_blocks_per_seq,
+                        keys_out, values_out, static_cast<cudaStream_t>(stream));
+    });
+}

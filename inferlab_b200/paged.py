@@ -61,17 +61,27 @@ def _require(tensor: torch.Tensor, name: str, dtype, device: int) -> torch.Tenso
 
 
 class CudaKvPool:
-    """HBM block pool: arenas [num_blocks][kv_heads][block_tokens][head_dim]."""
+    """HBM block pool: arenas [num_blocks][kv_heads][block_tokens][head_dim].
+
+    kv_bits=4 holds the rows in 4 bits (inferlab_cuda_pool_create_kv4): dtype is
+    then the 16-bit type that rows are rounded to before they are quantised and
+    that queries, outputs and gathered rows have; block_tokens is a multiple of
+    16 and head_dim 64 or 128. append, append_rotary, gather, gather_rows,
+    decode, prefill, output_project and copy_blocks work on such a pool."""
 
     def __init__(self, device: int, dtype: int, num_blocks: int, block_tokens: int,
-                 kv_heads: int, head_dim: int):
+                 kv_heads: int, head_dim: int, kv_bits: int | None = None):
         self._lib = _lib.lib()
+        if kv_bits not in (None, 4):
+            raise AttentionError("paged KV kv_bits must be None or 4")
+        create = (self._lib.inferlab_cuda_pool_create if kv_bits is None
+                  else self._lib.inferlab_cuda_pool_create_kv4)
         handle = ctypes.c_void_p()
         error = _lib.error_buffer()
-        _check(self._lib.inferlab_cuda_pool_create(device, dtype, num_blocks, block_tokens,
-                                                   kv_heads, head_dim, ctypes.byref(handle),
-                                                   error, len(error)), error)
+        _check(create(device, dtype, num_blocks, block_tokens, kv_heads, head_dim,
+                      ctypes.byref(handle), error, len(error)), error)
         self._handle = handle
+        self.kv_bits = kv_bits
         info = _lib.InferlabCudaPoolInfo()
         _check(self._lib.inferlab_cuda_pool_info(handle, ctypes.byref(info), error, len(error)),
                error)
@@ -82,7 +92,10 @@ class CudaKvPool:
         self.kv_heads = info.kv_heads
         self.head_dim = info.head_dim
         self.element_bytes = info.element_bytes
+        self.block_bytes = info.block_bytes
         self.arena_bytes = info.arena_bytes
+        # One token row of K and V over all kv-heads.
+        self.row_bytes = info.block_bytes // info.block_tokens * (1 if kv_bits == 4 else 2)
         self._key_ptr = info.key_arena
         self._value_ptr = info.value_arena
         self._workspaces: dict = {}
@@ -106,7 +119,21 @@ class CudaKvPool:
         self.close()
 
     # -- views ----------------------------------------------------------------
+    @property
+    def arena(self) -> torch.Tensor:
+        """A 4-bit pool's packed arena as bytes [num_blocks][kv_heads][block_tokens / 16][tile]
+        (no copy; valid while the pool lives; the layout is in the C header)."""
+        if self.kv_bits != 4:
+            raise AttentionError("only a 4-bit pool has a packed arena")
+        tiles = self.block_tokens // 16
+        shape = (self.num_blocks, self.kv_heads, tiles,
+                 self.block_bytes // (self.kv_heads * tiles))
+        return torch.as_tensor(_DeviceView(self._key_ptr, shape, "|u1"),
+                               device=f"cuda:{self.device}")
+
     def _arena(self, ptr: int) -> torch.Tensor:
+        if self.kv_bits == 4:
+            raise AttentionError("a 4-bit pool has one packed arena (arena)")
         shape = (self.num_blocks, self.kv_heads, self.block_tokens, self.head_dim)
         view = torch.as_tensor(_DeviceView(ptr, shape, _TYPESTR[self.dtype]),
                                device=f"cuda:{self.device}")
@@ -152,6 +179,83 @@ class CudaKvPool:
             self._handle, _vp(key_rows), _vp(value_rows), row_dtype, _vp(row_sequences),
             _vp(positions), rows, _vp(block_tables), block_tables.shape[-1],
             _stream_handle(dev, stream), error, len(error)), error)
+
+    def _rows(self, tensor: torch.Tensor, name: str, dtype, heads: int | None) -> int:
+        """Checks token rows [n][heads][head_dim], heads and dims contiguous (a view of a wider
+        projection output is fine); returns the elements between rows."""
+        if not isinstance(tensor, torch.Tensor) or tensor.device.type != "cuda" or \
+                tensor.device.index != self.device:
+            raise AttentionError(f"{name} must live on cuda:{self.device}")
+        if tensor.dtype != dtype:
+            raise AttentionError(f"{name} must have dtype {dtype}")
+        if tensor.dim() != 3 or tensor.shape[2] != self.head_dim or \
+                (heads is not None and tensor.shape[1] != heads):
+            raise AttentionError("paged KV append shapes do not match the pool")
+        if tensor.numel() and (tensor.stride(2) != 1 or
+                               (tensor.shape[1] > 1 and tensor.stride(1) != self.head_dim)):
+            raise AttentionError(f"{name} must have contiguous heads")
+        return tensor.stride(0)
+
+    def append_rotary(self, queries: torch.Tensor | None, key_rows: torch.Tensor,
+                      value_rows: torch.Tensor, cos_sin: torch.Tensor | None,
+                      row_sequences: torch.Tensor, positions: torch.Tensor,
+                      block_tables: torch.Tensor, interleaved: bool = False,
+                      q_out: torch.Tensor | None = None, stream=None) -> torch.Tensor | None:
+        """append with the position rotation on the way: Q and K rows are rotated by row
+        positions[r] of cos_sin (fp32 [positions][rotary_dim]: cosines, then sines; None for no
+        rotation), K and V go to the pool at (row_sequences[r], positions[r]), and the rotated Q is
+        returned (queries None: nothing). Pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) when
+        interleaved. Rows [n][heads][head_dim] are fp32 or the pool's type and may be views of one
+        projection output; q_out (default: like the queries) may be either type. Rows of sequence
+        -1 are padding: skipped, their q_out rows left as they were
+        (inferlab_cuda_kv_append_rotary)."""
+        dev = self.device
+        dtype = key_rows.dtype
+        if dtype not in (torch.float32, TORCH_DTYPES[self.dtype]):
+            raise AttentionError("paged KV row dtype must be FP32 or the pool dtype")
+        call = _lib.InferlabCudaRotaryAppend()
+        call.key_stride = self._rows(key_rows, "key_rows", dtype, self.kv_heads)
+        call.value_stride = self._rows(value_rows, "value_rows", dtype, self.kv_heads)
+        rows = key_rows.shape[0]
+        _require(row_sequences, "row_sequences", torch.int32, dev)
+        _require(positions, "positions", torch.int32, dev)
+        _require(block_tables, "block_tables", torch.int32, dev)
+        if value_rows.shape[0] != rows or row_sequences.numel() != rows or \
+                positions.numel() != rows or block_tables.dim() != 2:
+            raise AttentionError("paged KV append shapes do not match the pool")
+        if cos_sin is not None:
+            _require(cos_sin, "cos_sin", torch.float32, dev)
+            if cos_sin.dim() != 2:
+                raise AttentionError("cos_sin must be [positions][rotary_dim]")
+            call.cos_sin = cos_sin.data_ptr()
+            call.cos_sin_positions, call.rotary_dim = cos_sin.shape
+        if queries is not None:
+            call.query_stride = self._rows(queries, "queries", dtype, None)
+            if queries.shape[0] != rows:
+                raise AttentionError("paged KV append shapes do not match the pool")
+            if q_out is None:
+                q_out = torch.empty(queries.shape, dtype=dtype, device=queries.device)
+            _require(q_out, "q_out", None, dev)
+            if q_out.shape != queries.shape or \
+                    q_out.dtype not in (torch.float32, TORCH_DTYPES[self.dtype]):
+                raise AttentionError("q_out must be shaped like the queries, FP32 or the pool dtype")
+            call.queries, call.q_out = queries.data_ptr(), q_out.data_ptr()
+            call.q_heads = queries.shape[1]
+            call.q_out_dtype = KV_FP32 if q_out.dtype == torch.float32 else self.dtype
+        elif q_out is not None:
+            raise AttentionError("q_out needs queries")
+        call.key_rows, call.value_rows = key_rows.data_ptr(), value_rows.data_ptr()
+        call.row_dtype = KV_FP32 if dtype == torch.float32 else self.dtype
+        call.interleaved = 1 if interleaved else 0
+        call.row_sequences, call.positions = row_sequences.data_ptr(), positions.data_ptr()
+        call.rows = rows
+        call.block_tables = block_tables.data_ptr()
+        call.num_seqs, call.max_blocks_per_seq = block_tables.shape
+        error = _lib.error_buffer()
+        _check(self._lib.inferlab_cuda_kv_append_rotary(
+            self._handle, ctypes.byref(call), _stream_handle(dev, stream), error, len(error)),
+            error)
+        return q_out
 
     def project_append(self, hidden: torch.Tensor, weights: torch.Tensor, q_heads: int,
                        row_sequences: torch.Tensor, positions: torch.Tensor,
@@ -232,14 +336,41 @@ class CudaKvPool:
             _stream_handle(dev, stream), error, len(error)), error)
         return keys, values
 
-    def workspace_size(self, num_seqs: int, q_heads: int, max_context_len: int) -> int:
+    def gather_rows(self, row_sequences: torch.Tensor, positions: torch.Tensor,
+                    block_tables: torch.Tensor, stream=None):
+        """The rows at (row_sequences[r], positions[r]): K and V [rows][kv_heads][head_dim] in the
+        pool's type (a 4-bit pool's row type). Rows of sequence -1 are padding and left unset
+        (inferlab_cuda_kv_gather_rows)."""
+        dev = self.device
+        _require(row_sequences, "row_sequences", torch.int32, dev)
+        _require(positions, "positions", torch.int32, dev)
+        _require(block_tables, "block_tables", torch.int32, dev)
+        rows = row_sequences.numel()
+        if positions.numel() != rows or block_tables.dim() != 2:
+            raise AttentionError("paged KV gather shapes do not match")
+        keys = torch.empty((rows, self.kv_heads, self.head_dim), dtype=TORCH_DTYPES[self.dtype],
+                           device=f"cuda:{dev}")
+        values = torch.empty_like(keys)
+        error = _lib.error_buffer()
+        _check(self._lib.inferlab_cuda_kv_gather_rows(
+            self._handle, _vp(row_sequences), _vp(positions), rows, _vp(block_tables),
+            block_tables.shape[0], block_tables.shape[1], _vp(keys), _vp(values),
+            _stream_handle(dev, stream), error, len(error)), error)
+        return keys, values
+
+    def workspace_size(self, num_seqs: int, q_heads: int, max_context_len: int,
+                       max_query_count: int = 1) -> int:
+        if self.kv_bits == 4:
+            return int(self._lib.inferlab_cuda_kv4_workspace_size(
+                self._handle, num_seqs, q_heads, max_query_count, max_context_len))
         return int(self._lib.inferlab_cuda_paged_decode_workspace_size(
             self._handle, num_seqs, q_heads, max_context_len))
 
     def make_workspace(self, num_seqs: int, q_heads: int, max_context_len: int,
-                       stream=None) -> torch.Tensor:
-        """A zero-initialised decode workspace for this batch shape."""
-        size = max(16, self.workspace_size(num_seqs, q_heads, max_context_len))
+                       stream=None, max_query_count: int = 1) -> torch.Tensor:
+        """A zero-initialised decode workspace for this batch shape (max_query_count: the prefill
+        of a 4-bit pool)."""
+        size = max(16, self.workspace_size(num_seqs, q_heads, max_context_len, max_query_count))
         ws = torch.empty(size, dtype=torch.uint8, device=f"cuda:{self.device}")
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_paged_decode_workspace_init(
@@ -274,8 +405,13 @@ class CudaKvPool:
                context_lens: torch.Tensor, max_context_len: int | None = None,
                out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
                stream=None) -> torch.Tensor:
-        """One decode step: queries [num_seqs][q_heads][head_dim] fp32 -> fp32 output."""
+        """One decode step: queries [num_seqs][q_heads][head_dim] fp32 -> fp32 output. A 4-bit
+        pool also takes queries of its row type and returns the queries' type; its context length
+        0 is a slot without a sequence, whose output row is zero (inferlab_cuda_kv4_decode)."""
         dev = self.device
+        if self.kv_bits == 4:
+            return self._kv4_decode(queries, block_tables, context_lens, max_context_len, out,
+                                    workspace, stream)
         _require(queries, "queries", torch.float32, dev)
         _require(block_tables, "block_tables", torch.int32, dev)
         _require(context_lens, "context_lens", torch.int32, dev)
@@ -380,9 +516,17 @@ class CudaKvPool:
     def prefill(self, queries: torch.Tensor, block_tables: torch.Tensor,
                 query_starts: torch.Tensor, query_counts: torch.Tensor,
                 query_offsets: torch.Tensor, max_query_count: int,
-                out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
-        """Causal (chunked) prefill of segments whose K/V are already in the pool."""
+                out: torch.Tensor | None = None, stream=None,
+                max_context_len: int | None = None,
+                workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """Causal (chunked) prefill of segments whose K/V are already in the pool. A 4-bit pool
+        returns the queries' type; max_context_len (default: what the tables can hold) bounds its
+        query_starts + query_counts and workspace is as for decode (inferlab_cuda_kv4_prefill)."""
         dev = self.device
+        if self.kv_bits == 4:
+            return self._kv4_prefill(queries, block_tables, query_starts, query_counts,
+                                     query_offsets, max_query_count, out, stream, max_context_len,
+                                     workspace)
         if queries.dtype == torch.float32:
             qtype = KV_FP32
         elif queries.dtype == TORCH_DTYPES[self.dtype]:
@@ -405,6 +549,88 @@ class CudaKvPool:
             _vp(query_starts), _vp(query_counts), _vp(query_offsets), query_starts.numel(),
             q_heads, max_query_count, total, _vp(out), _stream_handle(dev, stream), error,
             len(error)), error)
+        return out
+
+    def _kv4_operands(self, queries, out):
+        """The query / output type code and the output of a 4-bit attention call."""
+        if queries.dtype not in (torch.float32, TORCH_DTYPES[self.dtype]):
+            raise AttentionError("4-bit attention query dtype must be FP32 or the pool's row type")
+        _require(queries, "queries", queries.dtype, self.device)
+        if queries.dim() != 3 or queries.shape[2] != self.head_dim:
+            raise AttentionError("4-bit attention shapes do not match the pool")
+        if out is None:
+            out = torch.empty_like(queries)
+        _require(out, "out", queries.dtype, self.device)
+        if out.shape != queries.shape:
+            raise AttentionError("4-bit attention output must be shaped like the queries")
+        return KV_FP32 if queries.dtype == torch.float32 else self.dtype, out
+
+    def _kv4_workspace(self, num_seqs, q_heads, max_query_count, max_context_len, stream):
+        """The pool's workspace of the stream; a capture gets its own, so that two graphs that
+        are replayed side by side never share one."""
+        used = stream if stream is not None else torch.cuda.current_stream(self.device)
+        with torch.cuda.stream(used):
+            if torch.cuda.is_current_stream_capturing():
+                return self.make_workspace(num_seqs, q_heads, max_context_len, used,
+                                           max_query_count)
+            need = self.workspace_size(num_seqs, q_heads, max_context_len, max_query_count)
+            ws = self._workspaces.get(used.cuda_stream)
+            if ws is None or ws.numel() < need:
+                ws = self.make_workspace(num_seqs, q_heads, max_context_len, used,
+                                         max_query_count)
+                self._workspaces[used.cuda_stream] = ws
+            return ws
+
+    def _kv4_decode(self, queries, block_tables, context_lens, max_context_len, out, workspace,
+                    stream):
+        dev = self.device
+        query_type, out = self._kv4_operands(queries, out)
+        _require(block_tables, "block_tables", torch.int32, dev)
+        _require(context_lens, "context_lens", torch.int32, dev)
+        num_seqs, q_heads, _ = queries.shape
+        if context_lens.numel() != num_seqs or block_tables.dim() != 2 or \
+                block_tables.shape[0] != num_seqs:
+            raise AttentionError("4-bit attention shapes do not match the pool")
+        if num_seqs == 0:
+            return out
+        if max_context_len is None:
+            max_context_len = max(1, int(context_lens.max().item()))
+        if workspace is None:
+            workspace = self._kv4_workspace(num_seqs, q_heads, 1, max_context_len, stream)
+        _require(workspace, "workspace", torch.uint8, dev)
+        error = _lib.error_buffer()
+        _check(self._lib.inferlab_cuda_kv4_decode(
+            self._handle, _vp(queries), query_type, _vp(block_tables), block_tables.shape[1],
+            _vp(context_lens), num_seqs, q_heads, max_context_len, _vp(out), _vp(workspace),
+            workspace.numel(), _stream_handle(dev, stream), error, len(error)), error)
+        return out
+
+    def _kv4_prefill(self, queries, block_tables, query_starts, query_counts, query_offsets,
+                     max_query_count, out, stream, max_context_len, workspace):
+        dev = self.device
+        query_type, out = self._kv4_operands(queries, out)
+        segments = query_starts.numel()
+        for name, t in (("block_tables", block_tables), ("query_starts", query_starts),
+                        ("query_counts", query_counts), ("query_offsets", query_offsets)):
+            _require(t, name, torch.int32, dev)
+        if block_tables.dim() != 2 or block_tables.shape[0] != segments or \
+                query_counts.numel() != segments or query_offsets.numel() != segments:
+            raise AttentionError("4-bit attention shapes do not match the pool")
+        total, q_heads, _ = queries.shape
+        if segments == 0 or total == 0:
+            return out
+        if max_context_len is None:
+            max_context_len = min(block_tables.shape[1] * self.block_tokens, 0x7fffffff)
+        if workspace is None:
+            workspace = self._kv4_workspace(segments, q_heads, max_query_count, max_context_len,
+                                            stream)
+        _require(workspace, "workspace", torch.uint8, dev)
+        error = _lib.error_buffer()
+        _check(self._lib.inferlab_cuda_kv4_prefill(
+            self._handle, _vp(queries), query_type, _vp(block_tables), block_tables.shape[1],
+            _vp(query_starts), _vp(query_counts), _vp(query_offsets), segments, q_heads,
+            max_query_count, total, max_context_len, _vp(out), _vp(workspace), workspace.numel(),
+            _stream_handle(dev, stream), error, len(error)), error)
         return out
 
 

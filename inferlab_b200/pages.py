@@ -46,8 +46,7 @@ class PageManager:
     @classmethod
     def for_pool(cls, pool, prefix_capacity: int = 0) -> "PageManager":
         """A manager of every block of a CudaKvPool."""
-        row = pool.kv_heads * pool.head_dim * 2 * pool.element_bytes
-        return cls(pool.num_blocks, pool.block_tokens, row, prefix_capacity)
+        return cls(pool.num_blocks, pool.block_tokens, pool.row_bytes, prefix_capacity)
 
     def close(self) -> None:
         if self._handle:
