@@ -4,7 +4,7 @@
 // For a query q and the keys it sees, s_t = q . k_t / sqrt(D), p_t = exp(s_t -
 // m), out = sum p_t v_t / sum p_t in one pass over the tokens with a running
 // maximum m. With k = (c - 8) scale + zero per 64 dims,
-//   s   = sum_groups [ scale (q . c) + (zero - 8 scale) (q . 1) ]
+//   s   = sum_groups [ scale (q . c - 8 q . 1) + zero (q . 1) ]
 //   out = sum_t p_t scale_t (c_t - 8) + sum_t p_t zero_t,
 // so both products run on the codes, which mma.sync takes as small exact
 // numbers, and the pairs meet only scores and weights: 4 numbers per 16 tokens
@@ -13,18 +13,22 @@
 //     c 2^-24, in bits 4-7 it is c 2^-20, so a mask is the whole conversion; q
 //     is scaled by a power of two per row (exact) into f16's range, and by 2^-4
 //     where it meets the latter.
-//   output: V codes as bf16, (0x4300 | c) - 136 = c - 8. The weights p scale are
-//     split into two bf16 parts (16 bits together, any range).
+//   output: V codes as f16 c - 8, one mask-or and one subtraction for two, and
+//     the weights p scale as f16, in two parts (22 bits together) for fp32
+//     results. f16's range is kept by what m is: not the largest score but the
+//     largest p scale, kept between 2^10 and 2^15, so that the first part loses
+//     bits only 24 octaves below it and the second 13; l and the zero sums are
+//     in the same unit.
 // The mma computes S^T = K Q^T and O^T = V^T P^T: 16 tokens or dims by 8 query
-// columns, so a GQA group of up to 4 fills the columns with its heads' two
-// parts, one of 5 to 8 takes two products. P^T's operand layout is S^T's result
-// transposed (movmatrix).
+// columns. P^T's operand layout is S^T's result transposed (movmatrix).
 //
 // What bounds it: HBM, (D + D / 8) bytes a token and kv-head (144 at D = 128,
 // 23 bytes a clock and SM), with ~70% of the issue slots behind it. One CTA of
 // four warps per (sequence, kv-head, 8 columns, split); every warp streams its
-// own 16-token tiles (one bulk copy each) through a ring in shared memory, so
-// that the warps never wait for each other before the merge.
+// own 16-token tiles through a ring in shared memory, so that the warps never
+// wait for each other before the merge. The copies are 16-byte cp.async by all
+// lanes: five instructions a tile, where a bulk copy by one lane with its
+// barrier took ~40 issue slots of ~430.
 #include "common.cuh"
 #include "internal.cuh"
 #include "kv4.cuh"
@@ -40,8 +44,9 @@ namespace ilb {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStages = 4;
-constexpr float kRescale = 8.0f;       // log2: weights may grow to 2^8 before the maximum moves
+constexpr int kRing = 3;                // steps in a warp's ring
+constexpr int kStep = 2;               // tiles a warp takes at once
+constexpr float kHeadroom = 10.0f;     // log2: the largest scaled weight starts at 2^10 (below)
 constexpr float kNoScore = -3.0e38f;   // running maximum before any key
 constexpr std::uint32_t kMaxSplits = 256;
 
@@ -64,65 +69,82 @@ struct Kv4Params {
     int tiles_per_split;
     float scale_log2;
     std::uint32_t* ws_count;  // [unit]
-    float* ws_part;           // [unit][split][columns][D + 2]: m, l, o
+    float* ws_part;           // [unit][split]: o [columns][D], then (m, l) per column, padded to [columns][D + 4]
     std::uint32_t* error_word;
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], std::uint32_t a0, std::uint32_t a1,
                                         std::uint32_t a2, std::uint32_t a3, std::uint32_t b0,
                                         std::uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], std::uint32_t a0, std::uint32_t a1,
-                                         std::uint32_t a2, std::uint32_t a3, std::uint32_t b0,
-                                         std::uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// The same onto c0, c1 (one for each column of the lane).
+__device__ __forceinline__ void mma_f16_onto(float (&d)[4], std::uint32_t a0, std::uint32_t a1,
+                                             std::uint32_t a2, std::uint32_t a3, std::uint32_t b0,
+                                             std::uint32_t b1, float c0, float c1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ std::uint32_t transpose8(std::uint32_t x) {
     std::uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ std::uint32_t bf16_pair(float low, float high) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(low, high);
+// Codes as f16 c - 8: bits 0-3 of each half under 2^10's exponent are 1024 + c,
+// bits 4-7 under 2^6's are 64 + c.
+__device__ __forceinline__ std::uint32_t centred(std::uint32_t raw, float bias) {
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&raw), __float2half2_rn(bias));
     return *reinterpret_cast<const std::uint32_t*>(&v);
 }
-// Two codes (bits 0-3 of each half) as bf16 c - 8.
-__device__ __forceinline__ std::uint32_t centred_codes(std::uint32_t nibbles) {
-    std::uint32_t x = (nibbles & 0x000f000fu) | 0x43004300u;
-    __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&x);
-    v = __hsub2(v, __float2bfloat162_rn(136.0f));
-    return *reinterpret_cast<const std::uint32_t*>(&v);
+__device__ __forceinline__ std::uint32_t centred_low(std::uint32_t x) {
+    return centred((x & 0x000f000fu) | 0x64006400u, 1032.0f);
+}
+__device__ __forceinline__ std::uint32_t centred_high(std::uint32_t x) {
+    return centred((x & 0x00f000f0u) | 0x54005400u, 72.0f);
 }
 __device__ __forceinline__ std::uint32_t f16_pair(float low, float high) {
     const __half2 v = __floats2half2_rn(low, high);
     return *reinterpret_cast<const std::uint32_t*>(&v);
+}
+// The (scale, zero) pairs of N neighbouring groups.
+__device__ __forceinline__ void load_pairs(const unsigned char* at, float2 (&pairs)[1]) {
+    pairs[0] = __half22float2(*reinterpret_cast<const __half2*>(at));
+}
+__device__ __forceinline__ void load_pairs(const unsigned char* at, float2 (&pairs)[2]) {
+    const uint2 raw = *reinterpret_cast<const uint2*>(at);
+    pairs[0] = __half22float2(*reinterpret_cast<const __half2*>(&raw.x));
+    pairs[1] = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
 }
 // Token slot (0..7) that sits in row r of an 8-token mma half: r = 2t is token
 // t, r = 2t + 1 token 7 - t. Rows 2t of all t (what four lanes read of V at
 // once) and rows r of neighbouring r (K) then fall on different banks.
 __device__ __forceinline__ int slot_of_row(int r) { return r & 1 ? 7 - (r >> 1) : r >> 1; }
 
-// kHeads4: at most 4 live columns, each twice: columns 4-7 carry the second
-// part of the weights of columns 0-3.
-template <typename RowT, typename QT, int D, bool kHeads4>
+// Up to 8 live query columns, or (kFour) up to 4 that stand twice, so that
+// columns 4-7 carry something else of the same queries:
+//   fp32 queries: the second part of the weights (8 columns: a second product);
+//   16-bit queries, whose outputs are rounded to 2^-12 or 2^-9 anyway, take the
+//   weights in one f16 part (2^-12 each, before they average out), and with
+//   D = 128 columns 4-7 the weights scaled for dims 64-127 instead of 0-63: a
+//   lane then has one value pair per token, and the columns of the other half
+//   of the dims are not used.
+template <typename RowT, typename QT, int D, bool kFour>
 __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4Params p) {
     constexpr int kTile = kv4::tile_bytes(D);
     constexpr int kGroups = D / kv4::kGroup;
     constexpr int kWords = D / 32;  // key words of a lane and token
     constexpr int kMt = D / 16;     // 16-dim tiles of the output
-    constexpr int kCols = kHeads4 ? 4 : 8;
-    constexpr int kRegion = kStages * kTile;  // a warp's ring, and later its state
+    constexpr int kCols = kFour ? 4 : 8;
+    constexpr bool kTwoParts = std::is_same<QT, float>::value;
+    constexpr bool kByGroup = kFour && !kTwoParts && kGroups == 2;
+    constexpr int kPairs = kByGroup ? 1 : kGroups;  // value pairs of a lane and token
+    constexpr int kStepBytes = kStep * kTile;
+    constexpr int kRegion = kRing * kStepBytes;  // a warp's ring, and later its state
     static_assert(kCols * (D + 2) * 4 <= kRegion, "a warp's state must fit its ring");
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ std::uint64_t bars[kWarps * kStages];
-    __shared__ int failed;
     __shared__ std::uint32_t ticket;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -174,46 +196,49 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
     if (static_cast<int>(split) >= splits) return;
     const int b0 = static_cast<int>(split) * p.tiles_per_split;
     const int nb = min(tiles - b0, p.tiles_per_split);
-    const int mine = warp < nb ? (nb - warp + kWarps - 1) / kWarps : 0;  // tiles b0 + warp + 4 i
+    // This warp's tiles: kStep neighbours, then kStep past the other warps'.
+    const int mine = [&] {
+        const int whole = nb / (kStep * kWarps) * kStep, rest = nb % (kStep * kWarps) - kStep * warp;
+        return whole + min(max(rest, 0), kStep);
+    }();
 
-    // ---- the ring. Lane i holds the arena tile of the warp's tile 32 k + i.
+    // ---- the ring: 16-byte asynchronous copies by all lanes, one group a step.
+    // Lane i holds the address of the warp's tile 32 k + i.
     unsigned char* ring = smem + warp * kRegion;
-    std::uint64_t* full = bars + warp * kStages;
     const std::int32_t* table = p.tables + static_cast<std::size_t>(seq) * p.max_blocks;
-    auto arena_tile = [&](int i) -> std::uint64_t {
+    auto tile_address = [&](int i) -> std::uint64_t {
         if (i >= mine) return 0;
-        const std::uint32_t tile = static_cast<std::uint32_t>(b0 + warp + kWarps * i);
+        const std::uint32_t tile = static_cast<std::uint32_t>(b0 + kStep * (warp + kWarps * (i / kStep)) + i % kStep);
         std::int32_t block = table[tile / p.tiles_per_block];
         if (block < 0 || static_cast<std::uint64_t>(block) >= p.num_blocks) {
             flag_error(p.error_word, kErrBadBlock);
             block = 0;  // never dereferenced outside the pool
         }
-        return (static_cast<std::uint64_t>(block) * p.kv_heads + kv_head) * p.tiles_per_block + tile % p.tiles_per_block;
+        const std::uint64_t at = (static_cast<std::uint64_t>(block) * p.kv_heads + kv_head) * p.tiles_per_block + tile % p.tiles_per_block;
+        return reinterpret_cast<std::uint64_t>(p.arena) + at * kTile;
     };
-    std::uint64_t ids = arena_tile(lane), next_ids = 0;
-    auto issue = [&](int i, std::uint64_t id) {  // lane 0
-        const int stage = i % kStages;
-        mbar_arrive_expect_tx(&full[stage], kTile);
-        bulk_copy_g2s(ring + stage * kTile, p.arena + id * kTile, kTile, &full[stage]);
-    };
-    if (lane == 0) {
-        for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
-        fence_barrier_init();
-    }
-    __syncwarp();
+    std::uint64_t addresses = tile_address(lane), next_addresses = 0;
+    const std::uint32_t ring_at = smem_u32(ring) + lane * 16;
+    auto fetch = [&](std::uint32_t to, std::uint64_t from) {  // one tile
+        const unsigned char* src = reinterpret_cast<const unsigned char*>(from) + lane * 16;
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) {
-        const std::uint64_t id = __shfl_sync(0xffffffffu, ids, i);
-        if (lane == 0 && i < mine) issue(i, id);
+        for (int c = 0; c < kTile; c += 512) {
+            if (c + 512 <= kTile || lane * 16 < kTile - c) cp_async16(to + c, src + c);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kRing * kStep; ++i) {
+        const std::uint64_t from = __shfl_sync(0xffffffffu, addresses, i);
+        if (i < mine) fetch(ring_at + i * kTile, from);
+        if (i % kStep == kStep - 1) cp_async_commit();
     }
-    if (threadIdx.x == 0) failed = 0;
 
     // ---- queries as the B operand: lane holds column g, dims 32 w + 8 t4 + 0..7.
     std::uint32_t qf[kWords][4];
     float q_sum[kGroups][2], factor[2];  // of this lane's result columns 2 t4, 2 t4 + 1
     int limit[2];                        // keys they see
     {
-        const int col = kHeads4 ? g & 3 : g;
+        const int col = kFour ? g & 3 : g;
         float x[kWords][8];
         float most = 0.0f;
         bool bad = false;
@@ -260,7 +285,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
         for (int c = 0; c < 2; ++c) {
             const int from = (2 * t4 + c) * 4;
             factor[c] = __shfl_sync(0xffffffffu, down, from);
-            const int cc = kHeads4 ? (2 * t4 + c) & 3 : 2 * t4 + c;
+            const int cc = kFour ? (2 * t4 + c) & 3 : 2 * t4 + c;
             limit[c] = cc < live ? static_cast<int>(start + (r0 + cc) / p.group + 1) : 0;
         }
 #pragma unroll
@@ -276,89 +301,140 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
     const int shortest = static_cast<int>(start + r0 / p.group + 1);  // keys every live column sees
 
     float m[2] = {kNoScore, kNoScore}, l[2] = {0.0f, 0.0f};
-    float z[kGroups][2];
+    float z[kPairs][2];
     float o[kMt][4];
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) z[k][0] = z[k][1] = 0.0f;
+    for (int k = 0; k < kPairs; ++k) z[k][0] = z[k][1] = 0.0f;
 #pragma unroll
     for (int i = 0; i < kMt; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
     const int slot = slot_of_row(g);
-    const std::uint32_t second_part = kHeads4 && t4 >= 2 ? 0xffffffffu : 0u;
+    const std::uint32_t second_part = kFour && t4 >= 2 ? 0xffffffffu : 0u;
+    const int key_at = slot * (D / 2) + t4 * (D / 8);
+    const int pair_key = kv4::pair_at(D, slot, 0, 0), pair_value = kv4::pair_at(D, slot, kByGroup ? t4 >> 1 : 0, 1);
+    const int value_a = kv4::value_word(D, t4, g), value_b = kv4::value_word(D, 7 - t4, g);
+    const int end = static_cast<int>(min(longest, static_cast<long long>(b0 + nb) * kv4::kTileTokens));
+    const int clear = min(shortest, end);  // keys below it are this split's and every live column's
 
-    int done = 0;
-    for (; done < mine; ++done) {
+    std::uint32_t in_ring = 0;
+    int first = (b0 + kStep * warp) * kv4::kTileTokens;
+    for (int done = 0; done < mine; done += kStep, first += kStep * kWarps * kv4::kTileTokens) {
         if ((done & 31) == 0) {
-            if (done > 0) ids = next_ids;
-            next_ids = arena_tile(done + 32 + lane);
+            if (done > 0) addresses = next_addresses;
+            next_addresses = tile_address(done + 32 + lane);
         }
-        const int stage = done % kStages;
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[stage], (done / kStages) & 1, p.error_word))) {
-            if (lane == 0) failed = 1;
-            break;
-        }
-        const unsigned char* tile = ring + stage * kTile;
-        const int first = (b0 + warp + kWarps * done) * kv4::kTileTokens;
+        cp_async_wait_group<kRing - 1>();
+        __syncwarp();
+        const unsigned char* base = ring + in_ring;
 
-        // S^T: rows are tokens slot, slot + 8; per group of 64 dims.
-        float acc[kGroups][4];
+        // S^T - 8 q . 1: rows are tokens slot, slot + 8; per group of 64 dims.
+        float s[kStep][4];  // (token half, column): scores in log2
 #pragma unroll
-        for (int k = 0; k < kGroups; ++k) acc[k][0] = acc[k][1] = acc[k][2] = acc[k][3] = 0.0f;
-        std::uint32_t k0[kWords], k1[kWords];
-        const unsigned char* key = tile + slot * (D / 2) + t4 * (D / 8);
-        if constexpr (D == 128) {
-            const uint4 a = *reinterpret_cast<const uint4*>(key);
-            const uint4 b = *reinterpret_cast<const uint4*>(key + 8 * (D / 2));
-            k0[0] = a.x, k0[1] = a.y, k0[2] = a.z, k0[3] = a.w;
-            k1[0] = b.x, k1[1] = b.y, k1[2] = b.z, k1[3] = b.w;
-        } else {
-            const uint2 a = *reinterpret_cast<const uint2*>(key);
-            const uint2 b = *reinterpret_cast<const uint2*>(key + 8 * (D / 2));
-            k0[0] = a.x, k0[1] = a.y, k1[0] = b.x, k1[1] = b.y;
-        }
-#pragma unroll
-        for (int w = 0; w < kWords; ++w) {
-            const std::uint32_t h0 = k0[w] >> 8, h1 = k1[w] >> 8;
-            mma_f16(acc[w / 2], k0[w] & 0x000f000fu, k1[w] & 0x000f000fu, h0 & 0x000f000fu, h1 & 0x000f000fu,
-                    qf[w][0], qf[w][1]);
-            mma_f16(acc[w / 2], k0[w] & 0x00f000f0u, k1[w] & 0x00f000f0u, h0 & 0x00f000f0u, h1 & 0x00f000f0u,
-                    qf[w][2], qf[w][3]);
-        }
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (token half, column): log2 scores
-        float2 vp[2][kGroups];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int k = 0; k < kGroups; ++k) {
-                const float2 kp = kv4::load_pair(tile, kv4::pair_at(D, slot + 8 * h, k, 0));
-                vp[h][k] = kv4::load_pair(tile, kv4::pair_at(D, slot + 8 * h, k, 1));
-                const float base = fmaf(-8.0f, kp.x, kp.y);
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    s[2 * h + c] = fmaf(kp.x, acc[k][2 * h + c], s[2 * h + c]);
-                    s[2 * h + c] = fmaf(base, q_sum[k][c], s[2 * h + c]);
-                }
+        for (int u = 0; u < kStep; ++u) {
+            const unsigned char* tile = base + u * kTile;
+            float acc[kGroups][4];
+            std::uint32_t k0[kWords], k1[kWords];
+            if constexpr (D == 128) {
+                const uint4 a = *reinterpret_cast<const uint4*>(tile + key_at);
+                const uint4 b = *reinterpret_cast<const uint4*>(tile + key_at + 8 * (D / 2));
+                k0[0] = a.x, k0[1] = a.y, k0[2] = a.z, k0[3] = a.w;
+                k1[0] = b.x, k1[1] = b.y, k1[2] = b.z, k1[3] = b.w;
+            } else {
+                const uint2 a = *reinterpret_cast<const uint2*>(tile + key_at);
+                const uint2 b = *reinterpret_cast<const uint2*>(tile + key_at + 8 * (D / 2));
+                k0[0] = a.x, k0[1] = a.y, k1[0] = b.x, k1[1] = b.y;
             }
-        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] *= factor[i & 1];
-        if (first + kv4::kTileTokens > shortest) {
-            // Slots behind the last key may hold anything; their pairs count as 0.
+            for (int w = 0; w < kWords; ++w) {
+                const std::uint32_t h0 = k0[w] >> 8, h1 = k1[w] >> 8;
+                if (w % 2 == 0) {
+                    mma_f16_onto(acc[w / 2], k0[w] & 0x000f000fu, k1[w] & 0x000f000fu, h0 & 0x000f000fu,
+                                 h1 & 0x000f000fu, qf[w][0], qf[w][1], -8.0f * q_sum[w / 2][0], -8.0f * q_sum[w / 2][1]);
+                } else {
+                    mma_f16(acc[w / 2], k0[w] & 0x000f000fu, k1[w] & 0x000f000fu, h0 & 0x000f000fu, h1 & 0x000f000fu,
+                            qf[w][0], qf[w][1]);
+                }
+                mma_f16(acc[w / 2], k0[w] & 0x00f000f0u, k1[w] & 0x00f000f0u, h0 & 0x00f000f0u, h1 & 0x00f000f0u,
+                        qf[w][2], qf[w][3]);
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int token = first + slot + 8 * h;
+                float2 kp[kGroups];
+                load_pairs(tile + pair_key + 8 * h * kGroups * 4, kp);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) s[2 * h + c] = token < limit[c] ? s[2 * h + c] : -INFINITY;
-                if (token >= longest) {
+                for (int k = 0; k < kGroups; ++k) {
 #pragma unroll
-                    for (int k = 0; k < kGroups; ++k) vp[h][k] = make_float2(0.0f, 0.0f);
+                    for (int c = 0; c < 2; ++c) {
+                        float& x = s[u][2 * h + c];
+                        x = k == 0 ? kp[k].x * acc[k][2 * h + c] : fmaf(kp[k].x, acc[k][2 * h + c], x);
+                        x = fmaf(kp[k].y, q_sum[k][c], x);
+                    }
+                }
+            }
+            // Rounded before m is taken off: scores of 2^28 and more would
+            // otherwise differ from their own maximum.
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[u][i] *= factor[i & 1];
+        }
+        float2 vp[kStep][2][kPairs];
+#pragma unroll
+        for (int u = 0; u < kStep; ++u) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) load_pairs(base + u * kTile + pair_value + 8 * h * kGroups * 4, vp[u][h]);
+        }
+        if (first + kStep * kv4::kTileTokens > clear) {
+            // Slots behind the last key may hold anything; their pairs count as 0.
+#pragma unroll
+            for (int u = 0; u < kStep; ++u) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int token = first + kv4::kTileTokens * u + slot + 8 * h;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) s[u][2 * h + c] = token < min(limit[c], end) ? s[u][2 * h + c] : -INFINITY;
+                    if (token >= end) {
+#pragma unroll
+                        for (int k = 0; k < kPairs; ++k) vp[u][h][k] = make_float2(0.0f, 0.0f);
+                    }
                 }
             }
         }
-        const bool grown = fmaxf(s[0], s[2]) > m[0] + kRescale || fmaxf(s[1], s[3]) > m[1] + kRescale;
-        if (__any_sync(0xffffffffu, grown)) {
+        // Weights 2^(s - m), and times the value scales, which must fit
+        // f16: m moves when one outgrows 2^15 (or a weight 2^34, where scales
+        // are tiny).
+        float weight[kStep][4], scaled[kStep][2][kPairs][2];
+        float most_weight = 0.0f, most_scaled = 0.0f;
+        auto weigh = [&] {
+#pragma unroll
+            for (int u = 0; u < kStep; ++u) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        weight[u][2 * h + c] = ex2_ftz(s[u][2 * h + c] - m[c]);
+#pragma unroll
+                        for (int k = 0; k < kPairs; ++k) scaled[u][h][k][c] = weight[u][2 * h + c] * vp[u][h][k].x;
+                    }
+                    most_weight = fmax3(most_weight, weight[u][2 * h], weight[u][2 * h + 1]);
+#pragma unroll
+                    for (int k = 0; k < kPairs; ++k) most_scaled = fmax3(most_scaled, scaled[u][h][k][0], scaled[u][h][k][1]);
+                }
+            }
+        };
+        weigh();
+        if (__any_sync(0xffffffffu, most_scaled > 32768.0f || most_weight > 17179869184.0f)) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float top = fmaxf(s[c], s[2 + c]);
+                float top = kNoScore;
+#pragma unroll
+                for (int u = 0; u < kStep; ++u) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float scale = 9.5367431640625e-07f;  // 2^-20
+#pragma unroll
+                        for (int k = 0; k < kPairs; ++k) scale = fmaxf(scale, vp[u][h][k].x);
+                        top = fmaxf(top, s[u][2 * h + c] + (__log2f(scale) - kHeadroom));
+                    }
+                }
+                if constexpr (kFour) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));  // the column's twin
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
                 top = fmaxf(top, m[c]);
@@ -366,76 +442,83 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
                 m[c] = top;
                 l[c] *= alpha;
 #pragma unroll
-                for (int k = 0; k < kGroups; ++k) z[k][c] *= alpha;
+                for (int k = 0; k < kPairs; ++k) z[k][c] *= alpha;
 #pragma unroll
                 for (int i = 0; i < kMt; ++i) o[i][c] *= alpha, o[i][2 + c] *= alpha;
             }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s[i] = ex2_ftz(s[i] - m[i & 1]);
-            l[i & 1] += s[i];
+            weigh();
         }
 
-        // P^T as the B operand, per group of dims: weights times scale.
-        std::uint32_t pf[kGroups][2][kHeads4 ? 1 : 2];
 #pragma unroll
-        for (int k = 0; k < kGroups; ++k) {
+        for (int u = 0; u < kStep; ++u) {
+            const unsigned char* tile = base + u * kTile;
+            // P^T as the B operand, per value pair.
+            std::uint32_t pf[kPairs][2], pf2[kPairs][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float w0 = s[2 * h] * vp[h][k].x, w1 = s[2 * h + 1] * vp[h][k].x;
-                z[k][0] = fmaf(s[2 * h], vp[h][k].y, z[k][0]);
-                z[k][1] = fmaf(s[2 * h + 1], vp[h][k].y, z[k][1]);
-                const std::uint32_t high = bf16_pair(w0, w1);
-                if constexpr (kHeads4) {
-                    // Columns 4-7: what the first part leaves.
-                    const std::uint32_t taken = high & second_part;
-                    const float r0_ = w0 - __uint_as_float(taken << 16), r1_ = w1 - __uint_as_float(taken & 0xffff0000u);
-                    pf[k][h][0] = transpose8(bf16_pair(r0_, r1_));
+                l[0] += weight[u][2 * h];
+                l[1] += weight[u][2 * h + 1];
+#pragma unroll
+                for (int k = 0; k < kPairs; ++k) {
+                    const float w0 = scaled[u][h][k][0], w1 = scaled[u][h][k][1];
+                    z[k][0] = fmaf(weight[u][2 * h], vp[u][h][k].y, z[k][0]);
+                    z[k][1] = fmaf(weight[u][2 * h + 1], vp[u][h][k].y, z[k][1]);
+                    const std::uint32_t high = f16_pair(w0, w1);
+                    if constexpr (kTwoParts) {
+                        const std::uint32_t taken = kFour ? high & second_part : high;
+                        const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&taken));
+                        const std::uint32_t left = f16_pair(w0 - t.x, w1 - t.y);
+                        pf[k][h] = transpose8(kFour ? left : high);
+                        if constexpr (!kFour) pf2[k][h] = transpose8(left);
+                    } else {
+                        pf[k][h] = transpose8(high);
+                    }
+                }
+            }
+            // O^T += V^T P^T: k index 2 t4 is token t4, 2 t4 + 1 token 7 - t4.
+            std::uint32_t v[4][kGroups];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned char* at = tile + (i % 2 ? value_b : value_a) + i / 2 * 8 * (D / 2);
+                if constexpr (D == 128) {
+                    const uint2 x = *reinterpret_cast<const uint2*>(at);
+                    v[i][0] = x.x, v[i][1] = x.y;
                 } else {
-                    pf[k][h][0] = transpose8(high);
-                    pf[k][h][1] = transpose8(bf16_pair(w0 - __uint_as_float(high << 16), w1 - __uint_as_float(high & 0xffff0000u)));
+                    v[i][0] = *reinterpret_cast<const std::uint32_t*>(at);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kGroups; ++k) {
+                constexpr int kLast = kPairs - 1;
+                const std::uint32_t(&b)[2] = pf[k < kLast ? k : kLast];
+                const std::uint32_t(&b2)[2] = pf2[k < kLast ? k : kLast];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {  // nibbles 0-3, 4-7: dims 8 g + 0..3, + 4..7
+                    std::uint32_t x = __byte_perm(v[0][k], v[1][k], half ? 0x7632 : 0x5410);
+                    std::uint32_t y = __byte_perm(v[2][k], v[3][k], half ? 0x7632 : 0x5410);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float (&d)[4] = o[4 * k + 2 * half + j];
+                        const std::uint32_t a0 = centred_low(x), a1 = centred_high(x);
+                        const std::uint32_t a2 = centred_low(y), a3 = centred_high(y);
+                        mma_f16(d, a0, a1, a2, a3, b[0], b[1]);
+                        if constexpr (kTwoParts && !kFour) mma_f16(d, a0, a1, a2, a3, b2[0], b2[1]);
+                        x >>= 8, y >>= 8;
+                    }
                 }
             }
         }
-        // O^T += V^T P^T: k index 2 t4 is token t4, 2 t4 + 1 token 7 - t4.
-        std::uint32_t v[4][kGroups];
-        const int rows[4] = {t4, 7 - t4, 8 + t4, 15 - t4};
+        __syncwarp();  // the tiles are read
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const unsigned char* at = tile + kv4::value_word(D, rows[i], g);
-            if constexpr (D == 128) {
-                const uint2 x = *reinterpret_cast<const uint2*>(at);
-                v[i][0] = x.x, v[i][1] = x.y;
-            } else {
-                v[i][0] = *reinterpret_cast<const std::uint32_t*>(at);
-            }
+        for (int u = 0; u < kStep; ++u) {
+            const int i = done + kRing * kStep + u;
+            const std::uint64_t from = __shfl_sync(0xffffffffu, (i ^ done) & ~31 ? next_addresses : addresses, i & 31);
+            if (i < mine) fetch(ring_at + in_ring + u * kTile, from);
         }
-#pragma unroll
-        for (int k = 0; k < kGroups; ++k) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {  // nibbles 0-3, 4-7: dims 8 g + 0..3, + 4..7
-                const std::uint32_t a = __byte_perm(v[0][k], v[1][k], half ? 0x7632 : 0x5410);
-                const std::uint32_t b = __byte_perm(v[2][k], v[3][k], half ? 0x7632 : 0x5410);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float (&d)[4] = o[4 * k + 2 * half + j];
-                    const std::uint32_t a0 = centred_codes(a >> (8 * j)), a1 = centred_codes(a >> (8 * j + 4));
-                    const std::uint32_t a2 = centred_codes(b >> (8 * j)), a3 = centred_codes(b >> (8 * j + 4));
-                    mma_bf16(d, a0, a1, a2, a3, pf[k][0][0], pf[k][1][0]);
-                    if constexpr (!kHeads4) mma_bf16(d, a0, a1, a2, a3, pf[k][0][1], pf[k][1][1]);
-                }
-            }
-        }
-        __syncwarp();  // the tile is read
-        const std::uint64_t id = __shfl_sync(0xffffffffu, ((done + kStages) & 31) < kStages ? next_ids : ids, (done + kStages) & 31);
-        if (lane == 0 && done + kStages < mine) issue(done + kStages, id);
+        cp_async_commit();
+        in_ring = in_ring + kStepBytes == kRegion ? 0 : in_ring + kStepBytes;
     }
-    if (done < mine && lane == 0) {  // a wait ran out: let this warp's own copies land before it leaves
-        for (int i = done; i < min(mine, done + kStages); ++i) {
-            mbar_wait_bounded(&full[i % kStages], (i / kStages) & 1, p.error_word);
-        }
-    }
+    cp_async_wait_group<0>();
     __syncwarp();
 
     // ---- a warp's state into its ring: [column][D] output sums, then m and l.
@@ -445,23 +528,25 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
         for (int off = 4; off < 32; off <<= 1) {
             l[c] += __shfl_xor_sync(0xffffffffu, l[c], off);
 #pragma unroll
-            for (int k = 0; k < kGroups; ++k) z[k][c] += __shfl_xor_sync(0xffffffffu, z[k][c], off);
+            for (int k = 0; k < kPairs; ++k) z[k][c] += __shfl_xor_sync(0xffffffffu, z[k][c], off);
         }
     }
     float* state = reinterpret_cast<float*>(ring);
 #pragma unroll
     for (int i = 0; i < kMt; ++i) {
-        if constexpr (kHeads4) {  // both parts of the weights meet
+        if constexpr (kFour && kTwoParts) {  // both parts of the weights meet
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][e] += __shfl_xor_sync(0xffffffffu, o[i][e], 2);
         }
         const int dim = 64 * (i / 4) + 8 * g + 2 * (i % 4);
+        const int pair = kPairs == 1 ? 0 : i / 4;
+        const bool holds = kByGroup ? t4 >> 1 == i / 4 : !kFour || t4 < 2;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const int col = 2 * t4 + c;
-            if (col < kCols) {
+            const int col = (2 * t4 + c) & (kCols - 1);
+            if (holds) {
                 *reinterpret_cast<float2*>(state + col * D + dim) =
-                    make_float2(o[i][c] + z[i / 4][c], o[i][2 + c] + z[i / 4][c]);
+                    make_float2(o[i][c] + z[pair][c], o[i][2 + c] + z[pair][c]);
             }
         }
     }
@@ -474,7 +559,8 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
     }
     __syncthreads();
     auto state_of = [&](int w) { return reinterpret_cast<const float*>(smem + w * kRegion); };
-    float* part = p.ws_part + (static_cast<std::size_t>(unit) * p.max_splits + split) * kCols * (D + 2);
+    constexpr int kPart = kCols * (D + 4);  // a split's o [column][D], then m and l per column (padded)
+    float* part = p.ws_part + (static_cast<std::size_t>(unit) * p.max_splits + split) * kPart;
     for (int i = threadIdx.x; i < live * D; i += blockDim.x) {
         const int col = i / D;
         float top = kNoScore, sum = 0.0f, total = 0.0f;
@@ -487,12 +573,12 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
             total = fmaf(weight, state_of(w)[i], total);
         }
         if (splits == 1) {
-            const bool ok = isfinite(sum) && sum > 0.0f && failed == 0;
+            const bool ok = isfinite(sum) && sum > 0.0f;
             if (!ok) flag_error(p.error_word, kErrNormalizer);
             static_cast<QT*>(p.out)[row_of(col) * D + i % D] = Storage<QT>::from_float(ok ? total / sum : 0.0f);
         } else {
-            part[2 * kCols + i] = total;
-            if (i % D == 0) part[2 * col] = top, part[2 * col + 1] = sum;
+            part[i] = total;
+            if (i % D == 0) part[kCols * D + 2 * col] = top, part[kCols * D + 2 * col + 1] = sum;
         }
     }
     if (splits == 1) return;
@@ -508,14 +594,14 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
     if (ticket != static_cast<std::uint32_t>(splits) - 1) return;
     __threadfence();
     float* weights = reinterpret_cast<float*>(smem);  // [column][split], then 1 / sum per column
-    const float* parts = p.ws_part + static_cast<std::size_t>(unit) * p.max_splits * kCols * (D + 2);
+    const float* parts = p.ws_part + static_cast<std::size_t>(unit) * p.max_splits * kPart;
     for (int col = warp; col < live; col += kWarps) {
         float top = kNoScore;
-        for (int i = lane; i < splits; i += 32) top = fmaxf(top, __ldcg(parts + static_cast<std::size_t>(i) * kCols * (D + 2) + 2 * col));
+        for (int i = lane; i < splits; i += 32) top = fmaxf(top, __ldcg(parts + static_cast<std::size_t>(i) * kPart + kCols * D + 2 * col));
         top = warp_max(top);
         float sum = 0.0f;
         for (int i = lane; i < splits; i += 32) {
-            const float* ml = parts + static_cast<std::size_t>(i) * kCols * (D + 2) + 2 * col;
+            const float* ml = parts + static_cast<std::size_t>(i) * kPart + kCols * D + 2 * col;
             const float weight = ex2_ftz(__ldcg(ml) - top);
             weights[col * kMaxSplits + i] = weight;
             sum = fmaf(weight, __ldcg(ml + 1), sum);
@@ -526,14 +612,25 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
         if (lane == 0) weights[kCols * kMaxSplits + col] = ok ? 1.0f / sum : 0.0f;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < live * D; i += blockDim.x) {
-        const int col = i / D;
-        float total = 0.0f;
-#pragma unroll 8
+    for (int i = threadIdx.x; i < live * D / 4; i += blockDim.x) {
+        const int col = i / (D / 4);
+        const float4* o4 = reinterpret_cast<const float4*>(parts) + i;
+        const float* w = weights + col * kMaxSplits;
+        float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 16
         for (int k = 0; k < splits; ++k) {
-            total = fmaf(weights[col * kMaxSplits + k], __ldcg(parts + static_cast<std::size_t>(k) * kCols * (D + 2) + 2 * kCols + i), total);
+            const float4 x = __ldcg(o4 + static_cast<std::size_t>(k) * (kPart / 4));
+            total.x = fmaf(w[k], x.x, total.x);
+            total.y = fmaf(w[k], x.y, total.y);
+            total.z = fmaf(w[k], x.z, total.z);
+            total.w = fmaf(w[k], x.w, total.w);
         }
-        static_cast<QT*>(p.out)[row_of(col) * D + i % D] = Storage<QT>::from_float(total * weights[kCols * kMaxSplits + col]);
+        const float inv = weights[kCols * kMaxSplits + col];
+        QT* out = static_cast<QT*>(p.out) + row_of(col) * D + 4 * i % D;
+        out[0] = Storage<QT>::from_float(total.x * inv);
+        out[1] = Storage<QT>::from_float(total.y * inv);
+        out[2] = Storage<QT>::from_float(total.z * inv);
+        out[3] = Storage<QT>::from_float(total.w * inv);
     }
 }
 
@@ -567,7 +664,7 @@ Kv4Plan plan_kv4(const InferlabCudaKvPool& p, std::uint32_t num_seqs, std::uint3
     plan.column_tiles = static_cast<std::uint32_t>(column_tiles);
     if (plan.max_splits > 1) {
         plan.counter_bytes = (units * 4 + 255) & ~std::size_t(255);
-        plan.part_bytes = checked_mul(units * plan.max_splits, plan.columns * (p.head_dim + 2) * 4, "4-bit attention batch is too large");
+        plan.part_bytes = checked_mul(units * plan.max_splits, plan.columns * (p.head_dim + 4) * 4, "4-bit attention batch is too large");
     }
     return plan;
 }
@@ -582,7 +679,7 @@ void check_kv4(const InferlabCudaKvPool& p, const void* queries, std::uint32_t q
     if (q_heads == 0 || q_heads % p.kv_heads != 0) {
         throw std::runtime_error("4-bit attention q_heads must be a positive multiple of kv_heads");
     }
-    if (max_blocks == 0 || max_context_len == 0 || max_context_len > 0x7FFFFFF0u) {
+    if (max_blocks == 0 || max_context_len == 0 || max_context_len > 0x7FFFFF00u) {
         throw std::runtime_error("4-bit attention block table and context bound must be positive");
     }
     if (reinterpret_cast<std::uintptr_t>(queries) % 16 != 0 || reinterpret_cast<std::uintptr_t>(out) % 16 != 0) {
@@ -596,6 +693,9 @@ void run_kv4(InferlabCudaKvPool& p, Kv4Params k, std::uint32_t query_dtype, std:
     const Kv4Plan plan = plan_kv4(p, num_seqs, k.q_heads, k.max_count, max_context_len);
     if (plan.part_bytes != 0 && (workspace == nullptr || workspace_bytes < plan.counter_bytes + plan.part_bytes)) {
         throw std::runtime_error("4-bit attention workspace is too small");
+    }
+    if (plan.part_bytes != 0 && reinterpret_cast<std::uintptr_t>(workspace) % 16 != 0) {
+        throw std::runtime_error("4-bit attention workspace must be 16-byte aligned");
     }
     k.arena = static_cast<const unsigned char*>(p.key_arena);
     k.num_blocks = p.num_blocks;
@@ -617,7 +717,7 @@ void run_kv4(InferlabCudaKvPool& p, Kv4Params k, std::uint32_t query_dtype, std:
         auto* kernel = p.head_dim == 128
             ? (plan.columns == 4 ? kv4_attention_kernel<RowT, QT, 128, true> : kv4_attention_kernel<RowT, QT, 128, false>)
             : (plan.columns == 4 ? kv4_attention_kernel<RowT, QT, 64, true> : kv4_attention_kernel<RowT, QT, 64, false>);
-        const int smem = kWarps * kStages * kv4::tile_bytes(static_cast<int>(p.head_dim));
+        const int smem = kWarps * kRing * kStep * kv4::tile_bytes(static_cast<int>(p.head_dim));
         cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute");
         kernel<<<grid, kWarps * 32, smem, s>>>(k);
     };

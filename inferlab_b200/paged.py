@@ -620,7 +620,7 @@ class CudaKvPool:
         if segments == 0 or total == 0:
             return out
         if max_context_len is None:
-            max_context_len = min(block_tables.shape[1] * self.block_tokens, 0x7fffffff)
+            max_context_len = min(block_tables.shape[1] * self.block_tokens, 0x7fffff00)
         if workspace is None:
             workspace = self._kv4_workspace(segments, q_heads, max_query_count, max_context_len,
                                             stream)

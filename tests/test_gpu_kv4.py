@@ -6,8 +6,9 @@ Tolerances count roundings. eps below is half a unit in the last place of the ty
 - rotation: two products and a sum in fp32, each 2^-24 relative to at most |a| + |b|: 2^-23 (|a| + |b|), then the type's
   rounding.
 - attention: the result's rounding, and on the weights p what scores, exponentials and splits of p cost: at most dim + 64
-  fp32 roundings of the sum |q k| (2^-24 each), 2^-17 for p carried as two bf16 parts and 2^-21 for its exponential. A
-  weight off by a share w moves the output by at most 2 w max|v|.
+  fp32 roundings of the sum |q k| (2^-24 each), 2^-21 for its exponential, and p's own rounding: one f16 number for 16-bit
+  queries (2^-11), two f16 parts for fp32 queries (2^-17 with room for the second part's subnormals). A weight off by a
+  share w moves the output by at most 2 w max|v|.
 """
 import ctypes
 
@@ -66,7 +67,7 @@ def rounding(kind, ref):
 
 
 def attention_bound(kind, out, reach, size, dim):
-    share = (dim + 64) * 2.0 ** -24 * reach + 2.0 ** -17 + 2.0 ** -21
+    share = (dim + 64) * 2.0 ** -24 * reach + (2.0 ** -17 if kind == "f32" else 2.0 ** -11) + 2.0 ** -21
     extra = (2 * share * size)[..., None]
     return rounding(kind, np.abs(out) + extra) + extra
 
