@@ -13,7 +13,9 @@
 //     c 2^-24, in bits 4-7 it is c 2^-20, so a mask is the whole conversion; q
 //     is scaled by a power of two per row (exact) into f16's range, and by 2^-4
 //     where it meets the latter.
-//   output: V codes as f16 c - 8, one mask-or and one subtraction for two, and
+//   output: V codes as such f16 numbers less 8 of their unit, one mask and one
+//     subtraction for two (each unit belongs to rows of the result, which are
+//     scaled at the end), and
 //     the weights p scale as f16, in two parts (22 bits together) for fp32
 //     results. f16's range is kept by what m is: not the largest score but the
 //     largest p scale, kept between 2^10 and 2^15, so that the first part loses
@@ -93,17 +95,17 @@ __device__ __forceinline__ std::uint32_t transpose8(std::uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-// Codes as f16 c - 8: bits 0-3 of each half under 2^10's exponent are 1024 + c,
-// bits 4-7 under 2^6's are 64 + c.
-__device__ __forceinline__ std::uint32_t centred(std::uint32_t raw, float bias) {
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&raw), __float2half2_rn(bias));
+// Two masked codes c 2^-24 (low nibbles) or c 2^-20 (high ones) as f16, less 8
+// of that unit: exact, subnormal or not.
+__device__ __forceinline__ std::uint32_t centred_low(std::uint32_t x) {
+    x &= 0x000f000fu;
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x0008)));
     return *reinterpret_cast<const std::uint32_t*>(&v);
 }
-__device__ __forceinline__ std::uint32_t centred_low(std::uint32_t x) {
-    return centred((x & 0x000f000fu) | 0x64006400u, 1032.0f);
-}
 __device__ __forceinline__ std::uint32_t centred_high(std::uint32_t x) {
-    return centred((x & 0x00f000f0u) | 0x54005400u, 72.0f);
+    x &= 0x00f000f0u;
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x0080)));
+    return *reinterpret_cast<const std::uint32_t*>(&v);
 }
 __device__ __forceinline__ std::uint32_t f16_pair(float low, float high) {
     const __half2 v = __floats2half2_rn(low, high);
@@ -203,7 +205,8 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
     }();
 
     // ---- the ring: 16-byte asynchronous copies by all lanes, one group a step.
-    // Lane i holds the address of the warp's tile 32 k + i.
+    // Lane i holds the address of the warp's tile kAhead + 32 k + i.
+    constexpr int kAhead = kRing * kStep;
     unsigned char* ring = smem + warp * kRegion;
     const std::int32_t* table = p.tables + static_cast<std::size_t>(seq) * p.max_blocks;
     auto tile_address = [&](int i) -> std::uint64_t {
@@ -217,7 +220,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
         const std::uint64_t at = (static_cast<std::uint64_t>(block) * p.kv_heads + kv_head) * p.tiles_per_block + tile % p.tiles_per_block;
         return reinterpret_cast<std::uint64_t>(p.arena) + at * kTile;
     };
-    std::uint64_t addresses = tile_address(lane), next_addresses = 0;
+    std::uint64_t addresses = lane < kAhead ? tile_address(lane) : 0;
     const std::uint32_t ring_at = smem_u32(ring) + lane * 16;
     auto fetch = [&](std::uint32_t to, std::uint64_t from) {  // one tile
         const unsigned char* src = reinterpret_cast<const unsigned char*>(from) + lane * 16;
@@ -227,11 +230,12 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
         }
     };
 #pragma unroll
-    for (int i = 0; i < kRing * kStep; ++i) {
+    for (int i = 0; i < kAhead; ++i) {
         const std::uint64_t from = __shfl_sync(0xffffffffu, addresses, i);
         if (i < mine) fetch(ring_at + i * kTile, from);
         if (i % kStep == kStep - 1) cp_async_commit();
     }
+    std::uint64_t next_addresses = tile_address(kAhead + lane);
 
     // ---- queries as the B operand: lane holds column g, dims 32 w + 8 t4 + 0..7.
     std::uint32_t qf[kWords][4];
@@ -315,19 +319,13 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
     const int end = static_cast<int>(min(longest, static_cast<long long>(b0 + nb) * kv4::kTileTokens));
     const int clear = min(shortest, end);  // keys below it are this split's and every live column's
 
-    std::uint32_t in_ring = 0;
-    int first = (b0 + kStep * warp) * kv4::kTileTokens;
-    for (int done = 0; done < mine; done += kStep, first += kStep * kWarps * kv4::kTileTokens) {
-        if ((done & 31) == 0) {
-            if (done > 0) addresses = next_addresses;
-            next_addresses = tile_address(done + 32 + lane);
-        }
-        cp_async_wait_group<kRing - 1>();
-        __syncwarp();
-        const unsigned char* base = ring + in_ring;
-
+    // Per step: scores of the next one beside the output product of this one
+    // (independent work for the scheduler), then the next one's weights.
+    float s[kStep][4];  // (token half, column): scores in log2
+    float2 vp[kStep][2][kPairs];
+    std::uint32_t pf[kStep][kPairs][2], pf2[kStep][kPairs][2];
+    auto scores = [&](const unsigned char* base) {
         // S^T - 8 q . 1: rows are tokens slot, slot + 8; per group of 64 dims.
-        float s[kStep][4];  // (token half, column): scores in log2
 #pragma unroll
         for (int u = 0; u < kStep; ++u) {
             const unsigned char* tile = base + u * kTile;
@@ -375,12 +373,13 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[u][i] *= factor[i & 1];
         }
-        float2 vp[kStep][2][kPairs];
 #pragma unroll
         for (int u = 0; u < kStep; ++u) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) load_pairs(base + u * kTile + pair_value + 8 * h * kGroups * 4, vp[u][h]);
         }
+    };
+    auto weights = [&](int first) {
         if (first + kStep * kv4::kTileTokens > clear) {
             // Slots behind the last key may hold anything; their pairs count as 0.
 #pragma unroll
@@ -451,9 +450,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
 
 #pragma unroll
         for (int u = 0; u < kStep; ++u) {
-            const unsigned char* tile = base + u * kTile;
             // P^T as the B operand, per value pair.
-            std::uint32_t pf[kPairs][2], pf2[kPairs][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 l[0] += weight[u][2 * h];
@@ -468,13 +465,19 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
                         const std::uint32_t taken = kFour ? high & second_part : high;
                         const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&taken));
                         const std::uint32_t left = f16_pair(w0 - t.x, w1 - t.y);
-                        pf[k][h] = transpose8(kFour ? left : high);
-                        if constexpr (!kFour) pf2[k][h] = transpose8(left);
+                        pf[u][k][h] = transpose8(kFour ? left : high);
+                        if constexpr (!kFour) pf2[u][k][h] = transpose8(left);
                     } else {
-                        pf[k][h] = transpose8(high);
+                        pf[u][k][h] = transpose8(high);
                     }
                 }
             }
+        }
+    };
+    auto output = [&](const unsigned char* base) {
+#pragma unroll
+        for (int u = 0; u < kStep; ++u) {
+            const unsigned char* tile = base + u * kTile;
             // O^T += V^T P^T: k index 2 t4 is token t4, 2 t4 + 1 token 7 - t4.
             std::uint32_t v[4][kGroups];
 #pragma unroll
@@ -490,8 +493,8 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
 #pragma unroll
             for (int k = 0; k < kGroups; ++k) {
                 constexpr int kLast = kPairs - 1;
-                const std::uint32_t(&b)[2] = pf[k < kLast ? k : kLast];
-                const std::uint32_t(&b2)[2] = pf2[k < kLast ? k : kLast];
+                const std::uint32_t(&b)[2] = pf[u][k < kLast ? k : kLast];
+                const std::uint32_t(&b2)[2] = pf2[u][k < kLast ? k : kLast];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {  // nibbles 0-3, 4-7: dims 8 g + 0..3, + 4..7
                     std::uint32_t x = __byte_perm(v[0][k], v[1][k], half ? 0x7632 : 0x5410);
@@ -508,15 +511,29 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
                 }
             }
         }
-        __syncwarp();  // the tiles are read
+    };
+    int first = (b0 + kStep * warp) * kv4::kTileTokens;
+    std::uint32_t in_ring = 0;
+    int done = 0;
+    for (; done < mine; done += kStep) {
+        if ((done & 31) == 0) {
+            addresses = next_addresses;
+            next_addresses = tile_address(kAhead + done + 32 + lane);
+        }
+        cp_async_wait_group<kRing - 1>();
+        __syncwarp();
+        scores(ring + in_ring);
+        weights(first);
+        output(ring + in_ring);
+        __syncwarp();  // this step's tiles are read
 #pragma unroll
         for (int u = 0; u < kStep; ++u) {
-            const int i = done + kRing * kStep + u;
-            const std::uint64_t from = __shfl_sync(0xffffffffu, (i ^ done) & ~31 ? next_addresses : addresses, i & 31);
-            if (i < mine) fetch(ring_at + in_ring + u * kTile, from);
+            const std::uint64_t from = __shfl_sync(0xffffffffu, addresses, (done + u) & 31);
+            if (kAhead + done + u < mine) fetch(ring_at + in_ring + u * kTile, from);
         }
         cp_async_commit();
         in_ring = in_ring + kStepBytes == kRegion ? 0 : in_ring + kStepBytes;
+        first += kStep * kWarps * kv4::kTileTokens;
     }
     cp_async_wait_group<0>();
     __syncwarp();
@@ -545,8 +562,9 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
         for (int c = 0; c < 2; ++c) {
             const int col = (2 * t4 + c) & (kCols - 1);
             if (holds) {
+                // Back from the codes' units: 2^24 in rows g, 2^20 in rows g + 8.
                 *reinterpret_cast<float2*>(state + col * D + dim) =
-                    make_float2(o[i][c] + z[pair][c], o[i][2 + c] + z[pair][c]);
+                    make_float2(fmaf(o[i][c], 16777216.0f, z[pair][c]), fmaf(o[i][2 + c], 1048576.0f, z[pair][c]));
             }
         }
     }
@@ -593,7 +611,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
     __syncthreads();
     if (ticket != static_cast<std::uint32_t>(splits) - 1) return;
     __threadfence();
-    float* weights = reinterpret_cast<float*>(smem);  // [column][split], then 1 / sum per column
+    float* split_weights = reinterpret_cast<float*>(smem);  // [column][split], then 1 / sum per column
     const float* parts = p.ws_part + static_cast<std::size_t>(unit) * p.max_splits * kPart;
     for (int col = warp; col < live; col += kWarps) {
         float top = kNoScore;
@@ -603,19 +621,19 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
         for (int i = lane; i < splits; i += 32) {
             const float* ml = parts + static_cast<std::size_t>(i) * kPart + kCols * D + 2 * col;
             const float weight = ex2_ftz(__ldcg(ml) - top);
-            weights[col * kMaxSplits + i] = weight;
+            split_weights[col * kMaxSplits + i] = weight;
             sum = fmaf(weight, __ldcg(ml + 1), sum);
         }
         sum = warp_sum(sum);
         const bool ok = isfinite(sum) && sum > 0.0f;
         if (!ok && lane == 0) flag_error(p.error_word, kErrNormalizer);
-        if (lane == 0) weights[kCols * kMaxSplits + col] = ok ? 1.0f / sum : 0.0f;
+        if (lane == 0) split_weights[kCols * kMaxSplits + col] = ok ? 1.0f / sum : 0.0f;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < live * D / 4; i += blockDim.x) {
         const int col = i / (D / 4);
         const float4* o4 = reinterpret_cast<const float4*>(parts) + i;
-        const float* w = weights + col * kMaxSplits;
+        const float* w = split_weights + col * kMaxSplits;
         float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 16
         for (int k = 0; k < splits; ++k) {
@@ -625,7 +643,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
             total.z = fmaf(w[k], x.z, total.z);
             total.w = fmaf(w[k], x.w, total.w);
         }
-        const float inv = weights[kCols * kMaxSplits + col];
+        const float inv = split_weights[kCols * kMaxSplits + col];
         QT* out = static_cast<QT*>(p.out) + row_of(col) * D + 4 * i % D;
         out[0] = Storage<QT>::from_float(total.x * inv);
         out[1] = Storage<QT>::from_float(total.y * inv);
