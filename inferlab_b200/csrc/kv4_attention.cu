@@ -4,7 +4,7 @@
 // For a query q and the keys it sees, s_t = q . k_t / sqrt(D), p_t = exp(s_t -
 // m), out = sum p_t v_t / sum p_t in one pass over the tokens with a running
 // maximum m. With k = (c - 8) scale + zero per 64 dims,
-//   s   = sum_groups [ scale (q . c - 8 q . 1) + zero (q . 1) ]
+//   s   = sum_groups [ scale (q . c) + (zero - 8 scale) (q . 1) ]
 //   out = sum_t p_t scale_t (c_t - 8) + sum_t p_t zero_t,
 // so both products run on the codes, which mma.sync takes as small exact
 // numbers, and the pairs meet only scores and weights: 4 numbers per 16 tokens
@@ -60,7 +60,7 @@ struct Kv4Params {
     void* out;
     const std::int32_t* tables;
     std::uint32_t max_blocks;
-    long long max_context;
+    int max_context;
     const std::int32_t* context_lens;  // decode; null: segments
     const std::int32_t* starts;
     const std::int32_t* counts;
@@ -82,13 +82,13 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], std::uint32_t a0, std::ui
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// The same onto c0, c1 (one for each column of the lane).
-__device__ __forceinline__ void mma_f16_onto(float (&d)[4], std::uint32_t a0, std::uint32_t a1,
-                                             std::uint32_t a2, std::uint32_t a3, std::uint32_t b0,
-                                             std::uint32_t b1, float c0, float c1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+// The same onto zero.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], std::uint32_t a0, std::uint32_t a1,
+                                              std::uint32_t a2, std::uint32_t a3, std::uint32_t b0,
+                                              std::uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ std::uint32_t transpose8(std::uint32_t x) {
     std::uint32_t y;
@@ -156,35 +156,48 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
     const std::uint32_t column_tile = unit % p.column_tiles;
     const std::uint32_t kv_head = unit / p.column_tiles % p.kv_heads;
     const std::uint32_t seq = unit / p.column_tiles / p.kv_heads;
+    const int b0 = static_cast<int>(split) * p.tiles_per_split;
+
+    // Block ids of the split's first tiles are asked for at once, beside the
+    // context length (an entry behind the sequence's last block is not used).
+    // The warp's tiles: kStep neighbours, then kStep past the other warps'.
+    // Lane i has tile i of the first kAhead, then tile kAhead + 32 k + i.
+    constexpr int kAhead = kRing * kStep;
+    const std::int32_t* table = p.tables + static_cast<std::size_t>(seq) * p.max_blocks;
+    auto tile_of = [&](int i) { return static_cast<std::uint32_t>(b0 + kStep * (warp + kWarps * (i / kStep)) + i % kStep); };
+    auto block_of = [&](int i) { return table[min(tile_of(i) / p.tiles_per_block, p.max_blocks - 1)]; };
+    const std::int32_t first_blocks = lane < kAhead ? block_of(lane) : 0;
+    std::int32_t next_blocks = block_of(kAhead + lane);
 
     // ---- what this CTA works on: columns r0 .. r0 + live - 1 of the sequence's
     // count * group query rows (token-major), keys 0 .. longest - 1.
-    long long start, count, offset;
+    std::uint32_t start, count, offset;
     bool valid;
     if (p.context_lens != nullptr) {
-        const long long ctx = p.context_lens[seq];
-        start = ctx - 1;
+        const std::int32_t ctx = p.context_lens[seq];
+        valid = ctx >= 0 && ctx <= p.max_context;
+        start = static_cast<std::uint32_t>(ctx) - 1;
         count = 1;
         offset = seq;
-        valid = ctx >= 0 && ctx <= p.max_context;
         if (!valid && split == 0 && threadIdx.x == 0) flag_error(p.error_word, kErrContext);
     } else {
-        start = p.starts[seq];
-        count = p.counts[seq];
-        offset = p.offsets[seq];
-        valid = start >= 0 && count >= 0 && start + count <= p.max_context;
-        const bool rows_ok = count >= 0 && count <= p.max_count && offset >= 0 && offset + count <= p.total_queries;
+        const std::int32_t s = p.starts[seq], c = p.counts[seq], o = p.offsets[seq];
+        start = static_cast<std::uint32_t>(s);
+        count = static_cast<std::uint32_t>(c);
+        offset = static_cast<std::uint32_t>(o);
+        valid = s >= 0 && c >= 0 && static_cast<long long>(s) + c <= p.max_context;
+        const bool rows_ok = c >= 0 && count <= p.max_count && o >= 0 && static_cast<long long>(o) + c <= p.total_queries;
         if (!(valid && rows_ok) && split == 0 && threadIdx.x == 0) flag_error(p.error_word, kErrSegment);
         if (!rows_ok) return;
     }
-    const long long r0 = static_cast<long long>(column_tile) * kCols;
-    const int live = static_cast<int>(min(static_cast<long long>(kCols), count * p.group - r0));
-    if (live <= 0) return;
-    auto row_of = [&](int col) {  // the row of queries / out of a live column
-        const long long r = r0 + col;
-        return (offset + r / p.group) * p.q_heads + kv_head * p.group + r % p.group;
+    const std::uint32_t r0 = column_tile * kCols;
+    if (r0 >= count * p.group) return;
+    const int live = static_cast<int>(min(static_cast<std::uint32_t>(kCols), count * p.group - r0));
+    auto row_of = [&](int col) -> std::size_t {  // the row of queries / out of a live column
+        const std::uint32_t token = (r0 + col) / p.group;
+        return static_cast<std::size_t>(offset + token) * p.q_heads + kv_head * p.group + (r0 + col - token * p.group);
     };
-    const long long longest = valid ? start + (r0 + live - 1) / p.group + 1 : 0;
+    const int longest = valid ? static_cast<int>(start + (r0 + live - 1) / p.group + 1) : 0;
     if (longest == 0) {  // no sequence, or a bad one: zero rows
         if (split == 0) {
             for (int i = threadIdx.x; i < live * D; i += blockDim.x) {
@@ -193,34 +206,27 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
         }
         return;
     }
-    const int tiles = static_cast<int>((longest + kv4::kTileTokens - 1) / kv4::kTileTokens);
+    const int tiles = (longest + kv4::kTileTokens - 1) / kv4::kTileTokens;
     const int splits = (tiles + p.tiles_per_split - 1) / p.tiles_per_split;
     if (static_cast<int>(split) >= splits) return;
-    const int b0 = static_cast<int>(split) * p.tiles_per_split;
     const int nb = min(tiles - b0, p.tiles_per_split);
-    // This warp's tiles: kStep neighbours, then kStep past the other warps'.
     const int mine = [&] {
         const int whole = nb / (kStep * kWarps) * kStep, rest = nb % (kStep * kWarps) - kStep * warp;
         return whole + min(max(rest, 0), kStep);
     }();
 
     // ---- the ring: 16-byte asynchronous copies by all lanes, one group a step.
-    // Lane i holds the address of the warp's tile kAhead + 32 k + i.
-    constexpr int kAhead = kRing * kStep;
     unsigned char* ring = smem + warp * kRegion;
-    const std::int32_t* table = p.tables + static_cast<std::size_t>(seq) * p.max_blocks;
-    auto tile_address = [&](int i) -> std::uint64_t {
+    auto tile_address = [&](int i, std::int32_t block) -> std::uint64_t {
         if (i >= mine) return 0;
-        const std::uint32_t tile = static_cast<std::uint32_t>(b0 + kStep * (warp + kWarps * (i / kStep)) + i % kStep);
-        std::int32_t block = table[tile / p.tiles_per_block];
         if (block < 0 || static_cast<std::uint64_t>(block) >= p.num_blocks) {
             flag_error(p.error_word, kErrBadBlock);
             block = 0;  // never dereferenced outside the pool
         }
-        const std::uint64_t at = (static_cast<std::uint64_t>(block) * p.kv_heads + kv_head) * p.tiles_per_block + tile % p.tiles_per_block;
+        const std::uint64_t at = (static_cast<std::uint64_t>(block) * p.kv_heads + kv_head) * p.tiles_per_block + tile_of(i) % p.tiles_per_block;
         return reinterpret_cast<std::uint64_t>(p.arena) + at * kTile;
     };
-    std::uint64_t addresses = lane < kAhead ? tile_address(lane) : 0;
+    std::uint64_t addresses = lane < kAhead ? tile_address(lane, first_blocks) : 0;
     const std::uint32_t ring_at = smem_u32(ring) + lane * 16;
     auto fetch = [&](std::uint32_t to, std::uint64_t from) {  // one tile
         const unsigned char* src = reinterpret_cast<const unsigned char*>(from) + lane * 16;
@@ -229,14 +235,6 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
             if (c + 512 <= kTile || lane * 16 < kTile - c) cp_async16(to + c, src + c);
         }
     };
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-        const std::uint64_t from = __shfl_sync(0xffffffffu, addresses, i);
-        if (i < mine) fetch(ring_at + i * kTile, from);
-        if (i % kStep == kStep - 1) cp_async_commit();
-    }
-    std::uint64_t next_addresses = tile_address(kAhead + lane);
-
     // ---- queries as the B operand: lane holds column g, dims 32 w + 8 t4 + 0..7.
     std::uint32_t qf[kWords][4];
     float q_sum[kGroups][2], factor[2];  // of this lane's result columns 2 t4, 2 t4 + 1
@@ -246,16 +244,25 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
         float x[kWords][8];
         float most = 0.0f;
         bool bad = false;
+        // Asked for before the tiles, which would keep them waiting.
+        const QT* row = static_cast<const QT*>(p.queries) + row_of(min(col, live - 1)) * D + 8 * t4;
+        constexpr int kPer = 16 / sizeof(QT);
+        uint4 raw[kWords][8 / kPer];
 #pragma unroll
         for (int w = 0; w < kWords; ++w) {
-            if (col < live) {
-                const QT* q = static_cast<const QT*>(p.queries) + row_of(col) * D + 32 * w + 8 * t4;
-                constexpr int kPer = 16 / sizeof(QT);
 #pragma unroll
-                for (int c = 0; c < 8 / kPer; ++c) {
-                    widen16(reinterpret_cast<const uint4*>(q)[c], &x[w][c * kPer], QT{});
-                }
-            }
+            for (int c = 0; c < 8 / kPer; ++c) raw[w][c] = reinterpret_cast<const uint4*>(row + 32 * w)[c];
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const std::uint64_t from = __shfl_sync(0xffffffffu, addresses, i);
+            if (i < mine) fetch(ring_at + i * kTile, from);
+            if (i % kStep == kStep - 1) cp_async_commit();
+        }
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+#pragma unroll
+            for (int c = 0; c < 8 / kPer; ++c) widen16(raw[w][c], &x[w][c * kPer], QT{});
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 x[w][i] = col < live ? Storage<RowT>::to_float(Storage<RowT>::from_float(x[w][i])) : 0.0f;
@@ -316,7 +323,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
     const int key_at = slot * (D / 2) + t4 * (D / 8);
     const int pair_key = kv4::pair_at(D, slot, 0, 0), pair_value = kv4::pair_at(D, slot, kByGroup ? t4 >> 1 : 0, 1);
     const int value_a = kv4::value_word(D, t4, g), value_b = kv4::value_word(D, 7 - t4, g);
-    const int end = static_cast<int>(min(longest, static_cast<long long>(b0 + nb) * kv4::kTileTokens));
+    const int end = min(longest, (b0 + nb) * kv4::kTileTokens);
     const int clear = min(shortest, end);  // keys below it are this split's and every live column's
 
     // Per step: scores of the next one beside the output product of this one
@@ -325,7 +332,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
     float2 vp[kStep][2][kPairs];
     std::uint32_t pf[kStep][kPairs][2], pf2[kStep][kPairs][2];
     auto scores = [&](const unsigned char* base) {
-        // S^T - 8 q . 1: rows are tokens slot, slot + 8; per group of 64 dims.
+        // S^T: rows are tokens slot, slot + 8; per group of 64 dims.
 #pragma unroll
         for (int u = 0; u < kStep; ++u) {
             const unsigned char* tile = base + u * kTile;
@@ -345,8 +352,8 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
             for (int w = 0; w < kWords; ++w) {
                 const std::uint32_t h0 = k0[w] >> 8, h1 = k1[w] >> 8;
                 if (w % 2 == 0) {
-                    mma_f16_onto(acc[w / 2], k0[w] & 0x000f000fu, k1[w] & 0x000f000fu, h0 & 0x000f000fu,
-                                 h1 & 0x000f000fu, qf[w][0], qf[w][1], -8.0f * q_sum[w / 2][0], -8.0f * q_sum[w / 2][1]);
+                    mma_f16_first(acc[w / 2], k0[w] & 0x000f000fu, k1[w] & 0x000f000fu, h0 & 0x000f000fu,
+                                  h1 & 0x000f000fu, qf[w][0], qf[w][1]);
                 } else {
                     mma_f16(acc[w / 2], k0[w] & 0x000f000fu, k1[w] & 0x000f000fu, h0 & 0x000f000fu, h1 & 0x000f000fu,
                             qf[w][0], qf[w][1]);
@@ -360,11 +367,12 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
                 load_pairs(tile + pair_key + 8 * h * kGroups * 4, kp);
 #pragma unroll
                 for (int k = 0; k < kGroups; ++k) {
+                    const float rest = fmaf(-8.0f, kp[k].x, kp[k].y);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         float& x = s[u][2 * h + c];
-                        x = k == 0 ? kp[k].x * acc[k][2 * h + c] : fmaf(kp[k].x, acc[k][2 * h + c], x);
-                        x = fmaf(kp[k].y, q_sum[k][c], x);
+                        x = k == 0 ? rest * q_sum[k][c] : fmaf(rest, q_sum[k][c], x);
+                        x = fmaf(kp[k].x, acc[k][2 * h + c], x);
                     }
                 }
             }
@@ -517,8 +525,8 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
     int done = 0;
     for (; done < mine; done += kStep) {
         if ((done & 31) == 0) {
-            addresses = next_addresses;
-            next_addresses = tile_address(kAhead + done + 32 + lane);
+            addresses = tile_address(kAhead + done + lane, next_blocks);
+            next_blocks = block_of(kAhead + done + 32 + lane);
         }
         cp_async_wait_group<kRing - 1>();
         __syncwarp();
@@ -601,49 +609,52 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
     }
     if (splits == 1) return;
 
-    // ---- the unit's last CTA merges the splits in their order.
-    __threadfence();
+    // ---- the unit's last CTA merges the splits in their order, every thread
+    // four dims: one round of loads for each kRound splits.
     __syncthreads();
     if (threadIdx.x == 0) {
+        __threadfence();
         ticket = atomicAdd(&p.ws_count[unit], 1u);
         if (ticket == static_cast<std::uint32_t>(splits) - 1) p.ws_count[unit] = 0;
+        __threadfence();
     }
     __syncthreads();
     if (ticket != static_cast<std::uint32_t>(splits) - 1) return;
-    __threadfence();
-    float* split_weights = reinterpret_cast<float*>(smem);  // [column][split], then 1 / sum per column
+    constexpr int kRound = 8;
     const float* parts = p.ws_part + static_cast<std::size_t>(unit) * p.max_splits * kPart;
-    for (int col = warp; col < live; col += kWarps) {
-        float top = kNoScore;
-        for (int i = lane; i < splits; i += 32) top = fmaxf(top, __ldcg(parts + static_cast<std::size_t>(i) * kPart + kCols * D + 2 * col));
-        top = warp_max(top);
-        float sum = 0.0f;
-        for (int i = lane; i < splits; i += 32) {
-            const float* ml = parts + static_cast<std::size_t>(i) * kPart + kCols * D + 2 * col;
-            const float weight = ex2_ftz(__ldcg(ml) - top);
-            split_weights[col * kMaxSplits + i] = weight;
-            sum = fmaf(weight, __ldcg(ml + 1), sum);
-        }
-        sum = warp_sum(sum);
-        const bool ok = isfinite(sum) && sum > 0.0f;
-        if (!ok && lane == 0) flag_error(p.error_word, kErrNormalizer);
-        if (lane == 0) split_weights[kCols * kMaxSplits + col] = ok ? 1.0f / sum : 0.0f;
-    }
-    __syncthreads();
     for (int i = threadIdx.x; i < live * D / 4; i += blockDim.x) {
         const int col = i / (D / 4);
-        const float4* o4 = reinterpret_cast<const float4*>(parts) + i;
-        const float* w = split_weights + col * kMaxSplits;
+        float top = kNoScore, sum = 0.0f;
         float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 16
-        for (int k = 0; k < splits; ++k) {
-            const float4 x = __ldcg(o4 + static_cast<std::size_t>(k) * (kPart / 4));
-            total.x = fmaf(w[k], x.x, total.x);
-            total.y = fmaf(w[k], x.y, total.y);
-            total.z = fmaf(w[k], x.z, total.z);
-            total.w = fmaf(w[k], x.w, total.w);
+        for (int k0 = 0; k0 < splits; k0 += kRound) {
+            float2 ml[kRound];
+            float4 x[kRound];
+#pragma unroll
+            for (int k = 0; k < kRound; ++k) {
+                const float* at = parts + static_cast<std::size_t>(min(k0 + k, splits - 1)) * kPart;
+                ml[k] = __ldcg(reinterpret_cast<const float2*>(at + kCols * D + 2 * col));
+                x[k] = __ldcg(reinterpret_cast<const float4*>(at) + i);
+            }
+            float next = top;
+#pragma unroll
+            for (int k = 0; k < kRound; ++k) next = fmaxf(next, ml[k].x);
+            const float kept = ex2_ftz(top - next);
+            sum *= kept;
+            total.x *= kept, total.y *= kept, total.z *= kept, total.w *= kept;
+            top = next;
+#pragma unroll
+            for (int k = 0; k < kRound; ++k) {
+                const float w = k0 + k < splits ? ex2_ftz(ml[k].x - top) : 0.0f;
+                sum = fmaf(w, ml[k].y, sum);
+                total.x = fmaf(w, x[k].x, total.x);
+                total.y = fmaf(w, x[k].y, total.y);
+                total.z = fmaf(w, x[k].z, total.z);
+                total.w = fmaf(w, x[k].w, total.w);
+            }
         }
-        const float inv = split_weights[kCols * kMaxSplits + col];
+        const bool ok = isfinite(sum) && sum > 0.0f;
+        if (!ok) flag_error(p.error_word, kErrNormalizer);
+        const float inv = ok ? 1.0f / sum : 0.0f;
         QT* out = static_cast<QT*>(p.out) + row_of(col) * D + 4 * i % D;
         out[0] = Storage<QT>::from_float(total.x * inv);
         out[1] = Storage<QT>::from_float(total.y * inv);
@@ -720,7 +731,7 @@ void run_kv4(InferlabCudaKvPool& p, Kv4Params k, std::uint32_t query_dtype, std:
     k.kv_heads = p.kv_heads;
     k.group = k.q_heads / p.kv_heads;
     k.tiles_per_block = p.block_tokens / kv4::kTileTokens;
-    k.max_context = std::min<long long>(max_context_len, static_cast<long long>(k.max_blocks) * p.block_tokens);
+    k.max_context = static_cast<int>(std::min<long long>(max_context_len, static_cast<long long>(k.max_blocks) * p.block_tokens));
     k.column_tiles = plan.column_tiles;
     k.max_splits = plan.max_splits;
     k.tiles_per_split = plan.tiles_per_split;
