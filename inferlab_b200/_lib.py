@@ -238,3 +238,15 @@ def lib() -> ctypes.CDLL:
 def error_buffer(size: int = 512):
     """Same 512-byte error buffer the Rust facade passes (worker/src/lib.rs:40)."""
     return ctypes.create_string_buffer(size)
+
+
+_thread = threading.local()
+
+
+def call_error_buffer():
+    """A 512-byte error buffer of this thread, for calls whose time is the host's (the library
+    clears it on entry)."""
+    buffer = getattr(_thread, "error", None)
+    if buffer is None:
+        buffer = _thread.error = ctypes.create_string_buffer(512)
+    return buffer

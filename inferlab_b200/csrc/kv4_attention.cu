@@ -39,6 +39,7 @@
 #include "../../include/inferlab_attention.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -679,12 +680,26 @@ Kv4Plan plan_kv4(const InferlabCudaKvPool& p, std::uint32_t num_seqs, std::uint3
     const std::uint64_t units = checked_mul(checked_mul(num_seqs, p.kv_heads, "4-bit attention batch is too large"), column_tiles,
                                             "4-bit attention batch is too large");
     const std::uint32_t tiles = (max_context_len + kv4::kTileTokens - 1) / kv4::kTileTokens;
-    // About 2048 CTAs if every context were max_context_len long, each of at
-    // least 16 tiles (4 a warp).
     std::uint64_t per_split = p.decode_blocks_per_split;
     if (per_split == 0) {
-        const std::uint64_t splits = std::max<std::uint64_t>(1, 2048 / units);
-        per_split = std::max<std::uint64_t>(16, (tiles + splits - 1) / splits);
+        const std::uint64_t total = checked_mul(units, tiles, "4-bit attention batch is too large");
+        if (num_seqs == 1) {
+            // Units of one length: two CTAs an SM exactly (131072 tokens x 8
+            // kv-heads: 42 us; one or three an SM 60 and 53, four 46).
+            per_split = std::max<std::uint64_t>(8, (total + 295) / 296);
+        } else {
+            // The lengths are the device's: as if all were max_context_len long,
+            // two waves of four CTAs an SM (32 x zipf 8192: 103 tiles a split
+            // 41 us, 64 and 171 tiles 43 and 52). Where the units alone are two
+            // CTAs an SM a split costs more than it evens out below 128 tiles
+            // (64 x 64..2048: whole 20.6 us, 64 tiles 23.2), and above 256 one
+            // long context would be the tail; segments of many column tiles
+            // even that out themselves.
+            per_split = std::max<std::uint64_t>(total / 1184, units >= 296 ? 128 : 16);
+            per_split = std::min<std::uint64_t>(per_split, 256 * std::max<std::uint64_t>(1, column_tiles / 4));
+        }
+        const std::uint64_t splits = (tiles + per_split - 1) / per_split;
+        per_split = (tiles + splits - 1) / splits;
     }
     per_split = std::max<std::uint64_t>(per_split, (tiles + kMaxSplits - 1) / kMaxSplits);
     plan.tiles_per_split = static_cast<int>(per_split);
@@ -747,7 +762,13 @@ void run_kv4(InferlabCudaKvPool& p, Kv4Params k, std::uint32_t query_dtype, std:
             ? (plan.columns == 4 ? kv4_attention_kernel<RowT, QT, 128, true> : kv4_attention_kernel<RowT, QT, 128, false>)
             : (plan.columns == 4 ? kv4_attention_kernel<RowT, QT, 64, true> : kv4_attention_kernel<RowT, QT, 64, false>);
         const int smem = kWarps * kRing * kStep * kv4::tile_bytes(static_cast<int>(p.head_dim));
-        cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute");
+        static std::atomic<std::uint64_t> allowed[2][2];  // devices whose kernel may use it
+        auto& devices = allowed[p.head_dim == 128][plan.columns == 4];
+        const std::uint64_t bit = p.device < 64 ? 1ull << p.device : 0;
+        if ((devices.load() & bit) == 0) {
+            cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute");
+            devices.fetch_or(bit);
+        }
         kernel<<<grid, kWarps * 32, smem, s>>>(k);
     };
     if (p.dtype == kF16) {

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import weakref
 
 import torch
 
@@ -39,9 +40,11 @@ def _stream_handle(device: int, stream) -> ctypes.c_void_p:
 
 
 class _DeviceView:
-    """Exposes a raw device range through __cuda_array_interface__."""
+    """Exposes a raw device range through __cuda_array_interface__. The tensor made from it keeps
+    it, and so `owner`, whose memory it is, alive."""
 
-    def __init__(self, ptr: int, shape, typestr: str):
+    def __init__(self, ptr: int, shape, typestr: str, owner=None):
+        self.owner = owner
         self.__cuda_array_interface__ = {
             "shape": tuple(shape), "typestr": typestr, "data": (ptr, False), "version": 3,
             "strides": None,
@@ -58,6 +61,19 @@ def _require(tensor: torch.Tensor, name: str, dtype, device: int) -> torch.Tenso
     if not tensor.is_contiguous():
         raise AttentionError(f"{name} must be contiguous")
     return tensor
+
+
+def _expect(tensor, name: str, dtype, device: int) -> int:
+    """_require for the per-token calls, whose time is the host's: one pass over what a good
+    tensor satisfies, the messages only for others. Returns the address."""
+    if type(tensor) is not torch.Tensor or tensor.dtype is not dtype or \
+            tensor.get_device() != device or not tensor.is_contiguous():
+        _require(tensor, name, dtype, device)
+    return tensor.data_ptr()
+
+
+def _raw_stream(device: int, stream) -> int:
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
 
 
 class CudaKvPool:
@@ -99,6 +115,8 @@ class CudaKvPool:
         self._key_ptr = info.key_arena
         self._value_ptr = info.value_arena
         self._workspaces: dict = {}
+        self._views: dict = {}  # weak: a view keeps the pool, not the pool its views
+        self._kv4_workspaces: dict = {}  # (stream, batch shape) -> a workspace that fits it
 
     # -- lifetime -----------------------------------------------------------
     def close(self) -> None:
@@ -122,26 +140,32 @@ class CudaKvPool:
     @property
     def arena(self) -> torch.Tensor:
         """A 4-bit pool's packed arena as bytes [num_blocks][kv_heads][block_tokens / 16][tile]
-        (no copy; valid while the pool lives; the layout is in the C header)."""
+        (no copy; it keeps the pool alive, until close(); the layout is in the C header)."""
         if self.kv_bits != 4:
             raise AttentionError("only a 4-bit pool has a packed arena")
         tiles = self.block_tokens // 16
         shape = (self.num_blocks, self.kv_heads, tiles,
                  self.block_bytes // (self.kv_heads * tiles))
-        return torch.as_tensor(_DeviceView(self._key_ptr, shape, "|u1"),
+        return torch.as_tensor(_DeviceView(self._key_ptr, shape, "|u1", self),
                                device=f"cuda:{self.device}")
 
     def _arena(self, ptr: int) -> torch.Tensor:
         if self.kv_bits == 4:
             raise AttentionError("a 4-bit pool has one packed arena (arena)")
-        shape = (self.num_blocks, self.kv_heads, self.block_tokens, self.head_dim)
-        view = torch.as_tensor(_DeviceView(ptr, shape, _TYPESTR[self.dtype]),
-                               device=f"cuda:{self.device}")
-        return view.view(TORCH_DTYPES[self.dtype]) if self.dtype == KV_BF16 else view
+        known = self._views.get(ptr)
+        view = None if known is None else known()
+        if view is None:
+            shape = (self.num_blocks, self.kv_heads, self.block_tokens, self.head_dim)
+            view = torch.as_tensor(_DeviceView(ptr, shape, _TYPESTR[self.dtype], self),
+                                   device=f"cuda:{self.device}")
+            if self.dtype == KV_BF16:
+                view = view.view(TORCH_DTYPES[self.dtype])
+            self._views[ptr] = weakref.ref(view)
+        return view
 
     @property
     def key_arena(self) -> torch.Tensor:
-        """A torch view of the key arena (no copy; valid while the pool lives)."""
+        """A torch view of the key arena (no copy; it keeps the pool alive, until close())."""
         return self._arena(self._key_ptr)
 
     @property
@@ -183,18 +207,18 @@ class CudaKvPool:
     def _rows(self, tensor: torch.Tensor, name: str, dtype, heads: int | None) -> int:
         """Checks token rows [n][heads][head_dim], heads and dims contiguous (a view of a wider
         projection output is fine); returns the elements between rows."""
-        if not isinstance(tensor, torch.Tensor) or tensor.device.type != "cuda" or \
-                tensor.device.index != self.device:
+        if not isinstance(tensor, torch.Tensor) or tensor.get_device() != self.device:
             raise AttentionError(f"{name} must live on cuda:{self.device}")
-        if tensor.dtype != dtype:
+        if tensor.dtype is not dtype:
             raise AttentionError(f"{name} must have dtype {dtype}")
-        if tensor.dim() != 3 or tensor.shape[2] != self.head_dim or \
-                (heads is not None and tensor.shape[1] != heads):
+        shape = tensor.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or \
+                (heads is not None and shape[1] != heads):
             raise AttentionError("paged KV append shapes do not match the pool")
-        if tensor.numel() and (tensor.stride(2) != 1 or
-                               (tensor.shape[1] > 1 and tensor.stride(1) != self.head_dim)):
+        step, head, dim = tensor.stride()
+        if (dim != 1 or (shape[1] > 1 and head != self.head_dim)) and tensor.numel():
             raise AttentionError(f"{name} must have contiguous heads")
-        return tensor.stride(0)
+        return step
 
     def append_rotary(self, queries: torch.Tensor | None, key_rows: torch.Tensor,
                       value_rows: torch.Tensor, cos_sin: torch.Tensor | None,
@@ -211,50 +235,50 @@ class CudaKvPool:
         (inferlab_cuda_kv_append_rotary)."""
         dev = self.device
         dtype = key_rows.dtype
-        if dtype not in (torch.float32, TORCH_DTYPES[self.dtype]):
+        pool_dtype = TORCH_DTYPES[self.dtype]
+        if dtype is not torch.float32 and dtype is not pool_dtype:
             raise AttentionError("paged KV row dtype must be FP32 or the pool dtype")
-        call = _lib.InferlabCudaRotaryAppend()
-        call.key_stride = self._rows(key_rows, "key_rows", dtype, self.kv_heads)
-        call.value_stride = self._rows(value_rows, "value_rows", dtype, self.kv_heads)
+        key_stride = self._rows(key_rows, "key_rows", dtype, self.kv_heads)
+        value_stride = self._rows(value_rows, "value_rows", dtype, self.kv_heads)
         rows = key_rows.shape[0]
-        _require(row_sequences, "row_sequences", torch.int32, dev)
-        _require(positions, "positions", torch.int32, dev)
-        _require(block_tables, "block_tables", torch.int32, dev)
+        sequences_at = _expect(row_sequences, "row_sequences", torch.int32, dev)
+        positions_at = _expect(positions, "positions", torch.int32, dev)
+        tables_at = _expect(block_tables, "block_tables", torch.int32, dev)
         if value_rows.shape[0] != rows or row_sequences.numel() != rows or \
                 positions.numel() != rows or block_tables.dim() != 2:
             raise AttentionError("paged KV append shapes do not match the pool")
+        angles_at, angle_rows, rotary_dim = None, 0, 0
         if cos_sin is not None:
-            _require(cos_sin, "cos_sin", torch.float32, dev)
+            angles_at = _expect(cos_sin, "cos_sin", torch.float32, dev)
             if cos_sin.dim() != 2:
                 raise AttentionError("cos_sin must be [positions][rotary_dim]")
-            call.cos_sin = cos_sin.data_ptr()
-            call.cos_sin_positions, call.rotary_dim = cos_sin.shape
+            angle_rows, rotary_dim = cos_sin.shape
+        queries_at, query_stride, q_heads, out_at, out_type = None, 0, 0, None, 0
         if queries is not None:
-            call.query_stride = self._rows(queries, "queries", dtype, None)
+            query_stride = self._rows(queries, "queries", dtype, None)
             if queries.shape[0] != rows:
                 raise AttentionError("paged KV append shapes do not match the pool")
             if q_out is None:
                 q_out = torch.empty(queries.shape, dtype=dtype, device=queries.device)
-            _require(q_out, "q_out", None, dev)
+            out_dtype = q_out.dtype
+            out_at = _expect(q_out, "q_out", out_dtype, dev)
             if q_out.shape != queries.shape or \
-                    q_out.dtype not in (torch.float32, TORCH_DTYPES[self.dtype]):
+                    (out_dtype is not torch.float32 and out_dtype is not pool_dtype):
                 raise AttentionError("q_out must be shaped like the queries, FP32 or the pool dtype")
-            call.queries, call.q_out = queries.data_ptr(), q_out.data_ptr()
-            call.q_heads = queries.shape[1]
-            call.q_out_dtype = KV_FP32 if q_out.dtype == torch.float32 else self.dtype
+            queries_at, q_heads = queries.data_ptr(), queries.shape[1]
+            out_type = KV_FP32 if out_dtype is torch.float32 else self.dtype
         elif q_out is not None:
             raise AttentionError("q_out needs queries")
-        call.key_rows, call.value_rows = key_rows.data_ptr(), value_rows.data_ptr()
-        call.row_dtype = KV_FP32 if dtype == torch.float32 else self.dtype
-        call.interleaved = 1 if interleaved else 0
-        call.row_sequences, call.positions = row_sequences.data_ptr(), positions.data_ptr()
-        call.rows = rows
-        call.block_tables = block_tables.data_ptr()
-        call.num_seqs, call.max_blocks_per_seq = block_tables.shape
-        error = _lib.error_buffer()
-        _check(self._lib.inferlab_cuda_kv_append_rotary(
-            self._handle, ctypes.byref(call), _stream_handle(dev, stream), error, len(error)),
-            error)
+        call = _lib.InferlabCudaRotaryAppend(
+            queries_at, key_rows.data_ptr(), value_rows.data_ptr(),
+            KV_FP32 if dtype is torch.float32 else self.dtype, q_heads, query_stride, key_stride,
+            value_stride, angles_at, angle_rows, rotary_dim, 1 if interleaved else 0, sequences_at,
+            positions_at, rows, tables_at, block_tables.shape[0], block_tables.shape[1], out_at,
+            out_type, 0)
+        error = _lib.call_error_buffer()
+        if self._lib.inferlab_cuda_kv_append_rotary(self._handle, ctypes.byref(call),
+                                                    _raw_stream(dev, stream), error, 512):
+            raise AttentionError(error.value.decode())
         return q_out
 
     def project_append(self, hidden: torch.Tensor, weights: torch.Tensor, q_heads: int,
@@ -342,20 +366,20 @@ class CudaKvPool:
         pool's type (a 4-bit pool's row type). Rows of sequence -1 are padding and left unset
         (inferlab_cuda_kv_gather_rows)."""
         dev = self.device
-        _require(row_sequences, "row_sequences", torch.int32, dev)
-        _require(positions, "positions", torch.int32, dev)
-        _require(block_tables, "block_tables", torch.int32, dev)
+        sequences_at = _expect(row_sequences, "row_sequences", torch.int32, dev)
+        positions_at = _expect(positions, "positions", torch.int32, dev)
+        tables_at = _expect(block_tables, "block_tables", torch.int32, dev)
         rows = row_sequences.numel()
         if positions.numel() != rows or block_tables.dim() != 2:
             raise AttentionError("paged KV gather shapes do not match")
-        keys = torch.empty((rows, self.kv_heads, self.head_dim), dtype=TORCH_DTYPES[self.dtype],
-                           device=f"cuda:{dev}")
-        values = torch.empty_like(keys)
-        error = _lib.error_buffer()
-        _check(self._lib.inferlab_cuda_kv_gather_rows(
-            self._handle, _vp(row_sequences), _vp(positions), rows, _vp(block_tables),
-            block_tables.shape[0], block_tables.shape[1], _vp(keys), _vp(values),
-            _stream_handle(dev, stream), error, len(error)), error)
+        keys, values = torch.empty((2, rows, self.kv_heads, self.head_dim),
+                                   dtype=TORCH_DTYPES[self.dtype], device=positions.device).unbind()
+        error = _lib.call_error_buffer()
+        if self._lib.inferlab_cuda_kv_gather_rows(
+                self._handle, sequences_at, positions_at, rows, tables_at, block_tables.shape[0],
+                block_tables.shape[1], keys.data_ptr(), values.data_ptr(),
+                _raw_stream(dev, stream), error, 512):
+            raise AttentionError(error.value.decode())
         return keys, values
 
     def workspace_size(self, num_seqs: int, q_heads: int, max_context_len: int,
@@ -381,6 +405,7 @@ class CudaKvPool:
         """Fixes later decodes' split length at blocks_per_split 16-token
         blocks (0: the planner chooses, the default). A tuning and test knob
         (inferlab_cuda_pool_set_decode_split)."""
+        self._kv4_workspaces.clear()
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_pool_set_decode_split(
             self._handle, int(blocks_per_split), error, len(error)), error)
@@ -552,85 +577,99 @@ class CudaKvPool:
         return out
 
     def _kv4_operands(self, queries, out):
-        """The query / output type code and the output of a 4-bit attention call."""
-        if queries.dtype not in (torch.float32, TORCH_DTYPES[self.dtype]):
+        """The query / output type code, the addresses, and the output of a 4-bit attention call."""
+        dtype = queries.dtype
+        if dtype is not torch.float32 and dtype is not TORCH_DTYPES[self.dtype]:
             raise AttentionError("4-bit attention query dtype must be FP32 or the pool's row type")
-        _require(queries, "queries", queries.dtype, self.device)
+        queries_at = _expect(queries, "queries", dtype, self.device)
         if queries.dim() != 3 or queries.shape[2] != self.head_dim:
             raise AttentionError("4-bit attention shapes do not match the pool")
         if out is None:
             out = torch.empty_like(queries)
-        _require(out, "out", queries.dtype, self.device)
-        if out.shape != queries.shape:
-            raise AttentionError("4-bit attention output must be shaped like the queries")
-        return KV_FP32 if queries.dtype == torch.float32 else self.dtype, out
+            out_at = out.data_ptr()
+        else:
+            out_at = _expect(out, "out", dtype, self.device)
+            if out.shape != queries.shape:
+                raise AttentionError("4-bit attention output must be shaped like the queries")
+        return KV_FP32 if dtype is torch.float32 else self.dtype, queries_at, out_at, out
 
-    def _kv4_workspace(self, num_seqs, q_heads, max_query_count, max_context_len, stream):
-        """The pool's workspace of the stream; a capture gets its own, so that two graphs that
-        are replayed side by side never share one."""
+    def _kv4_workspace(self, raw, stream, *shape):
+        """The pool's workspace of the stream, for a batch shape (num_seqs, q_heads,
+        max_query_count, max_context_len). A capture gets its own, so that two graphs that are
+        replayed side by side never share one."""
+        if stream is None and not torch.cuda.is_current_stream_capturing():
+            known = self._kv4_workspaces.get((raw, *shape))
+            if known is not None:
+                return known
+        num_seqs, q_heads, queries, context = shape
         used = stream if stream is not None else torch.cuda.current_stream(self.device)
-        with torch.cuda.stream(used):
+        with torch.cuda.stream(used):  # the allocation belongs to that stream
             if torch.cuda.is_current_stream_capturing():
-                return self.make_workspace(num_seqs, q_heads, max_context_len, used,
-                                           max_query_count)
-            need = self.workspace_size(num_seqs, q_heads, max_context_len, max_query_count)
-            ws = self._workspaces.get(used.cuda_stream)
-            if ws is None or ws.numel() < need:
-                ws = self.make_workspace(num_seqs, q_heads, max_context_len, used,
-                                         max_query_count)
-                self._workspaces[used.cuda_stream] = ws
+                return self.make_workspace(num_seqs, q_heads, context, used, queries)
+            ws = self._workspaces.get(raw)
+            if ws is None or ws.numel() < self.workspace_size(num_seqs, q_heads, context, queries):
+                ws = self.make_workspace(num_seqs, q_heads, context, used, queries)
+                self._workspaces[raw] = ws
+                self._kv4_workspaces.clear()  # nothing keeps the outgrown one
+            if len(self._kv4_workspaces) > 1024:
+                self._kv4_workspaces.clear()
+            self._kv4_workspaces[(raw, *shape)] = ws
             return ws
 
     def _kv4_decode(self, queries, block_tables, context_lens, max_context_len, out, workspace,
                     stream):
         dev = self.device
-        query_type, out = self._kv4_operands(queries, out)
-        _require(block_tables, "block_tables", torch.int32, dev)
-        _require(context_lens, "context_lens", torch.int32, dev)
+        query_type, queries_at, out_at, out = self._kv4_operands(queries, out)
+        tables_at = _expect(block_tables, "block_tables", torch.int32, dev)
+        lens_at = _expect(context_lens, "context_lens", torch.int32, dev)
         num_seqs, q_heads, _ = queries.shape
-        if context_lens.numel() != num_seqs or block_tables.dim() != 2 or \
-                block_tables.shape[0] != num_seqs:
+        table_shape = block_tables.shape
+        if context_lens.numel() != num_seqs or len(table_shape) != 2 or table_shape[0] != num_seqs:
             raise AttentionError("4-bit attention shapes do not match the pool")
         if num_seqs == 0:
             return out
         if max_context_len is None:
             max_context_len = max(1, int(context_lens.max().item()))
+        raw = _raw_stream(dev, stream)
         if workspace is None:
-            workspace = self._kv4_workspace(num_seqs, q_heads, 1, max_context_len, stream)
-        _require(workspace, "workspace", torch.uint8, dev)
-        error = _lib.error_buffer()
-        _check(self._lib.inferlab_cuda_kv4_decode(
-            self._handle, _vp(queries), query_type, _vp(block_tables), block_tables.shape[1],
-            _vp(context_lens), num_seqs, q_heads, max_context_len, _vp(out), _vp(workspace),
-            workspace.numel(), _stream_handle(dev, stream), error, len(error)), error)
+            workspace = self._kv4_workspace(raw, stream, num_seqs, q_heads, 1, max_context_len)
+        workspace_at = _expect(workspace, "workspace", torch.uint8, dev)
+        error = _lib.call_error_buffer()
+        if self._lib.inferlab_cuda_kv4_decode(
+                self._handle, queries_at, query_type, tables_at, table_shape[1], lens_at, num_seqs,
+                q_heads, max_context_len, out_at, workspace_at, workspace.numel(), raw, error, 512):
+            raise AttentionError(error.value.decode())
         return out
 
     def _kv4_prefill(self, queries, block_tables, query_starts, query_counts, query_offsets,
                      max_query_count, out, stream, max_context_len, workspace):
         dev = self.device
-        query_type, out = self._kv4_operands(queries, out)
+        query_type, queries_at, out_at, out = self._kv4_operands(queries, out)
         segments = query_starts.numel()
-        for name, t in (("block_tables", block_tables), ("query_starts", query_starts),
-                        ("query_counts", query_counts), ("query_offsets", query_offsets)):
-            _require(t, name, torch.int32, dev)
-        if block_tables.dim() != 2 or block_tables.shape[0] != segments or \
+        tables_at = _expect(block_tables, "block_tables", torch.int32, dev)
+        starts_at = _expect(query_starts, "query_starts", torch.int32, dev)
+        counts_at = _expect(query_counts, "query_counts", torch.int32, dev)
+        offsets_at = _expect(query_offsets, "query_offsets", torch.int32, dev)
+        table_shape = block_tables.shape
+        if len(table_shape) != 2 or table_shape[0] != segments or \
                 query_counts.numel() != segments or query_offsets.numel() != segments:
             raise AttentionError("4-bit attention shapes do not match the pool")
         total, q_heads, _ = queries.shape
         if segments == 0 or total == 0:
             return out
         if max_context_len is None:
-            max_context_len = min(block_tables.shape[1] * self.block_tokens, 0x7fffff00)
+            max_context_len = min(table_shape[1] * self.block_tokens, 0x7fffff00)
+        raw = _raw_stream(dev, stream)
         if workspace is None:
-            workspace = self._kv4_workspace(segments, q_heads, max_query_count, max_context_len,
-                                            stream)
-        _require(workspace, "workspace", torch.uint8, dev)
-        error = _lib.error_buffer()
-        _check(self._lib.inferlab_cuda_kv4_prefill(
-            self._handle, _vp(queries), query_type, _vp(block_tables), block_tables.shape[1],
-            _vp(query_starts), _vp(query_counts), _vp(query_offsets), segments, q_heads,
-            max_query_count, total, max_context_len, _vp(out), _vp(workspace), workspace.numel(),
-            _stream_handle(dev, stream), error, len(error)), error)
+            workspace = self._kv4_workspace(raw, stream, segments, q_heads, max_query_count,
+                                            max_context_len)
+        workspace_at = _expect(workspace, "workspace", torch.uint8, dev)
+        error = _lib.call_error_buffer()
+        if self._lib.inferlab_cuda_kv4_prefill(
+                self._handle, queries_at, query_type, tables_at, table_shape[1], starts_at,
+                counts_at, offsets_at, segments, q_heads, max_query_count, total, max_context_len,
+                out_at, workspace_at, workspace.numel(), raw, error, 512):
+            raise AttentionError(error.value.decode())
         return out
 
 

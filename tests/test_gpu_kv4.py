@@ -511,6 +511,26 @@ def test_cache_beyond_32_bit_offsets(torch, kv4, il):
     pool.close()
 
 
+def test_views_keep_their_pool(torch, il):
+    """An arena outlives the name of its pool: its memory goes with the last view."""
+    import gc
+    import weakref
+
+    for bits in (None, 4):
+        pool = il.CudaKvPool(0, 2, 4, 16, 2, 64, kv_bits=bits)
+        alive = weakref.ref(pool)
+        view = pool.arena if bits else pool.key_arena
+        if bits is None:
+            assert pool.key_arena is view
+        view.fill_(3)
+        del pool
+        gc.collect()
+        assert alive() is not None and bool((view == 3).all())
+        del view
+        gc.collect()
+        assert alive() is None
+
+
 def test_pages_copied_and_shared(torch, il, kv4):
     """The page manager's copy on write moves a 4-bit block, and counts its bytes."""
     from inferlab_b200.pages import PageManager, copy_blocks
