@@ -192,6 +192,175 @@ __global__ void __launch_bounds__(kRowThreads) rotary_append_kernel(const Append
     }
 }
 
+// Eight consecutive elements as fp32, 16 bytes a load.
+template <typename T>
+__device__ __forceinline__ void load8(const T* at, float (&x)[8]) {
+    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+    for (int c = 0; c < 8 / kPer; ++c) widen16(reinterpret_cast<const uint4*>(at)[c], &x[c * kPer], T{});
+}
+template <typename T>
+struct Eight {
+    uint4 words[8 * sizeof(T) / 16];
+};
+// Rounded to T; `bad` where a value is not finite after it.
+template <typename T>
+__device__ __forceinline__ Eight<T> round8(const float (&x)[8], bool& bad) {
+    Eight<T> e;
+    T* t = reinterpret_cast<T*>(e.words);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        t[i] = Storage<T>::from_float(x[i]);
+        bad |= !isfinite(Storage<T>::to_float(t[i]));
+    }
+    return e;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* at, const Eight<T>& e) {
+#pragma unroll
+    for (int c = 0; c < static_cast<int>(8 * sizeof(T) / 16); ++c) reinterpret_cast<uint4*>(at)[c] = e.words[c];
+}
+
+// The common shapes: units of 8 dims, 16-byte accesses. One CTA per row; a
+// thread keeps to one unit of the head (its angles stay in registers) and goes
+// through the heads, blockDim / (head_dim / 8) at a time: the row's K and V in
+// at most kPasses rounds, held until the whole row is known to be good, then
+// its Q. The partner dims of a split rotation are loaded a second time (they
+// are in L1; exchanging them by shuffles takes four instructions).
+// Bound by HBM: 8192 rows of 32 + 8 + 8 bf16 heads x 128 move 12 KB in and 8 KB
+// (+ 2.3 KB a row in 4 bits) out each.
+template <typename RowT, typename PoolT, typename OutT, bool kFourBit, int kPasses>
+__global__ void __launch_bounds__(kRowThreads) rotary_append_vector_kernel(const AppendParams p) {
+    const std::size_t row = blockIdx.x;
+    const std::uint32_t d = p.head_dim, units = d / 8;
+    const std::uint32_t u = threadIdx.x % units, h0 = threadIdx.x / units, heads = blockDim.x / units;
+    const RowT* key_row = static_cast<const RowT*>(p.keys) + row * p.k_stride + 8 * u;
+    const RowT* value_row = static_cast<const RowT*>(p.values) + row * p.v_stride + 8 * u;
+    const bool turns = 8 * u < p.rotary_dim;
+    const std::uint32_t half = p.rotary_dim / 2;
+    const int partner = !turns || p.interleaved ? 0 : (8 * u < half ? static_cast<int>(half) : -static_cast<int>(half));
+
+    // The row's K and V are asked for while its place is looked up.
+    float k[kPasses][8], k2[kPasses][8], v[kPasses][8];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+        const std::uint32_t h = min(h0 + i * heads, p.kv_heads - 1);
+        load8(key_row + static_cast<std::size_t>(h) * d, k[i]);
+        if (partner != 0) load8(key_row + static_cast<std::size_t>(h) * d + partner, k2[i]);
+        load8(value_row + static_cast<std::size_t>(h) * d, v[i]);
+    }
+    std::uint32_t error = 0;
+    const Place place = find_place(p.row_sequences[row], p.positions[row], p.tables, p.num_seqs,
+                                   p.max_blocks, p.block_tokens, p.num_blocks, p.cos_sin_positions,
+                                   p.padded_rows, error);
+    if (error != 0 || place.block < 0) {
+        if (error != 0 && threadIdx.x == 0) flag_error(p.error_word, error);
+        return;
+    }
+    // Element i turns to x[i] c[i] + y[i] s[i], y the partners, the first of a
+    // pair with the sine's sign changed (exact).
+    float c[8], s[8];
+    if (turns) {
+        const float* angles = p.cos_sin + static_cast<std::size_t>(place.position) * p.rotary_dim;
+        if (p.interleaved) {
+            const float4 cs = *reinterpret_cast<const float4*>(angles + 4 * u);
+            const float4 sn = *reinterpret_cast<const float4*>(angles + half + 4 * u);
+            c[0] = c[1] = cs.x, c[2] = c[3] = cs.y, c[4] = c[5] = cs.z, c[6] = c[7] = cs.w;
+            s[1] = sn.x, s[3] = sn.y, s[5] = sn.z, s[7] = sn.w;
+            s[0] = -sn.x, s[2] = -sn.y, s[4] = -sn.z, s[6] = -sn.w;
+        } else {
+            const std::uint32_t pair = 8 * u < half ? 8 * u : 8 * u - half;
+            load8(angles + pair, c);
+            load8(angles + half + pair, s);
+            if (8 * u < half) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[i] = -s[i];
+            }
+        }
+    }
+    auto turn = [&](float (&x)[8], const float (&y)[8]) {
+        if (!turns) return;
+        float out[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            out[i] = __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(p.interleaved ? x[i ^ 1] : y[i], s[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = out[i];
+    };
+
+    bool bad = false;
+    if constexpr (kFourBit) {
+        std::uint32_t words[kPasses][2];
+        __half2 pairs[kPasses][2];
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            turn(k[i], k2[i]);
+            const bool live = h0 + i * heads < p.kv_heads;
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                float (&x)[8] = which ? v[i] : k[i];
+                bool out_of_range;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = Storage<PoolT>::to_float(Storage<PoolT>::from_float(x[e]));
+                words[i][which] = kv4::quantise(x, pairs[i][which], out_of_range);
+                bad |= live && out_of_range;
+            }
+        }
+        if (__syncthreads_or(bad)) {
+            if (threadIdx.x == 0) flag_error(p.error_word, kErrNonFinite);
+            return;
+        }
+        const std::size_t tiles_per_head = p.block_tokens / kv4::kTileTokens;
+        const int slot = static_cast<int>(place.slot % kv4::kTileTokens), dd = static_cast<int>(d), uu = static_cast<int>(u);
+        unsigned char* tile0 = p.key_arena +
+            (static_cast<std::size_t>(place.block) * p.kv_heads * tiles_per_head + place.slot / kv4::kTileTokens) * kv4::tile_bytes(dd);
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const std::uint32_t h = h0 + i * heads;
+            if (h >= p.kv_heads) break;
+            unsigned char* tile = tile0 + h * tiles_per_head * kv4::tile_bytes(dd);
+            *reinterpret_cast<std::uint32_t*>(tile + kv4::key_word(dd, slot, uu)) = words[i][0];
+            *reinterpret_cast<std::uint32_t*>(tile + kv4::value_word(dd, slot, uu)) = words[i][1];
+            if (u % 8 < 2) {
+                *reinterpret_cast<__half2*>(tile + kv4::pair_at(dd, slot, uu / 8, uu % 8)) = uu % 8 == 0 ? pairs[i][0] : pairs[i][1];
+            }
+        }
+    } else {
+        Eight<PoolT> held[kPasses][2];
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            turn(k[i], k2[i]);
+            held[i][0] = round8<PoolT>(k[i], bad);
+            held[i][1] = round8<PoolT>(v[i], bad);
+        }
+        if (__syncthreads_or(bad)) {
+            if (threadIdx.x == 0) flag_error(p.error_word, kErrNonFinite);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const std::uint32_t h = h0 + i * heads;
+            if (h >= p.kv_heads) break;
+            const std::size_t dst =
+                ((static_cast<std::size_t>(place.block) * p.kv_heads + h) * p.block_tokens + place.slot) * d + 8 * u;
+            store8(reinterpret_cast<PoolT*>(p.key_arena) + dst, held[i][0]);
+            store8(reinterpret_cast<PoolT*>(p.value_arena) + dst, held[i][1]);
+        }
+    }
+    if (p.queries == nullptr) return;
+    const RowT* q_row = static_cast<const RowT*>(p.queries) + row * p.q_stride + 8 * u;
+    OutT* out = static_cast<OutT*>(p.q_out) + row * p.q_heads * d + 8 * u;
+#pragma unroll 4
+    for (std::uint32_t h = h0; h < p.q_heads; h += heads) {
+        float x[8], y[8];
+        load8(q_row + static_cast<std::size_t>(h) * d, x);
+        if (partner != 0) load8(q_row + static_cast<std::size_t>(h) * d + partner, y);
+        turn(x, y);
+        store8(out + static_cast<std::size_t>(h) * d, round8<OutT>(x, bad));
+    }
+}
+
 struct GatherParams {
     const unsigned char* key_arena;
     const unsigned char* value_arena;
@@ -205,7 +374,52 @@ struct GatherParams {
     std::uint32_t* error_word;
 };
 
-// One CTA per row. Words of the pool's own element type are copied bit for
+// The common shapes of a gather: units of 8 dims, 16-byte accesses; a 4-bit
+// pool's unit is one word of codes and its group's pair.
+template <typename T, bool kFourBit>
+__global__ void __launch_bounds__(kRowThreads) gather_rows_vector_kernel(const GatherParams p) {
+    const std::size_t row = blockIdx.x;
+    std::uint32_t error = 0;
+    const Place place = find_place(p.row_sequences != nullptr ? p.row_sequences[row] : 0,
+                                   p.positions != nullptr ? p.positions[row] : static_cast<std::int32_t>(row),
+                                   p.tables, p.num_seqs, p.max_blocks, p.block_tokens, p.num_blocks,
+                                   ~0ull, p.row_sequences != nullptr, error);
+    if (place.block < 0) {
+        if (error != 0 && threadIdx.x == 0) flag_error(p.error_word, error);
+        return;
+    }
+    const std::uint32_t units = p.head_dim / 8, all = p.kv_heads * units;
+    for (std::uint32_t i = threadIdx.x; i < 2 * all; i += blockDim.x) {
+        const bool is_value = i >= all;
+        const std::uint32_t unit = is_value ? i - all : i, head = unit / units, u = unit % units;
+        T* out = static_cast<T*>(is_value ? p.values_out : p.keys_out) + (row * all + unit) * 8;
+        if constexpr (kFourBit) {
+            const float most = std::is_same<T, __half>::value ? 65504.0f : 3.3895313892515355e38f;
+            const std::uint32_t tiles_per_head = p.block_tokens / kv4::kTileTokens;
+            const int slot = static_cast<int>(place.slot % kv4::kTileTokens), dd = static_cast<int>(p.head_dim);
+            const unsigned char* tile = p.key_arena +
+                ((static_cast<std::size_t>(place.block) * p.kv_heads + head) * tiles_per_head +
+                 place.slot / kv4::kTileTokens) * kv4::tile_bytes(dd);
+            const std::uint32_t word = *reinterpret_cast<const std::uint32_t*>(
+                tile + (is_value ? kv4::value_word(dd, slot, u) : kv4::key_word(dd, slot, u)));
+            const float2 pair = kv4::load_pair(tile, kv4::pair_at(dd, slot, u / 8, is_value));
+            float x[8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) x[n] = fminf(fmaxf(kv4::code_value(word, n, pair), -most), most);
+            bool bad = false;
+            store8(out, round8<T>(x, bad));
+        } else {
+            const T* at = reinterpret_cast<const T*>(is_value ? p.value_arena : p.key_arena) +
+                ((static_cast<std::size_t>(place.block) * p.kv_heads + head) * p.block_tokens + place.slot) * p.head_dim + 8 * u;
+            Eight<T> e;
+#pragma unroll
+            for (int c = 0; c < static_cast<int>(8 * sizeof(T) / 16); ++c) e.words[c] = reinterpret_cast<const uint4*>(at)[c];
+            store8(out, e);
+        }
+    }
+}
+
+// Any shape, one CTA per row. Words of the pool's own element type are copied bit for
 // bit; a 4-bit pool's codes are widened and rounded to its row type T,
 // saturating at T's largest finite value.
 template <typename T, bool kFourBit>
@@ -255,9 +469,41 @@ __global__ void __launch_bounds__(kRowThreads) gather_rows_kernel(const GatherPa
     }
 }
 
+template <typename RowT, typename PoolT, typename OutT, bool kFourBit>
+void launch_vector(const AppendParams& a, unsigned grid, unsigned threads, std::uint32_t passes, cudaStream_t s) {
+    if (passes == 1) rotary_append_vector_kernel<RowT, PoolT, OutT, kFourBit, 1><<<grid, threads, 0, s>>>(a);
+    else if (passes == 2) rotary_append_vector_kernel<RowT, PoolT, OutT, kFourBit, 2><<<grid, threads, 0, s>>>(a);
+    else rotary_append_vector_kernel<RowT, PoolT, OutT, kFourBit, 4><<<grid, threads, 0, s>>>(a);
+}
+
+bool aligned16(const void* at) { return reinterpret_cast<std::uintptr_t>(at) % 16 == 0; }
+
 template <typename RowT, typename PoolT, typename OutT>
 void launch_rotary(const AppendParams& a, std::uint64_t rows, bool four_bit, cudaStream_t s) {
     const unsigned grid = static_cast<unsigned>(rows);
+    // The vector kernel's conditions: whole 8-dim units whose partners are whole
+    // units too, every access on 16 bytes, and the row's K/V heads within four
+    // rounds of the CTA (32 heads x 128 need two).
+    const std::uint32_t units = a.head_dim / 8;
+    const std::uint64_t step = 16 / sizeof(RowT);
+    if (a.head_dim % 8 == 0 && units <= kRowThreads && a.rotary_dim % (a.interleaved ? 8 : 16) == 0 &&
+        aligned16(a.keys) && aligned16(a.values) && a.k_stride % step == 0 && a.v_stride % step == 0 &&
+        (a.queries == nullptr || (aligned16(a.queries) && aligned16(a.q_out) && a.q_stride % step == 0)) &&
+        (a.rotary_dim == 0 || aligned16(a.cos_sin))) {
+        std::uint32_t heads = std::min<std::uint32_t>(kRowThreads / units, std::max(a.q_heads, a.kv_heads));
+        while (four_bit && heads * units % 32 != 0) ++heads;  // whole warps: the groups' minima are shuffled
+        const std::uint32_t passes = (a.kv_heads + heads - 1) / heads;
+        if (passes <= 4) {
+            if constexpr (!std::is_same<PoolT, float>::value) {
+                if (four_bit) {
+                    launch_vector<RowT, PoolT, OutT, true>(a, grid, heads * units, passes, s);
+                    return;
+                }
+            }
+            launch_vector<RowT, PoolT, OutT, false>(a, grid, heads * units, passes, s);
+            return;
+        }
+    }
     if constexpr (!std::is_same<PoolT, float>::value) {
         if (four_bit) {
             rotary_append_kernel<RowT, PoolT, OutT, true><<<grid, kRowThreads, 0, s>>>(a);
@@ -301,15 +547,23 @@ void run_gather_rows(InferlabCudaKvPool& p, const std::int32_t* row_sequences,
     g.values_out = values_out;
     g.error_word = p.error_word;
     const unsigned grid = static_cast<unsigned>(rows);
-    if (p.dtype == kFp32) {
-        gather_rows_kernel<float, false><<<grid, kRowThreads, 0, s>>>(g);
-    } else if (p.dtype == kF16) {
-        if (p.kv_bits != 0) gather_rows_kernel<__half, true><<<grid, kRowThreads, 0, s>>>(g);
-        else gather_rows_kernel<__half, false><<<grid, kRowThreads, 0, s>>>(g);
-    } else {
-        if (p.kv_bits != 0) gather_rows_kernel<__nv_bfloat16, true><<<grid, kRowThreads, 0, s>>>(g);
-        else gather_rows_kernel<__nv_bfloat16, false><<<grid, kRowThreads, 0, s>>>(g);
-    }
+    const bool whole = p.head_dim % 8 == 0 && aligned16(keys_out) && aligned16(values_out) &&
+                       static_cast<std::uint64_t>(p.kv_heads) * p.head_dim < 0x7FFFFFFFull;
+    auto launch = [&](auto type) {
+        using T = decltype(type);
+        if constexpr (!std::is_same<T, float>::value) {
+            if (p.kv_bits != 0) {
+                auto* kernel = whole ? gather_rows_vector_kernel<T, true> : gather_rows_kernel<T, true>;
+                kernel<<<grid, kRowThreads, 0, s>>>(g);
+                return;
+            }
+        }
+        auto* kernel = whole ? gather_rows_vector_kernel<T, false> : gather_rows_kernel<T, false>;
+        kernel<<<grid, kRowThreads, 0, s>>>(g);
+    };
+    if (p.dtype == kFp32) launch(float{});
+    else if (p.dtype == kF16) launch(__half{});
+    else launch(__nv_bfloat16{});
     cuda_check(cudaGetLastError(), "gather rows launch");
 }
 
