@@ -42,6 +42,9 @@ struct AppendParams {
     const std::int32_t* tables;
     std::uint32_t num_seqs, max_blocks, block_tokens;
     std::uint64_t num_blocks;
+    // Vector kernel: CTA threads per head round, and the Q items of a head; by_*
+    // divide a thread number (< 256) as (t * by) >> 16.
+    std::uint32_t heads, by_units, items, by_items, q_step;
     void* q_out;
     unsigned char* key_arena;  // 4-bit pools: the packed arena
     unsigned char* value_arena;
@@ -203,17 +206,36 @@ template <typename T>
 struct Eight {
     uint4 words[8 * sizeof(T) / 16];
 };
-// Rounded to T; `bad` where a value is not finite after it.
+__device__ __forceinline__ std::uint32_t round_pair(float low, float high, __half) {
+    const __half2 v = __floats2half2_rn(low, high);
+    return *reinterpret_cast<const std::uint32_t*>(&v);
+}
+__device__ __forceinline__ std::uint32_t round_pair(float low, float high, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(low, high);
+    return *reinterpret_cast<const std::uint32_t*>(&v);
+}
+// Rounded to T.
 template <typename T>
-__device__ __forceinline__ Eight<T> round8(const float (&x)[8], bool& bad) {
+__device__ __forceinline__ Eight<T> round8(const float (&x)[8]) {
     Eight<T> e;
-    T* t = reinterpret_cast<T*>(e.words);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        t[i] = Storage<T>::from_float(x[i]);
-        bad |= !isfinite(Storage<T>::to_float(t[i]));
+    if constexpr (sizeof(T) == 4) {
+        e.words[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+        e.words[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
+    } else {
+        e.words[0] = make_uint4(round_pair(x[0], x[1], T{}), round_pair(x[2], x[3], T{}), round_pair(x[4], x[5], T{}),
+                                round_pair(x[6], x[7], T{}));
     }
     return e;
+}
+// Whether a value rounds to something T cannot hold as a finite number (a NaN
+// compares false): from half a unit above T's largest.
+template <typename T>
+__device__ __forceinline__ bool outside8(const float (&x)[8]) {
+    const float limit = sizeof(T) == 4 ? INFINITY : std::is_same<T, __half>::value ? 65520.0f : __uint_as_float(0x7f7f8000u);
+    bool out = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out |= !(fabsf(x[i]) < limit);
+    return out;
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* at, const Eight<T>& e) {
@@ -221,34 +243,85 @@ __device__ __forceinline__ void store8(T* at, const Eight<T>& e) {
     for (int c = 0; c < static_cast<int>(8 * sizeof(T) / 16); ++c) reinterpret_cast<uint4*>(at)[c] = e.words[c];
 }
 
-// The common shapes: units of 8 dims, 16-byte accesses. One CTA per row; a
-// thread keeps to one unit of the head (its angles stay in registers) and goes
-// through the heads, blockDim / (head_dim / 8) at a time: the row's K and V in
-// at most kPasses rounds, held until the whole row is known to be good, then
-// its Q. The partner dims of a split rotation are loaded a second time (they
-// are in L1; exchanging them by shuffles takes four instructions).
+// out = x c + y s, y the pair's other elements and s with the first one's sine
+// negated (exact): each product and the sum rounded once, two lanes a time.
+__device__ __forceinline__ void turn8(float (&x)[8], const float (&y)[8], const float (&c)[8], const float (&s)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float2 own = kv4::mul2(make_float2(x[i], x[i + 1]), make_float2(c[i], c[i + 1]));
+        const float2 other = kv4::mul2(make_float2(y[i], y[i + 1]), make_float2(s[i], s[i + 1]));
+        x[i] = __fadd_rn(own.x, other.x), x[i + 1] = __fadd_rn(own.y, other.y);
+    }
+}
+// Both halves of split pairs: a' = a c - b s, b' = b c + a s.
+__device__ __forceinline__ void turn8_both(float (&a)[8], float (&b)[8], const float (&c)[8], const float (&s)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float2 x = make_float2(a[i], a[i + 1]), y = make_float2(b[i], b[i + 1]);
+        const float2 cc = make_float2(c[i], c[i + 1]), ss = make_float2(s[i], s[i + 1]);
+        const float2 xc = kv4::mul2(x, cc), ys = kv4::mul2(y, ss), yc = kv4::mul2(y, cc), xs = kv4::mul2(x, ss);
+        a[i] = __fsub_rn(xc.x, ys.x), a[i + 1] = __fsub_rn(xc.y, ys.y);
+        b[i] = __fadd_rn(yc.x, xs.x), b[i + 1] = __fadd_rn(yc.y, xs.y);
+    }
+}
+// Interleaved: c and s hold four angles, the pairs are neighbours.
+__device__ __forceinline__ void turn8_neighbours(float (&x)[8], const float (&c)[8], const float (&s)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = x[2 * i], b = x[2 * i + 1];
+        x[2 * i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
+        x[2 * i + 1] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
+    }
+}
+
+// The common shapes: units of 8 dims, 16-byte accesses. One CTA per row.
+// K and V: a thread keeps to one unit of the head and goes through the heads,
+// blockDim / (head_dim / 8) at a time, in at most kPasses rounds, held until the
+// whole row is known to be good; in a 4-bit pool eight neighbours then hold a
+// group. The partner dims of a split rotation are loaded a second time (from
+// L1). Q: a thread takes both units of a pair, so nothing is loaded or widened
+// twice; the first round is asked for at the start.
 // Bound by HBM: 8192 rows of 32 + 8 + 8 bf16 heads x 128 move 12 KB in and 8 KB
 // (+ 2.3 KB a row in 4 bits) out each.
-template <typename RowT, typename PoolT, typename OutT, bool kFourBit, int kPasses>
+template <typename RowT, typename PoolT, typename OutT, bool kFourBit, bool kNeighbours, int kPasses>
 __global__ void __launch_bounds__(kRowThreads) rotary_append_vector_kernel(const AppendParams p) {
     const std::size_t row = blockIdx.x;
-    const std::uint32_t d = p.head_dim, units = d / 8;
-    const std::uint32_t u = threadIdx.x % units, h0 = threadIdx.x / units, heads = blockDim.x / units;
+    const std::uint32_t d = p.head_dim, units = d / 8, half = p.rotary_dim / 2;
+    const std::uint32_t h0 = (threadIdx.x * p.by_units) >> 16, u = threadIdx.x - h0 * units, heads = p.heads;
     const RowT* key_row = static_cast<const RowT*>(p.keys) + row * p.k_stride + 8 * u;
     const RowT* value_row = static_cast<const RowT*>(p.values) + row * p.v_stride + 8 * u;
-    const bool turns = 8 * u < p.rotary_dim;
-    const std::uint32_t half = p.rotary_dim / 2;
-    const int partner = !turns || p.interleaved ? 0 : (8 * u < half ? static_cast<int>(half) : -static_cast<int>(half));
+    const bool turns = 8 * u < p.rotary_dim, second = 8 * u >= half;
+    const int partner = second ? -static_cast<int>(half) : static_cast<int>(half);
 
-    // The row's K and V are asked for while its place is looked up.
+    // The row's K and V, and the first Q units, are asked for while its place is
+    // looked up. A Q item is a pair of units, or one unit that does not turn.
     float k[kPasses][8], k2[kPasses][8], v[kPasses][8];
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
         const std::uint32_t h = min(h0 + i * heads, p.kv_heads - 1);
         load8(key_row + static_cast<std::size_t>(h) * d, k[i]);
-        if (partner != 0) load8(key_row + static_cast<std::size_t>(h) * d + partner, k2[i]);
+        if (!kNeighbours && turns) load8(key_row + static_cast<std::size_t>(h) * d + partner, k2[i]);
         load8(value_row + static_cast<std::size_t>(h) * d, v[i]);
     }
+    const std::uint32_t pair_items = kNeighbours ? p.rotary_dim / 8 : p.rotary_dim / 16;
+    std::uint32_t qh = (threadIdx.x * p.by_items) >> 16;
+    const std::uint32_t item = threadIdx.x - qh * p.items, q_step = p.q_step;
+    const bool item_turns = item < pair_items;
+    const std::uint32_t q_dim = item_turns ? 8 * item : p.rotary_dim + 8 * (item - pair_items);
+    const RowT* q_row = static_cast<const RowT*>(p.queries) + row * p.q_stride + q_dim;
+    if (qh >= q_step) qh = p.q_heads;  // left over
+    Eight<RowT> q1, q2;
+    auto ask = [&] {
+        if (qh >= p.q_heads) return;
+        const uint4* at = reinterpret_cast<const uint4*>(q_row + static_cast<std::size_t>(qh) * d);
+        const uint4* at2 = reinterpret_cast<const uint4*>(q_row + static_cast<std::size_t>(qh) * d + half);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(8 * sizeof(RowT) / 16); ++i) {
+            q1.words[i] = at[i];
+            if (!kNeighbours && item_turns) q2.words[i] = at2[i];
+        }
+    };
+    ask();
     std::uint32_t error = 0;
     const Place place = find_place(p.row_sequences[row], p.positions[row], p.tables, p.num_seqs,
                                    p.max_blocks, p.block_tokens, p.num_blocks, p.cos_sin_positions,
@@ -257,37 +330,30 @@ __global__ void __launch_bounds__(kRowThreads) rotary_append_vector_kernel(const
         if (error != 0 && threadIdx.x == 0) flag_error(p.error_word, error);
         return;
     }
-    // Element i turns to x[i] c[i] + y[i] s[i], y the partners, the first of a
-    // pair with the sine's sign changed (exact).
-    float c[8], s[8];
-    if (turns) {
-        const float* angles = p.cos_sin + static_cast<std::size_t>(place.position) * p.rotary_dim;
-        if (p.interleaved) {
-            const float4 cs = *reinterpret_cast<const float4*>(angles + 4 * u);
-            const float4 sn = *reinterpret_cast<const float4*>(angles + half + 4 * u);
-            c[0] = c[1] = cs.x, c[2] = c[3] = cs.y, c[4] = c[5] = cs.z, c[6] = c[7] = cs.w;
-            s[1] = sn.x, s[3] = sn.y, s[5] = sn.z, s[7] = sn.w;
-            s[0] = -sn.x, s[2] = -sn.y, s[4] = -sn.z, s[6] = -sn.w;
+    const float* angles = p.cos_sin + static_cast<std::size_t>(place.position) * p.rotary_dim;
+    // Cosines and sines of the pairs from `pair` on (neighbours: four).
+    auto load_angles = [&](std::uint32_t pair, float (&c)[8], float (&s)[8]) {
+        if constexpr (kNeighbours) {
+            widen16(*reinterpret_cast<const uint4*>(angles + pair), c, 0.0f);
+            widen16(*reinterpret_cast<const uint4*>(angles + half + pair), s, 0.0f);
         } else {
-            const std::uint32_t pair = 8 * u < half ? 8 * u : 8 * u - half;
             load8(angles + pair, c);
             load8(angles + half + pair, s);
-            if (8 * u < half) {
+        }
+    };
+    if (turns) {
+        float c[8], s[8];
+        load_angles(kNeighbours ? 4 * u : second ? 8 * u - half : 8 * u, c, s);
+        if (!kNeighbours && !second) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) s[i] = -s[i];
-            }
+            for (int i = 0; i < 8; ++i) s[i] = -s[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            if constexpr (kNeighbours) turn8_neighbours(k[i], c, s);
+            else turn8(k[i], k2[i], c, s);
         }
     }
-    auto turn = [&](float (&x)[8], const float (&y)[8]) {
-        if (!turns) return;
-        float out[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            out[i] = __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(p.interleaved ? x[i ^ 1] : y[i], s[i]));
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = out[i];
-    };
 
     bool bad = false;
     if constexpr (kFourBit) {
@@ -295,14 +361,13 @@ __global__ void __launch_bounds__(kRowThreads) rotary_append_vector_kernel(const
         __half2 pairs[kPasses][2];
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
-            turn(k[i], k2[i]);
             const bool live = h0 + i * heads < p.kv_heads;
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
                 float (&x)[8] = which ? v[i] : k[i];
                 bool out_of_range;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = Storage<PoolT>::to_float(Storage<PoolT>::from_float(x[e]));
+                const Eight<PoolT> rounded = round8<PoolT>(x);
+                widen16(rounded.words[0], x, PoolT{});
                 words[i][which] = kv4::quantise(x, pairs[i][which], out_of_range);
                 bad |= live && out_of_range;
             }
@@ -312,27 +377,32 @@ __global__ void __launch_bounds__(kRowThreads) rotary_append_vector_kernel(const
             return;
         }
         const std::size_t tiles_per_head = p.block_tokens / kv4::kTileTokens;
-        const int slot = static_cast<int>(place.slot % kv4::kTileTokens), dd = static_cast<int>(d), uu = static_cast<int>(u);
-        unsigned char* tile0 = p.key_arena +
-            (static_cast<std::size_t>(place.block) * p.kv_heads * tiles_per_head + place.slot / kv4::kTileTokens) * kv4::tile_bytes(dd);
+        const int slot = static_cast<int>(place.slot % kv4::kTileTokens), uu = static_cast<int>(u);
+        auto write = [&](auto dim) {  // head_dim as a constant
+            constexpr int kD = decltype(dim)::value;
+            unsigned char* tile0 = p.key_arena +
+                (static_cast<std::size_t>(place.block) * p.kv_heads * tiles_per_head + place.slot / kv4::kTileTokens) * kv4::tile_bytes(kD);
 #pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            const std::uint32_t h = h0 + i * heads;
-            if (h >= p.kv_heads) break;
-            unsigned char* tile = tile0 + h * tiles_per_head * kv4::tile_bytes(dd);
-            *reinterpret_cast<std::uint32_t*>(tile + kv4::key_word(dd, slot, uu)) = words[i][0];
-            *reinterpret_cast<std::uint32_t*>(tile + kv4::value_word(dd, slot, uu)) = words[i][1];
-            if (u % 8 < 2) {
-                *reinterpret_cast<__half2*>(tile + kv4::pair_at(dd, slot, uu / 8, uu % 8)) = uu % 8 == 0 ? pairs[i][0] : pairs[i][1];
+            for (int i = 0; i < kPasses; ++i) {
+                const std::uint32_t h = h0 + i * heads;
+                if (h >= p.kv_heads) break;
+                unsigned char* tile = tile0 + h * tiles_per_head * kv4::tile_bytes(kD);
+                *reinterpret_cast<std::uint32_t*>(tile + kv4::key_word(kD, slot, uu)) = words[i][0];
+                *reinterpret_cast<std::uint32_t*>(tile + kv4::value_word(kD, slot, uu)) = words[i][1];
+                if (u % 8 < 2) {
+                    *reinterpret_cast<__half2*>(tile + kv4::pair_at(kD, slot, uu / 8, uu % 8)) = uu % 8 == 0 ? pairs[i][0] : pairs[i][1];
+                }
             }
-        }
+        };
+        if (d == 128) write(std::integral_constant<int, 128>{});
+        else write(std::integral_constant<int, 64>{});
     } else {
         Eight<PoolT> held[kPasses][2];
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
-            turn(k[i], k2[i]);
-            held[i][0] = round8<PoolT>(k[i], bad);
-            held[i][1] = round8<PoolT>(v[i], bad);
+            bad |= outside8<PoolT>(k[i]) || outside8<PoolT>(v[i]);
+            held[i][0] = round8<PoolT>(k[i]);
+            held[i][1] = round8<PoolT>(v[i]);
         }
         if (__syncthreads_or(bad)) {
             if (threadIdx.x == 0) flag_error(p.error_word, kErrNonFinite);
@@ -348,16 +418,26 @@ __global__ void __launch_bounds__(kRowThreads) rotary_append_vector_kernel(const
             store8(reinterpret_cast<PoolT*>(p.value_arena) + dst, held[i][1]);
         }
     }
-    if (p.queries == nullptr) return;
-    const RowT* q_row = static_cast<const RowT*>(p.queries) + row * p.q_stride + 8 * u;
-    OutT* out = static_cast<OutT*>(p.q_out) + row * p.q_heads * d + 8 * u;
-#pragma unroll 4
-    for (std::uint32_t h = h0; h < p.q_heads; h += heads) {
-        float x[8], y[8];
-        load8(q_row + static_cast<std::size_t>(h) * d, x);
-        if (partner != 0) load8(q_row + static_cast<std::size_t>(h) * d + partner, y);
-        turn(x, y);
-        store8(out + static_cast<std::size_t>(h) * d, round8<OutT>(x, bad));
+
+    if (qh >= p.q_heads) return;
+    float c[8], s[8];
+    if (item_turns) load_angles(kNeighbours ? 4 * item : 8 * item, c, s);
+    OutT* out_row = static_cast<OutT*>(p.q_out) + row * p.q_heads * d + q_dim;
+    while (true) {
+        float a[8], b[8];
+        load8(reinterpret_cast<const RowT*>(q1.words), a);
+        if (!kNeighbours && item_turns) load8(reinterpret_cast<const RowT*>(q2.words), b);
+        OutT* out = out_row + static_cast<std::size_t>(qh) * d;
+        qh += q_step;
+        ask();
+        if (kNeighbours) {
+            if (item_turns) turn8_neighbours(a, c, s);
+        } else if (item_turns) {
+            turn8_both(a, b, c, s);
+            store8(out + half, round8<OutT>(b));
+        }
+        store8(out, round8<OutT>(a));
+        if (qh >= p.q_heads) return;
     }
 }
 
@@ -391,23 +471,30 @@ __global__ void __launch_bounds__(kRowThreads) gather_rows_vector_kernel(const G
     const std::uint32_t units = p.head_dim / 8, all = p.kv_heads * units;
     for (std::uint32_t i = threadIdx.x; i < 2 * all; i += blockDim.x) {
         const bool is_value = i >= all;
-        const std::uint32_t unit = is_value ? i - all : i, head = unit / units, u = unit % units;
+        const std::uint32_t unit = is_value ? i - all : i;
+        // A 4-bit pool's heads are 8 or 16 units: a shift.
+        const std::uint32_t head = kFourBit ? unit >> (units == 16 ? 4 : 3) : unit / units, u = unit - head * units;
         T* out = static_cast<T*>(is_value ? p.values_out : p.keys_out) + (row * all + unit) * 8;
         if constexpr (kFourBit) {
-            const float most = std::is_same<T, __half>::value ? 65504.0f : 3.3895313892515355e38f;
             const std::uint32_t tiles_per_head = p.block_tokens / kv4::kTileTokens;
-            const int slot = static_cast<int>(place.slot % kv4::kTileTokens), dd = static_cast<int>(p.head_dim);
-            const unsigned char* tile = p.key_arena +
-                ((static_cast<std::size_t>(place.block) * p.kv_heads + head) * tiles_per_head +
-                 place.slot / kv4::kTileTokens) * kv4::tile_bytes(dd);
-            const std::uint32_t word = *reinterpret_cast<const std::uint32_t*>(
-                tile + (is_value ? kv4::value_word(dd, slot, u) : kv4::key_word(dd, slot, u)));
-            const float2 pair = kv4::load_pair(tile, kv4::pair_at(dd, slot, u / 8, is_value));
-            float x[8];
+            const int slot = static_cast<int>(place.slot % kv4::kTileTokens), uu = static_cast<int>(u);
+            auto widen = [&](auto dim) {  // head_dim as a constant
+                constexpr int kD = decltype(dim)::value;
+                const unsigned char* tile = p.key_arena +
+                    ((static_cast<std::size_t>(place.block) * p.kv_heads + head) * tiles_per_head +
+                     place.slot / kv4::kTileTokens) * kv4::tile_bytes(kD);
+                const std::uint32_t word = *reinterpret_cast<const std::uint32_t*>(
+                    tile + (is_value ? kv4::value_word(kD, slot, uu) : kv4::key_word(kD, slot, uu)));
+                float x[8];
+                kv4::code_values(word, kv4::load_pair(tile, kv4::pair_at(kD, slot, uu / 8, is_value)), x);
+                if (std::is_same<T, __half>::value) {  // bf16 holds all of them: at most 9 x 65504
 #pragma unroll
-            for (int n = 0; n < 8; ++n) x[n] = fminf(fmaxf(kv4::code_value(word, n, pair), -most), most);
-            bool bad = false;
-            store8(out, round8<T>(x, bad));
+                    for (int n = 0; n < 8; ++n) x[n] = fminf(fmaxf(x[n], -65504.0f), 65504.0f);
+                }
+                store8(out, round8<T>(x));
+            };
+            if (p.head_dim == 128) widen(std::integral_constant<int, 128>{});
+            else widen(std::integral_constant<int, 64>{});
         } else {
             const T* at = reinterpret_cast<const T*>(is_value ? p.value_arena : p.key_arena) +
                 ((static_cast<std::size_t>(place.block) * p.kv_heads + head) * p.block_tokens + place.slot) * p.head_dim + 8 * u;
@@ -471,9 +558,15 @@ __global__ void __launch_bounds__(kRowThreads) gather_rows_kernel(const GatherPa
 
 template <typename RowT, typename PoolT, typename OutT, bool kFourBit>
 void launch_vector(const AppendParams& a, unsigned grid, unsigned threads, std::uint32_t passes, cudaStream_t s) {
-    if (passes == 1) rotary_append_vector_kernel<RowT, PoolT, OutT, kFourBit, 1><<<grid, threads, 0, s>>>(a);
-    else if (passes == 2) rotary_append_vector_kernel<RowT, PoolT, OutT, kFourBit, 2><<<grid, threads, 0, s>>>(a);
-    else rotary_append_vector_kernel<RowT, PoolT, OutT, kFourBit, 4><<<grid, threads, 0, s>>>(a);
+    auto launch = [&](auto neighbours) {
+        constexpr bool kN = decltype(neighbours)::value;
+        auto* kernel = passes == 1 ? rotary_append_vector_kernel<RowT, PoolT, OutT, kFourBit, kN, 1>
+                     : passes == 2 ? rotary_append_vector_kernel<RowT, PoolT, OutT, kFourBit, kN, 2>
+                                   : rotary_append_vector_kernel<RowT, PoolT, OutT, kFourBit, kN, 4>;
+        kernel<<<grid, threads, 0, s>>>(a);
+    };
+    if (a.interleaved) launch(std::true_type{});
+    else launch(std::false_type{});
 }
 
 bool aligned16(const void* at) { return reinterpret_cast<std::uintptr_t>(at) % 16 == 0; }
@@ -494,13 +587,19 @@ void launch_rotary(const AppendParams& a, std::uint64_t rows, bool four_bit, cud
         while (four_bit && heads * units % 32 != 0) ++heads;  // whole warps: the groups' minima are shuffled
         const std::uint32_t passes = (a.kv_heads + heads - 1) / heads;
         if (passes <= 4) {
+            AppendParams v = a;
+            v.heads = heads;
+            v.by_units = (65536 + units - 1) / units;
+            v.items = a.rotary_dim / (a.interleaved ? 8 : 16) + (a.head_dim - a.rotary_dim) / 8;
+            v.by_items = (65536 + v.items - 1) / v.items;
+            v.q_step = heads * units / v.items;
             if constexpr (!std::is_same<PoolT, float>::value) {
                 if (four_bit) {
-                    launch_vector<RowT, PoolT, OutT, true>(a, grid, heads * units, passes, s);
+                    launch_vector<RowT, PoolT, OutT, true>(v, grid, heads * units, passes, s);
                     return;
                 }
             }
-            launch_vector<RowT, PoolT, OutT, false>(a, grid, heads * units, passes, s);
+            launch_vector<RowT, PoolT, OutT, false>(v, grid, heads * units, passes, s);
             return;
         }
     }
