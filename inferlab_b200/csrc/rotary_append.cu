@@ -42,7 +42,7 @@ struct AppendParams {
     const std::int32_t* tables;
     std::uint32_t num_seqs, max_blocks, block_tokens;
     std::uint64_t num_blocks;
-    // Vector kernel: CTA threads per head round, and the Q items of a head; by_*
+    // Vector kernel: heads of a K/V round, Q items of a head and heads of a Q round; by_*
     // divide a thread number (< 256) as (t * by) >> 16.
     std::uint32_t heads, by_units, items, by_items, q_step;
     void* q_out;
@@ -238,30 +238,29 @@ __device__ __forceinline__ bool outside8(const float (&x)[8]) {
     return out;
 }
 template <typename T>
+__device__ __forceinline__ Eight<T> ask8(const T* at) {
+    Eight<T> e;
+#pragma unroll
+    for (int c = 0; c < static_cast<int>(8 * sizeof(T) / 16); ++c) e.words[c] = reinterpret_cast<const uint4*>(at)[c];
+    return e;
+}
+template <typename T>
 __device__ __forceinline__ void store8(T* at, const Eight<T>& e) {
 #pragma unroll
     for (int c = 0; c < static_cast<int>(8 * sizeof(T) / 16); ++c) reinterpret_cast<uint4*>(at)[c] = e.words[c];
 }
 
-// out = x c + y s, y the pair's other elements and s with the first one's sine
-// negated (exact): each product and the sum rounded once, two lanes a time.
-__device__ __forceinline__ void turn8(float (&x)[8], const float (&y)[8], const float (&c)[8], const float (&s)[8]) {
+// One half of split pairs, y the other: x c - y s, or (second) x c + y s, each
+// product and sum rounded once, products two lanes a time.
+__device__ __forceinline__ void turn8(float (&x)[8], const float (&y)[8], const float (&c)[8], const float (&s)[8],
+                                      bool second) {
+    const std::uint32_t sign = second ? 0u : 0x80000000u;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         const float2 own = kv4::mul2(make_float2(x[i], x[i + 1]), make_float2(c[i], c[i + 1]));
         const float2 other = kv4::mul2(make_float2(y[i], y[i + 1]), make_float2(s[i], s[i + 1]));
-        x[i] = __fadd_rn(own.x, other.x), x[i + 1] = __fadd_rn(own.y, other.y);
-    }
-}
-// Both halves of split pairs: a' = a c - b s, b' = b c + a s.
-__device__ __forceinline__ void turn8_both(float (&a)[8], float (&b)[8], const float (&c)[8], const float (&s)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const float2 x = make_float2(a[i], a[i + 1]), y = make_float2(b[i], b[i + 1]);
-        const float2 cc = make_float2(c[i], c[i + 1]), ss = make_float2(s[i], s[i + 1]);
-        const float2 xc = kv4::mul2(x, cc), ys = kv4::mul2(y, ss), yc = kv4::mul2(y, cc), xs = kv4::mul2(x, ss);
-        a[i] = __fsub_rn(xc.x, ys.x), a[i + 1] = __fsub_rn(xc.y, ys.y);
-        b[i] = __fadd_rn(yc.x, xs.x), b[i + 1] = __fadd_rn(yc.y, xs.y);
+        x[i] = __fadd_rn(own.x, __uint_as_float(__float_as_uint(other.x) ^ sign));
+        x[i + 1] = __fadd_rn(own.y, __uint_as_float(__float_as_uint(other.y) ^ sign));
     }
 }
 // Interleaved: c and s hold four angles, the pairs are neighbours.
@@ -274,84 +273,180 @@ __device__ __forceinline__ void turn8_neighbours(float (&x)[8], const float (&c)
     }
 }
 
-// The common shapes: units of 8 dims, 16-byte accesses. One CTA per row.
-// K and V: a thread keeps to one unit of the head and goes through the heads,
-// blockDim / (head_dim / 8) at a time, in at most kPasses rounds, held until the
-// whole row is known to be good; in a 4-bit pool eight neighbours then hold a
-// group. The partner dims of a split rotation are loaded a second time (from
-// L1). Q: a thread takes both units of a pair, so nothing is loaded or widened
-// twice; the first round is asked for at the start.
-// Bound by HBM: 8192 rows of 32 + 8 + 8 bf16 heads x 128 move 12 KB in and 8 KB
-// (+ 2.3 KB a row in 4 bits) out each.
+// Four consecutive elements.
+template <typename T>
+struct Four {
+    std::uint32_t words[sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ Four<T> ask4(const T* at) {
+    Four<T> e;
+    if constexpr (sizeof(T) == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(at);
+        e.words[0] = x.x, e.words[1] = x.y, e.words[2] = x.z, e.words[3] = x.w;
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(at);
+        e.words[0] = x.x, e.words[1] = x.y;
+    }
+    return e;
+}
+template <typename T>
+__device__ __forceinline__ void widen4(const Four<T>& e, float (&x)[4]) {
+    const T* t = reinterpret_cast<const T*>(e.words);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = Storage<T>::to_float(t[i]);
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* at, const float (&x)[4]) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
+    else *reinterpret_cast<uint2*>(at) = make_uint2(round_pair(x[0], x[1], T{}), round_pair(x[2], x[3], T{}));
+}
+
+// The common shapes: units of 8 dims, 16-byte accesses, two CTAs per row.
+//   K and V (blockIdx.y 0): a thread keeps to one unit of the head and goes
+//     through the heads, p.heads at a time, in at most kPasses rounds, held
+//     until the whole row is known to be good; in a 4-bit pool eight neighbours
+//     then hold a group. The partner dims of a split rotation are loaded a
+//     second time (from L1).
+//   Q (blockIdx.y 1): a thread takes four dims and their partners, so nothing is
+//     loaded or widened twice, and asks for several heads' at once.
+// Everything of a row is asked for in one round of loads behind its sequence and
+// position. Bound by HBM: 8192 rows of 32 + 8 + 8 bf16 heads x 128 move 12 KB in
+// and 8 KB (+ 2.3 KB a row in 4 bits) out each; what it needs for that is rows
+// in flight: as one CTA of 256 threads and 64 registers 51 us, split in two and
+// Q by eight dims (70 registers) 48.
 template <typename RowT, typename PoolT, typename OutT, bool kFourBit, bool kNeighbours, int kPasses>
 __global__ void __launch_bounds__(kRowThreads) rotary_append_vector_kernel(const AppendParams p) {
     const std::size_t row = blockIdx.x;
-    const std::uint32_t d = p.head_dim, units = d / 8, half = p.rotary_dim / 2;
-    const std::uint32_t h0 = (threadIdx.x * p.by_units) >> 16, u = threadIdx.x - h0 * units, heads = p.heads;
+    const std::uint32_t d = p.head_dim, half = p.rotary_dim / 2;
+    const std::int32_t seq = p.row_sequences[row], position = p.positions[row];
+    std::uint32_t error = 0;
+    auto find = [&] {
+        return find_place(seq, position, p.tables, p.num_seqs, p.max_blocks, p.block_tokens, p.num_blocks,
+                          p.cos_sin_positions, p.padded_rows, error);
+    };
+    // A position behind the table is found out with the place; it is not read.
+    const bool known = position >= 0 && static_cast<std::uint64_t>(position) < p.cos_sin_positions;
+    const float* angles = p.cos_sin + static_cast<std::size_t>(position) * p.rotary_dim;
+
+    if (blockIdx.y != 0) {
+        // A Q item is four dims and their partners, or four that do not turn
+        // (neighbours: four dims, their own partners).
+        const std::uint32_t turning = kNeighbours ? p.rotary_dim / 4 : p.rotary_dim / 8;
+        std::uint32_t h = (threadIdx.x * p.by_items) >> 16;
+        const std::uint32_t item = threadIdx.x - h * p.items, step = p.q_step;
+        if (h >= step || h >= p.q_heads) return;  // left over
+        const bool turns = item < turning;
+        const std::uint32_t dim = turns ? 4 * item : p.rotary_dim + 4 * (item - turning);
+        const RowT* q_row = static_cast<const RowT*>(p.queries) + row * p.q_stride + dim;
+        // Heads asked for at once: 16 bits want the registers (48 us, 2 heads 51),
+        // fp32 the loads (55 us, 2 heads 58).
+        constexpr int kRounds = sizeof(RowT) == 4 ? 4 : 1;
+        Four<RowT> q1[kRounds], q2[kRounds];
+        auto ask = [&] {
+#pragma unroll
+            for (int i = 0; i < kRounds; ++i) {
+                if (h + i * step >= p.q_heads) break;
+                const RowT* at = q_row + static_cast<std::size_t>(h + i * step) * d;
+                q1[i] = ask4(at);
+                if (!kNeighbours && turns) q2[i] = ask4(at + half);
+            }
+        };
+        ask();
+        float c[4], s[4];
+        if (turns && known) {
+            if constexpr (kNeighbours) {
+                const float2 x = *reinterpret_cast<const float2*>(angles + 2 * item);
+                const float2 y = *reinterpret_cast<const float2*>(angles + half + 2 * item);
+                c[0] = x.x, c[1] = x.y, s[0] = y.x, s[1] = y.y;
+            } else {
+                widen16(*reinterpret_cast<const uint4*>(angles + 4 * item), c, 0.0f);
+                widen16(*reinterpret_cast<const uint4*>(angles + half + 4 * item), s, 0.0f);
+            }
+        }
+        if (find().block < 0) return;  // a bad row is reported by the other CTA
+        OutT* out_row = static_cast<OutT*>(p.q_out) + row * p.q_heads * d + dim;
+        for (;;) {
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                if (h + r * step >= p.q_heads) return;
+                float a[4], b[4];
+                widen4(q1[r], a);
+                if (!kNeighbours && turns) widen4(q2[r], b);
+                OutT* out = out_row + static_cast<std::size_t>(h + r * step) * d;
+                if (turns) {
+                    if constexpr (kNeighbours) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float x = a[2 * i], y = a[2 * i + 1];
+                            a[2 * i] = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i]));
+                            a[2 * i + 1] = __fadd_rn(__fmul_rn(y, c[i]), __fmul_rn(x, s[i]));
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2) {
+                            const float2 x = make_float2(a[i], a[i + 1]), y = make_float2(b[i], b[i + 1]);
+                            const float2 cc = make_float2(c[i], c[i + 1]), ss = make_float2(s[i], s[i + 1]);
+                            const float2 xc = kv4::mul2(x, cc), ys = kv4::mul2(y, ss), yc = kv4::mul2(y, cc), xs = kv4::mul2(x, ss);
+                            a[i] = __fsub_rn(xc.x, ys.x), a[i + 1] = __fsub_rn(xc.y, ys.y);
+                            b[i] = __fadd_rn(yc.x, xs.x), b[i + 1] = __fadd_rn(yc.y, xs.y);
+                        }
+                        store4(out + half, b);
+                    }
+                }
+                store4(out, a);
+            }
+            h += kRounds * step;
+            ask();
+        }
+    }
+
+    const std::uint32_t units = d / 8, heads = p.heads;
+    const std::uint32_t h0 = (threadIdx.x * p.by_units) >> 16, u = threadIdx.x - h0 * units;
     const RowT* key_row = static_cast<const RowT*>(p.keys) + row * p.k_stride + 8 * u;
     const RowT* value_row = static_cast<const RowT*>(p.values) + row * p.v_stride + 8 * u;
-    const bool turns = 8 * u < p.rotary_dim, second = 8 * u >= half;
+    const bool turns = 8 * u < p.rotary_dim, second = !kNeighbours && 8 * u >= half;
     const int partner = second ? -static_cast<int>(half) : static_cast<int>(half);
-
-    // The row's K and V, and the first Q units, are asked for while its place is
-    // looked up. A Q item is a pair of units, or one unit that does not turn.
-    float k[kPasses][8], k2[kPasses][8], v[kPasses][8];
+    // Rounds in which this warp has a head (a quantising warp works whole).
+    const std::uint32_t warp_h0 = ((threadIdx.x & ~31u) * p.by_units) >> 16;
+    auto has = [&](int i) { return warp_h0 + i * heads < p.kv_heads; };
+    Eight<RowT> k_in[kPasses], k2_in[kPasses], v_in[kPasses];
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
+        if (!has(i)) break;
         const std::uint32_t h = min(h0 + i * heads, p.kv_heads - 1);
-        load8(key_row + static_cast<std::size_t>(h) * d, k[i]);
-        if (!kNeighbours && turns) load8(key_row + static_cast<std::size_t>(h) * d + partner, k2[i]);
-        load8(value_row + static_cast<std::size_t>(h) * d, v[i]);
+        k_in[i] = ask8(key_row + static_cast<std::size_t>(h) * d);
+        if (!kNeighbours && turns) k2_in[i] = ask8(key_row + static_cast<std::size_t>(h) * d + partner);
+        v_in[i] = ask8(value_row + static_cast<std::size_t>(h) * d);
     }
-    const std::uint32_t pair_items = kNeighbours ? p.rotary_dim / 8 : p.rotary_dim / 16;
-    std::uint32_t qh = (threadIdx.x * p.by_items) >> 16;
-    const std::uint32_t item = threadIdx.x - qh * p.items, q_step = p.q_step;
-    const bool item_turns = item < pair_items;
-    const std::uint32_t q_dim = item_turns ? 8 * item : p.rotary_dim + 8 * (item - pair_items);
-    const RowT* q_row = static_cast<const RowT*>(p.queries) + row * p.q_stride + q_dim;
-    if (qh >= q_step) qh = p.q_heads;  // left over
-    Eight<RowT> q1, q2;
-    auto ask = [&] {
-        if (qh >= p.q_heads) return;
-        const uint4* at = reinterpret_cast<const uint4*>(q_row + static_cast<std::size_t>(qh) * d);
-        const uint4* at2 = reinterpret_cast<const uint4*>(q_row + static_cast<std::size_t>(qh) * d + half);
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(8 * sizeof(RowT) / 16); ++i) {
-            q1.words[i] = at[i];
-            if (!kNeighbours && item_turns) q2.words[i] = at2[i];
+    float c[8], s[8];
+    if (turns && known) {
+        if constexpr (kNeighbours) {
+            widen16(*reinterpret_cast<const uint4*>(angles + 4 * u), c, 0.0f);
+            widen16(*reinterpret_cast<const uint4*>(angles + half + 4 * u), s, 0.0f);
+        } else {
+            load8(angles + (second ? 8 * u - half : 8 * u), c);
+            load8(angles + (second ? 8 * u : 8 * u + half), s);
         }
-    };
-    ask();
-    std::uint32_t error = 0;
-    const Place place = find_place(p.row_sequences[row], p.positions[row], p.tables, p.num_seqs,
-                                   p.max_blocks, p.block_tokens, p.num_blocks, p.cos_sin_positions,
-                                   p.padded_rows, error);
+    }
+    const Place place = find();
     if (error != 0 || place.block < 0) {
         if (error != 0 && threadIdx.x == 0) flag_error(p.error_word, error);
         return;
     }
-    const float* angles = p.cos_sin + static_cast<std::size_t>(place.position) * p.rotary_dim;
-    // Cosines and sines of the pairs from `pair` on (neighbours: four).
-    auto load_angles = [&](std::uint32_t pair, float (&c)[8], float (&s)[8]) {
+    float k[kPasses][8], v[kPasses][8];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+        if (!has(i)) break;
+        load8(reinterpret_cast<const RowT*>(k_in[i].words), k[i]);
+        load8(reinterpret_cast<const RowT*>(v_in[i].words), v[i]);
+        if (!turns) continue;
         if constexpr (kNeighbours) {
-            widen16(*reinterpret_cast<const uint4*>(angles + pair), c, 0.0f);
-            widen16(*reinterpret_cast<const uint4*>(angles + half + pair), s, 0.0f);
+            turn8_neighbours(k[i], c, s);
         } else {
-            load8(angles + pair, c);
-            load8(angles + half + pair, s);
-        }
-    };
-    if (turns) {
-        float c[8], s[8];
-        load_angles(kNeighbours ? 4 * u : second ? 8 * u - half : 8 * u, c, s);
-        if (!kNeighbours && !second) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] = -s[i];
-        }
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            if constexpr (kNeighbours) turn8_neighbours(k[i], c, s);
-            else turn8(k[i], k2[i], c, s);
+            float other[8];
+            load8(reinterpret_cast<const RowT*>(k2_in[i].words), other);
+            turn8(k[i], other, c, s, second);
         }
     }
 
@@ -361,6 +456,7 @@ __global__ void __launch_bounds__(kRowThreads) rotary_append_vector_kernel(const
         __half2 pairs[kPasses][2];
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
+            if (!has(i)) break;
             const bool live = h0 + i * heads < p.kv_heads;
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
@@ -400,6 +496,7 @@ __global__ void __launch_bounds__(kRowThreads) rotary_append_vector_kernel(const
         Eight<PoolT> held[kPasses][2];
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
+            if (!has(i)) break;
             bad |= outside8<PoolT>(k[i]) || outside8<PoolT>(v[i]);
             held[i][0] = round8<PoolT>(k[i]);
             held[i][1] = round8<PoolT>(v[i]);
@@ -418,27 +515,6 @@ __global__ void __launch_bounds__(kRowThreads) rotary_append_vector_kernel(const
             store8(reinterpret_cast<PoolT*>(p.value_arena) + dst, held[i][1]);
         }
     }
-
-    if (qh >= p.q_heads) return;
-    float c[8], s[8];
-    if (item_turns) load_angles(kNeighbours ? 4 * item : 8 * item, c, s);
-    OutT* out_row = static_cast<OutT*>(p.q_out) + row * p.q_heads * d + q_dim;
-    while (true) {
-        float a[8], b[8];
-        load8(reinterpret_cast<const RowT*>(q1.words), a);
-        if (!kNeighbours && item_turns) load8(reinterpret_cast<const RowT*>(q2.words), b);
-        OutT* out = out_row + static_cast<std::size_t>(qh) * d;
-        qh += q_step;
-        ask();
-        if (kNeighbours) {
-            if (item_turns) turn8_neighbours(a, c, s);
-        } else if (item_turns) {
-            turn8_both(a, b, c, s);
-            store8(out + half, round8<OutT>(b));
-        }
-        store8(out, round8<OutT>(a));
-        if (qh >= p.q_heads) return;
-    }
 }
 
 struct GatherParams {
@@ -455,9 +531,12 @@ struct GatherParams {
 };
 
 // The common shapes of a gather: units of 8 dims, 16-byte accesses; a 4-bit
-// pool's unit is one word of codes and its group's pair.
+// pool's unit is one word of codes and its group's pair. Bound by HBM as the
+// append is (8192 rows of 8 + 8 heads x 128: 12 us in 128 threads a row, 15 in
+// 256).
+constexpr int kGatherThreads = 128;
 template <typename T, bool kFourBit>
-__global__ void __launch_bounds__(kRowThreads) gather_rows_vector_kernel(const GatherParams p) {
+__global__ void __launch_bounds__(kGatherThreads) gather_rows_vector_kernel(const GatherParams p) {
     const std::size_t row = blockIdx.x;
     std::uint32_t error = 0;
     const Place place = find_place(p.row_sequences != nullptr ? p.row_sequences[row] : 0,
@@ -563,7 +642,7 @@ void launch_vector(const AppendParams& a, unsigned grid, unsigned threads, std::
         auto* kernel = passes == 1 ? rotary_append_vector_kernel<RowT, PoolT, OutT, kFourBit, kN, 1>
                      : passes == 2 ? rotary_append_vector_kernel<RowT, PoolT, OutT, kFourBit, kN, 2>
                                    : rotary_append_vector_kernel<RowT, PoolT, OutT, kFourBit, kN, 4>;
-        kernel<<<grid, threads, 0, s>>>(a);
+        kernel<<<dim3(grid, a.queries != nullptr ? 2 : 1), threads, 0, s>>>(a);
     };
     if (a.interleaved) launch(std::true_type{});
     else launch(std::false_type{});
@@ -583,16 +662,20 @@ void launch_rotary(const AppendParams& a, std::uint64_t rows, bool four_bit, cud
         aligned16(a.keys) && aligned16(a.values) && a.k_stride % step == 0 && a.v_stride % step == 0 &&
         (a.queries == nullptr || (aligned16(a.queries) && aligned16(a.q_out) && a.q_stride % step == 0)) &&
         (a.rotary_dim == 0 || aligned16(a.cos_sin))) {
-        std::uint32_t heads = std::min<std::uint32_t>(kRowThreads / units, std::max(a.q_heads, a.kv_heads));
+        // 128 threads, or 256 where they would need more than two K/V rounds or a
+        // Q item each (8192 rows of 16 fp32 heads: 57 us, 256 threads 63).
+        const std::uint32_t items = a.rotary_dim / (a.interleaved ? 4 : 8) + (a.head_dim - a.rotary_dim) / 4;
+        const std::uint32_t wish = std::max(1u, 128 / units);
+        std::uint32_t heads = a.kv_heads <= 2 * wish && items <= wish * units ? wish : kRowThreads / units;
         while (four_bit && heads * units % 32 != 0) ++heads;  // whole warps: the groups' minima are shuffled
         const std::uint32_t passes = (a.kv_heads + heads - 1) / heads;
-        if (passes <= 4) {
+        if (passes <= 4 && items <= heads * units) {
             AppendParams v = a;
             v.heads = heads;
             v.by_units = (65536 + units - 1) / units;
-            v.items = a.rotary_dim / (a.interleaved ? 8 : 16) + (a.head_dim - a.rotary_dim) / 8;
-            v.by_items = (65536 + v.items - 1) / v.items;
-            v.q_step = heads * units / v.items;
+            v.items = items;
+            v.by_items = (65536 + items - 1) / items;
+            v.q_step = heads * units / items;
             if constexpr (!std::is_same<PoolT, float>::value) {
                 if (four_bit) {
                     launch_vector<RowT, PoolT, OutT, true>(v, grid, heads * units, passes, s);
@@ -653,12 +736,12 @@ void run_gather_rows(InferlabCudaKvPool& p, const std::int32_t* row_sequences,
         if constexpr (!std::is_same<T, float>::value) {
             if (p.kv_bits != 0) {
                 auto* kernel = whole ? gather_rows_vector_kernel<T, true> : gather_rows_kernel<T, true>;
-                kernel<<<grid, kRowThreads, 0, s>>>(g);
+                kernel<<<grid, whole ? kGatherThreads : kRowThreads, 0, s>>>(g);
                 return;
             }
         }
         auto* kernel = whole ? gather_rows_vector_kernel<T, false> : gather_rows_kernel<T, false>;
-        kernel<<<grid, kRowThreads, 0, s>>>(g);
+        kernel<<<grid, whole ? kGatherThreads : kRowThreads, 0, s>>>(g);
     };
     if (p.dtype == kFp32) launch(float{});
     else if (p.dtype == kF16) launch(__half{});
