@@ -70,6 +70,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return make_float2(low_f32(d), high_f32(d));
 }
 __device__ __forceinline__ float2 sub2(float2 a, float2 b) { return add2(a, make_float2(-b.x, -b.y)); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    std::uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pack_f32x2(a.x, a.y)), "l"(pack_f32x2(b.x, b.y)), "l"(pack_f32x2(c.x, c.y)));
+    return make_float2(low_f32(d), high_f32(d));
+}
 // Maximum of three that keeps a NaN.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float d;

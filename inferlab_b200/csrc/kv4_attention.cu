@@ -66,6 +66,7 @@ struct Kv4Params {
     const std::int32_t* starts;
     const std::int32_t* counts;
     const std::int32_t* offsets;
+    std::uint32_t num_seqs;
     std::uint32_t max_count;           // query tokens a sequence may have
     long long total_queries;
     std::uint32_t column_tiles, max_splits;
@@ -125,6 +126,70 @@ __device__ __forceinline__ void load_pairs(const unsigned char* at, float2 (&pai
 // t, r = 2t + 1 token 7 - t. Rows 2t of all t (what four lanes read of V at
 // once) and rows r of neighbouring r (K) then fall on different banks.
 __device__ __forceinline__ int slot_of_row(int r) { return r & 1 ? 7 - (r >> 1) : r >> 1; }
+
+// Whether this CTA is the last of `splits` to come here; what the others wrote
+// before is then visible. Returns the counter to zero.
+__device__ __forceinline__ bool last_of(std::uint32_t* counter, int splits, std::uint32_t& ticket) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        ticket = atomicAdd(counter, 1u);
+        if (ticket == static_cast<std::uint32_t>(splits) - 1) *counter = 0;
+        __threadfence();
+    }
+    __syncthreads();
+    return ticket == static_cast<std::uint32_t>(splits) - 1;
+}
+
+// Four dims (the i-th of a part) of a row merged over the splits in their order,
+// one round of loads for each kRound of them. A part is kPart floats: o, then
+// from kMl on (m, l) per row.
+template <int kPart, int kMl>
+__device__ __forceinline__ float4 merge_parts(const float* parts, int splits, int row, int i, bool& ok) {
+    constexpr int kRound = 8;
+    float top = kNoScore, sum = 0.0f;
+    float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k0 = 0; k0 < splits; k0 += kRound) {
+        float2 ml[kRound];
+        float4 x[kRound];
+#pragma unroll
+        for (int k = 0; k < kRound; ++k) {
+            const float* at = parts + static_cast<std::size_t>(min(k0 + k, splits - 1)) * kPart;
+            ml[k] = __ldcg(reinterpret_cast<const float2*>(at + kMl + 2 * row));
+            x[k] = __ldcg(reinterpret_cast<const float4*>(at) + i);
+        }
+        float next = top;
+#pragma unroll
+        for (int k = 0; k < kRound; ++k) next = fmaxf(next, ml[k].x);
+        const float kept = ex2_ftz(top - next);
+        sum *= kept;
+        total.x *= kept, total.y *= kept, total.z *= kept, total.w *= kept;
+        top = next;
+#pragma unroll
+        for (int k = 0; k < kRound; ++k) {
+            const float w = k0 + k < splits ? ex2_ftz(ml[k].x - top) : 0.0f;
+            sum = fmaf(w, ml[k].y, sum);
+            total.x = fmaf(w, x[k].x, total.x);
+            total.y = fmaf(w, x[k].y, total.y);
+            total.z = fmaf(w, x[k].z, total.z);
+            total.w = fmaf(w, x[k].w, total.w);
+        }
+    }
+    ok = isfinite(sum) && sum > 0.0f;
+    const float inv = ok ? 1.0f / sum : 0.0f;
+    return make_float4(total.x * inv, total.y * inv, total.z * inv, total.w * inv);
+}
+
+template <typename QT>
+__device__ __forceinline__ void store_row4(QT* out, float4 x) {
+    if constexpr (sizeof(QT) == 4) {
+        *reinterpret_cast<float4*>(out) = x;
+    } else {
+        QT v[4] = {Storage<QT>::from_float(x.x), Storage<QT>::from_float(x.y), Storage<QT>::from_float(x.z),
+                   Storage<QT>::from_float(x.w)};
+        *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(v);
+    }
+}
 
 // Up to 8 live query columns, or (kFour) up to 4 that stand twice, so that
 // columns 4-7 carry something else of the same queries:
@@ -610,71 +675,64 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
     }
     if (splits == 1) return;
 
-    // ---- the unit's last CTA merges the splits in their order, every thread
-    // four dims: one round of loads for each kRound splits.
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        ticket = atomicAdd(&p.ws_count[unit], 1u);
-        if (ticket == static_cast<std::uint32_t>(splits) - 1) p.ws_count[unit] = 0;
-        __threadfence();
-    }
-    __syncthreads();
-    if (ticket != static_cast<std::uint32_t>(splits) - 1) return;
-    constexpr int kRound = 8;
+    // ---- the unit's last CTA merges the splits, every thread four dims.
+    if (!last_of(p.ws_count + unit, splits, ticket)) return;
     const float* parts = p.ws_part + static_cast<std::size_t>(unit) * p.max_splits * kPart;
     for (int i = threadIdx.x; i < live * D / 4; i += blockDim.x) {
         const int col = i / (D / 4);
-        float top = kNoScore, sum = 0.0f;
-        float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int k0 = 0; k0 < splits; k0 += kRound) {
-            float2 ml[kRound];
-            float4 x[kRound];
-#pragma unroll
-            for (int k = 0; k < kRound; ++k) {
-                const float* at = parts + static_cast<std::size_t>(min(k0 + k, splits - 1)) * kPart;
-                ml[k] = __ldcg(reinterpret_cast<const float2*>(at + kCols * D + 2 * col));
-                x[k] = __ldcg(reinterpret_cast<const float4*>(at) + i);
-            }
-            float next = top;
-#pragma unroll
-            for (int k = 0; k < kRound; ++k) next = fmaxf(next, ml[k].x);
-            const float kept = ex2_ftz(top - next);
-            sum *= kept;
-            total.x *= kept, total.y *= kept, total.z *= kept, total.w *= kept;
-            top = next;
-#pragma unroll
-            for (int k = 0; k < kRound; ++k) {
-                const float w = k0 + k < splits ? ex2_ftz(ml[k].x - top) : 0.0f;
-                sum = fmaf(w, ml[k].y, sum);
-                total.x = fmaf(w, x[k].x, total.x);
-                total.y = fmaf(w, x[k].y, total.y);
-                total.z = fmaf(w, x[k].z, total.z);
-                total.w = fmaf(w, x[k].w, total.w);
-            }
-        }
-        const bool ok = isfinite(sum) && sum > 0.0f;
+        bool ok;
+        const float4 x = merge_parts<kPart, kCols * D>(parts, splits, col, i, ok);
         if (!ok) flag_error(p.error_word, kErrNormalizer);
-        const float inv = ok ? 1.0f / sum : 0.0f;
-        QT* out = static_cast<QT*>(p.out) + row_of(col) * D + 4 * i % D;
-        out[0] = Storage<QT>::from_float(total.x * inv);
-        out[1] = Storage<QT>::from_float(total.y * inv);
-        out[2] = Storage<QT>::from_float(total.z * inv);
-        out[3] = Storage<QT>::from_float(total.w * inv);
+        store_row4(static_cast<QT*>(p.out) + row_of(col) * D + 4 * i % D, x);
     }
 }
 
-// Columns a CTA works on, and how the keys are cut.
+}  // namespace
+}  // namespace ilb
+
+#include "kv4_rows.cuh"
+
+namespace ilb {
+namespace {
+
+// Columns a CTA works on, and how the keys are cut; or whole row tiles
+// (kv4_rows.cuh).
 struct Kv4Plan {
     std::uint32_t columns, column_tiles, max_splits;
     int tiles_per_split;
     std::size_t counter_bytes, part_bytes;
+    bool rows;
 };
 
 Kv4Plan plan_kv4(const InferlabCudaKvPool& p, std::uint32_t num_seqs, std::uint32_t q_heads,
                  std::uint32_t max_count, std::uint32_t max_context_len) {
     Kv4Plan plan{};
     const std::uint64_t rows = static_cast<std::uint64_t>(q_heads / p.kv_heads) * max_count;
+    if (rows > 0x7FFFFFFFull) throw std::runtime_error("4-bit attention batch is too large");
+    // Many rows per kv-head share the widened codes, if there are CTAs enough
+    // without cutting the keys.
+    const std::uint64_t row_tiles = (rows + kRowTile - 1) / kRowTile;
+    const std::uint64_t row_units = checked_mul(checked_mul(num_seqs, p.kv_heads, "4-bit attention batch is too large"),
+                                                row_tiles, "4-bit attention batch is too large");
+    if (max_count > 1 && rows > 24 && row_units >= 148) {
+        plan.rows = true;
+        plan.columns = kRowTile;
+        plan.column_tiles = static_cast<std::uint32_t>(row_tiles);
+        // Up to 4096 CTAs (nine waves of three an SM) if all contexts were
+        // max_context_len long: the lengths are the device's and most are shorter.
+        const std::uint64_t all = (max_context_len + kv4::kTileTokens - 1) / kv4::kTileTokens;
+        std::uint64_t per = p.decode_blocks_per_split;
+        if (per == 0) per = std::max<std::uint64_t>(64, checked_mul(row_units, all, "4-bit attention batch is too large") / 4096);
+        per = (std::max<std::uint64_t>(per, (all + kMaxSplits - 1) / kMaxSplits) + kBlockTiles - 1) / kBlockTiles * kBlockTiles;
+        plan.tiles_per_split = static_cast<int>(per);
+        plan.max_splits = static_cast<std::uint32_t>((all + per - 1) / per);
+        if (row_units > 0x7FFFFFFFull / plan.max_splits) throw std::runtime_error("4-bit attention batch is too large");
+        if (plan.max_splits > 1) {
+            plan.counter_bytes = (row_units * 4 + 255) & ~std::size_t(255);
+            plan.part_bytes = checked_mul(row_units * plan.max_splits, kRowTile * (p.head_dim + 4) * 4, "4-bit attention batch is too large");
+        }
+        return plan;
+    }
     plan.columns = rows <= 4 ? 4 : 8;
     const std::uint64_t column_tiles = (rows + plan.columns - 1) / plan.columns;
     const std::uint64_t units = checked_mul(checked_mul(num_seqs, p.kv_heads, "4-bit attention batch is too large"), column_tiles,
@@ -754,16 +812,20 @@ void run_kv4(InferlabCudaKvPool& p, Kv4Params k, std::uint32_t query_dtype, std:
     k.ws_count = static_cast<std::uint32_t*>(workspace);
     k.ws_part = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + plan.counter_bytes);
     k.error_word = p.error_word;
+    k.num_seqs = num_seqs;
     const unsigned grid = static_cast<unsigned>(num_seqs * p.kv_heads * plan.column_tiles * plan.max_splits);
     auto launch = [&](auto row_type, auto query_type) {
         using RowT = decltype(row_type);
         using QT = decltype(query_type);
-        auto* kernel = p.head_dim == 128
-            ? (plan.columns == 4 ? kv4_attention_kernel<RowT, QT, 128, true> : kv4_attention_kernel<RowT, QT, 128, false>)
-            : (plan.columns == 4 ? kv4_attention_kernel<RowT, QT, 64, true> : kv4_attention_kernel<RowT, QT, 64, false>);
-        const int smem = kWarps * kRing * kStep * kv4::tile_bytes(static_cast<int>(p.head_dim));
-        static std::atomic<std::uint64_t> allowed[2][2];  // devices whose kernel may use it
-        auto& devices = allowed[p.head_dim == 128][plan.columns == 4];
+        const bool wide = p.head_dim == 128;
+        auto* kernel = plan.rows
+            ? (wide ? kv4_rows_kernel<RowT, QT, 128> : kv4_rows_kernel<RowT, QT, 64>)
+            : wide ? (plan.columns == 4 ? kv4_attention_kernel<RowT, QT, 128, true> : kv4_attention_kernel<RowT, QT, 128, false>)
+                   : (plan.columns == 4 ? kv4_attention_kernel<RowT, QT, 64, true> : kv4_attention_kernel<RowT, QT, 64, false>);
+        const int smem = plan.rows ? (wide ? RowSmem<128>::kBytes : RowSmem<64>::kBytes)
+                                   : kWarps * kRing * kStep * kv4::tile_bytes(static_cast<int>(p.head_dim));
+        static std::atomic<std::uint64_t> allowed[2][3];  // devices whose kernel may use it
+        auto& devices = allowed[wide][plan.rows ? 2 : plan.columns == 4];
         const std::uint64_t bit = p.device < 64 ? 1ull << p.device : 0;
         if ((devices.load() & bit) == 0) {
             cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute");
