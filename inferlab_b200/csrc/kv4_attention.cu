@@ -691,6 +691,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
 }  // namespace ilb
 
 #include "kv4_rows.cuh"
+#include "kv4_prefill_tc.cuh"
 
 namespace ilb {
 namespace {
@@ -701,22 +702,22 @@ struct Kv4Plan {
     std::uint32_t columns, column_tiles, max_splits;
     int tiles_per_split;
     std::size_t counter_bytes, part_bytes;
-    bool rows;
+    enum { kColumns, kRows, kTensor } kind;
 };
 
 Kv4Plan plan_kv4(const InferlabCudaKvPool& p, std::uint32_t num_seqs, std::uint32_t q_heads,
-                 std::uint32_t max_count, std::uint32_t max_context_len) {
+                 std::uint32_t max_count, std::uint32_t max_context_len, std::uint32_t query_dtype) {
     Kv4Plan plan{};
     const std::uint64_t rows = static_cast<std::uint64_t>(q_heads / p.kv_heads) * max_count;
     if (rows > 0x7FFFFFFFull) throw std::runtime_error("4-bit attention batch is too large");
-    // Many rows per kv-head share the widened codes, if there are CTAs enough
-    // without cutting the keys.
-    const std::uint64_t row_tiles = (rows + kRowTile - 1) / kRowTile;
-    const std::uint64_t row_units = checked_mul(checked_mul(num_seqs, p.kv_heads, "4-bit attention batch is too large"),
-                                                row_tiles, "4-bit attention batch is too large");
-    if (max_count > 1 && rows > 24 && row_units >= 148) {
-        plan.rows = true;
-        plan.columns = kRowTile;
+    // Many rows per kv-head share the widened codes. fp32 results need two-part
+    // weights and take the rows kernel.
+    if (max_count > 1 && rows > 24) {
+        plan.kind = query_dtype == kFp32 ? Kv4Plan::kRows : Kv4Plan::kTensor;
+        plan.columns = plan.kind == Kv4Plan::kRows ? kRowTile : kTcRows;
+        const std::uint64_t row_tiles = (rows + plan.columns - 1) / plan.columns;
+        const std::uint64_t row_units = checked_mul(checked_mul(num_seqs, p.kv_heads, "4-bit attention batch is too large"),
+                                                    row_tiles, "4-bit attention batch is too large");
         plan.column_tiles = static_cast<std::uint32_t>(row_tiles);
         // Up to 4096 CTAs (nine waves of three an SM) if all contexts were
         // max_context_len long: the lengths are the device's and most are shorter.
@@ -729,7 +730,7 @@ Kv4Plan plan_kv4(const InferlabCudaKvPool& p, std::uint32_t num_seqs, std::uint3
         if (row_units > 0x7FFFFFFFull / plan.max_splits) throw std::runtime_error("4-bit attention batch is too large");
         if (plan.max_splits > 1) {
             plan.counter_bytes = (row_units * 4 + 255) & ~std::size_t(255);
-            plan.part_bytes = checked_mul(row_units * plan.max_splits, kRowTile * (p.head_dim + 4) * 4, "4-bit attention batch is too large");
+            plan.part_bytes = checked_mul(row_units * plan.max_splits, plan.columns * (p.head_dim + 4) * 4, "4-bit attention batch is too large");
         }
         return plan;
     }
@@ -792,7 +793,7 @@ void check_kv4(const InferlabCudaKvPool& p, const void* queries, std::uint32_t q
 void run_kv4(InferlabCudaKvPool& p, Kv4Params k, std::uint32_t query_dtype, std::uint32_t num_seqs,
              std::uint32_t max_context_len, void* workspace, std::size_t workspace_bytes,
              cudaStream_t s) {
-    const Kv4Plan plan = plan_kv4(p, num_seqs, k.q_heads, k.max_count, max_context_len);
+    const Kv4Plan plan = plan_kv4(p, num_seqs, k.q_heads, k.max_count, max_context_len, query_dtype);
     if (plan.part_bytes != 0 && (workspace == nullptr || workspace_bytes < plan.counter_bytes + plan.part_bytes)) {
         throw std::runtime_error("4-bit attention workspace is too small");
     }
@@ -818,20 +819,28 @@ void run_kv4(InferlabCudaKvPool& p, Kv4Params k, std::uint32_t query_dtype, std:
         using RowT = decltype(row_type);
         using QT = decltype(query_type);
         const bool wide = p.head_dim == 128;
-        auto* kernel = plan.rows
-            ? (wide ? kv4_rows_kernel<RowT, QT, 128> : kv4_rows_kernel<RowT, QT, 64>)
-            : wide ? (plan.columns == 4 ? kv4_attention_kernel<RowT, QT, 128, true> : kv4_attention_kernel<RowT, QT, 128, false>)
-                   : (plan.columns == 4 ? kv4_attention_kernel<RowT, QT, 64, true> : kv4_attention_kernel<RowT, QT, 64, false>);
-        const int smem = plan.rows ? (wide ? RowSmem<128>::kBytes : RowSmem<64>::kBytes)
-                                   : kWarps * kRing * kStep * kv4::tile_bytes(static_cast<int>(p.head_dim));
+        void (*kernel)(Kv4Params) = nullptr;
+        int smem = kWarps * kRing * kStep * kv4::tile_bytes(static_cast<int>(p.head_dim));
+        unsigned threads = kWarps * 32;
+        if (plan.kind == Kv4Plan::kColumns) {
+            kernel = wide ? (plan.columns == 4 ? kv4_attention_kernel<RowT, QT, 128, true> : kv4_attention_kernel<RowT, QT, 128, false>)
+                          : (plan.columns == 4 ? kv4_attention_kernel<RowT, QT, 64, true> : kv4_attention_kernel<RowT, QT, 64, false>);
+        } else if constexpr (std::is_same<QT, float>::value) {
+            kernel = wide ? kv4_rows_kernel<RowT, 128> : kv4_rows_kernel<RowT, 64>;
+            smem = wide ? RowSmem<128>::kBytes : RowSmem<64>::kBytes;
+        } else {
+            kernel = wide ? kv4_prefill_tc_kernel<QT, 128> : kv4_prefill_tc_kernel<QT, 64>;
+            smem = wide ? TcSmem<128>::kBytes : TcSmem<64>::kBytes;
+            threads = kTcThreads;
+        }
         static std::atomic<std::uint64_t> allowed[2][3];  // devices whose kernel may use it
-        auto& devices = allowed[wide][plan.rows ? 2 : plan.columns == 4];
+        auto& devices = allowed[wide][plan.kind != Kv4Plan::kColumns ? 2 : plan.columns == 4];
         const std::uint64_t bit = p.device < 64 ? 1ull << p.device : 0;
         if ((devices.load() & bit) == 0) {
             cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute");
             devices.fetch_or(bit);
         }
-        kernel<<<grid, kWarps * 32, smem, s>>>(k);
+        kernel<<<grid, threads, smem, s>>>(k);
     };
     if (p.dtype == kF16) {
         if (query_dtype == kFp32) launch(__half{}, float{});
@@ -855,8 +864,13 @@ extern "C" std::size_t inferlab_cuda_kv4_workspace_size(const InferlabCudaKvPool
         return 0;
     }
     try {
-        const auto plan = ilb::plan_kv4(*pool, num_seqs, q_heads, max_query_count, max_context_len);
-        return plan.counter_bytes + plan.part_bytes;
+        // For either type of query.
+        std::size_t most = 0;
+        for (const std::uint32_t dtype : {ilb::kFp32, ilb::kF16}) {
+            const auto plan = ilb::plan_kv4(*pool, num_seqs, q_heads, max_query_count, max_context_len, dtype);
+            most = std::max(most, plan.counter_bytes + plan.part_bytes);
+        }
+        return most;
     } catch (...) {
         return 0;  // the call itself reports why
     }

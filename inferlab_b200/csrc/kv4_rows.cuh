@@ -51,14 +51,14 @@ __device__ __forceinline__ void ldmatrix4_trans(std::uint32_t (&r)[4], std::uint
                  : "memory");
 }
 
-template <typename RowT, typename QT, int D>
+template <typename RowT, int D>
 __global__ void __launch_bounds__(kRowWarps * 32, 3) kv4_rows_kernel(const Kv4Params p) {
     using L = RowSmem<D>;
+    using QT = float;
     constexpr int kTile = kv4::tile_bytes(D);
     constexpr int kGroups = D / kv4::kGroup;
     constexpr int kUnits = D / 8;  // words of a token's row
     constexpr int kSteps = D / 16;
-    constexpr bool kTwoParts = std::is_same<QT, float>::value;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ std::uint32_t ticket;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) kv4_rows_kernel(const Kv4Pa
                     for (int r = 0; r < 2; ++r) {
                         const float w0 = scaled[h][k][r].x, w1 = scaled[h][k][r].y;
                         a[2 * h + r] = f16_pair(w0, w1);
-                        if constexpr (kTwoParts) {
+                        {
                             const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&a[2 * h + r]));
                             a2[2 * h + r] = f16_pair(w0 - t.x, w1 - t.y);
                         }
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) kv4_rows_kernel(const Kv4Pa
                     ldmatrix4_trans(vf, at + L::kValue + token * L::kRow + ((unit ^ (token & 7)) << 4));
                     mma_f16(o[u], a[0], a[1], a[2], a[3], vf[0], vf[1]);
                     mma_f16(o[u + 1], a[0], a[1], a[2], a[3], vf[2], vf[3]);
-                    if constexpr (kTwoParts) {
+                    {
                         mma_f16(o[u], a2[0], a2[1], a2[2], a2[3], vf[0], vf[1]);
                         mma_f16(o[u + 1], a2[0], a2[1], a2[2], a2[3], vf[2], vf[3]);
                     }

@@ -66,8 +66,14 @@ def rounding(kind, ref):
     return EPS[kind] * np.abs(ref) + (2.0 ** -25 if kind == "f16" else 0.0)
 
 
-def attention_bound(kind, out, reach, size, dim):
+def attention_bound(kind, out, reach, size, dim, f16_cache=False):
+    """Share of the largest value by which weights may be off (relative errors of scores, weights, sums), twice for a
+    quotient of two sums. `f16_cache`: keys and values are widened to f16 of an exact power of two, which is off by 2^-11
+    of each: a score sum q k by 2^-11 of sum |q k| (and with it exp of it), a value by 2^-11 of it (below 2^-14 of the
+    row's largest by 2^-40 of that, covered by the last term)."""
     share = (dim + 64) * 2.0 ** -24 * reach + (2.0 ** -17 if kind == "f32" else 2.0 ** -11) + 2.0 ** -21
+    if f16_cache:
+        share = share + 2.0 ** -11 * reach + 2.0 ** -11
     extra = (2 * share * size)[..., None]
     return rounding(kind, np.abs(out) + extra) + extra
 
@@ -357,7 +363,8 @@ def check_attention(torch, kv4, il, kind, q_kind, heads, q_heads, dim, block, st
             continue
         keys, values = kv4.read_rows(arena, tables[i], int(totals[i]), dim)
         out, reach, size = kv4.attend(rounded[at:at + n], keys, values, int(first))
-        within(got[at:at + n], out, attention_bound(q_kind, out, reach, size, dim))
+        many = not decode and q_kind != "f32" and q_heads // heads * int(counts.max()) > 24
+        within(got[at:at + n], out, attention_bound(q_kind, out, reach, size, dim, f16_cache=many))
         at += n
     pool.close()
 
@@ -399,6 +406,85 @@ def test_prefill_splits(torch, kv4, il, split):
 @pytest.mark.parametrize("heads,q_heads,dim,block,start,count", [(1, 4, 128, 16, 0, 600), (2, 2, 64, 32, 1000, 300), (1, 8, 128, 16, 2500, 130)])
 def test_prefill_long_chunks(torch, kv4, il, heads, q_heads, dim, block, start, count):
     check_attention(torch, kv4, il, "bf16", "bf16", heads, q_heads, dim, block, [start, 0], [count, 37], poison=False)
+
+
+@pytest.mark.parametrize("heads,q_heads,dim,block", [(2, 8, 128, 16), (1, 7, 64, 32), (3, 3, 128, 64), (1, 16, 64, 16)])
+@pytest.mark.parametrize("kind,q_kind", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32"), ("f16", "f32")])
+def test_prefill_around_row_tiles(torch, kv4, il, kind, q_kind, heads, q_heads, dim, block):
+    """Rows one below, at and above 64 and 128, keys around 64, with and without splits of the keys."""
+    group = q_heads // heads
+    counts = [max(1, n // group + extra) for n in (63, 64, 127, 128, 256) for extra in (0, 1)] + [0, 1]
+    starts = [0, 1, 63, 64, 65, 127, 0, 300, 15, 0, 20, 0]
+    for split in (0, 4, 12):
+        check_attention(torch, kv4, il, kind, q_kind, heads, q_heads, dim, block, starts, counts, seed=split, split=split)
+
+
+@pytest.mark.parametrize("q_kind", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prefill_many_rows_large_and_tiny_scales(torch, kv4, il, dim, q_kind):
+    """40 query tokens: keys whose scores differ a lot, values of very different size token by token."""
+    rng = np.random.default_rng(dim)
+    length, count = 333, 40
+    tables, blocks = deal(rng, [length], 16)
+    for q_size, spread in ((0.0, 1.0), (1.0, 1e3), (12.0, 1.0), (1e-20, 1e-2), (3e2, 10.0)):
+        arena = np.zeros((blocks, 2, 1, kv4.tile_bytes(dim)), np.uint8)
+        keys = rng.standard_normal((length, 2, dim)).astype(np.float32)
+        values = (rng.standard_normal((length, 2, dim)) * spread ** rng.uniform(-1, 1, (length, 2, 1))).astype(np.float32)
+        values[::7] = np.float32(0.25)  # groups without a range: scale 0
+        kv4.write_rows(arena, tables[0, np.arange(length) // 16], np.arange(length) % 16, kv4.bf16(keys), kv4.bf16(values))
+        pool = filled_pool(torch, il, arena, "bf16", 16, dim)
+        raw = kv4.bf16(rng.standard_normal((count, 8, dim)) * q_size)
+        q = torch.from_numpy(raw).to("cuda:0", kind_of(torch, q_kind))
+        got = host(pool.prefill(q, i32(torch, tables), i32(torch, [length - count]), i32(torch, [count]), i32(torch, [0]), count,
+                                max_context_len=length))
+        pool.synchronize()
+        k, v = kv4.read_rows(arena, tables[0], length, dim)
+        out, reach, size = kv4.attend(raw.astype(np.float64), k, v, length - count)
+        within(got, out, attention_bound(q_kind, out, reach, size, dim, f16_cache=q_kind != "f32"))
+        pool.close()
+
+
+@pytest.mark.parametrize("q_kind", ["bf16", "f32"])
+def test_prefill_of_many_rows_reports_what_it_cannot_read(torch, kv4, il, q_kind):
+    rng = np.random.default_rng(13)
+    tables, blocks = deal(rng, [90, 90], 16)
+    arena = random_arena(kv4, rng, blocks, 1, 16, 64)
+    pool = filled_pool(torch, il, arena, "bf16", 16, 64)
+    raw = kv4.bf16(rng.standard_normal((60, 2, 64)))
+    q = torch.from_numpy(raw).to("cuda:0", kind_of(torch, q_kind))
+
+    def run(queries=q, starts=(60, 60), counts=(30, 30), offsets=(0, 30), at=tables):
+        out = torch.full((60, 2, 64), 7.0, device="cuda:0", dtype=q.dtype)
+        pool.prefill(queries, i32(torch, at), i32(torch, starts), i32(torch, counts), i32(torch, offsets), 30, max_context_len=90, out=out)
+        return host(out)
+
+    good = run()
+    pool.synchronize()
+    for change, rows in ((dict(starts=(60, 61)), "zero"), (dict(starts=(60, -1)), "zero"), (dict(counts=(30, 31)), "kept"),
+                         (dict(offsets=(0, 31)), "kept"), (dict(offsets=(0, -1)), "kept"), (dict(counts=(30, -1)), "kept")):
+        out = run(**change)
+        with pytest.raises(il.AttentionError, match="^paged prefill segment is invalid$"):
+            pool.synchronize()
+        assert np.array_equal(out[:30], good[:30]) and (out[30:] == (0.0 if rows == "zero" else 7.0)).all()
+    for bad in (-1, blocks, 1 << 30):
+        broken = tables.copy()
+        broken[1, 4] = bad
+        out = run(at=broken)
+        with pytest.raises(il.AttentionError, match="^paged KV block table contains an invalid page$"):
+            pool.synchronize()
+        assert np.array_equal(out[:30], good[:30])
+    for value in (float("nan"), float("inf")):
+        wrong = q.clone()
+        wrong[40, 1, 5] = value
+        out = run(wrong)
+        with pytest.raises(il.AttentionError, match="^attention input must be finite$"):
+            pool.synchronize()
+        assert np.array_equal(out[:30], good[:30])
+    # rows behind and between the segments stay as they are
+    out = run(counts=(20, 25))
+    pool.synchronize()
+    assert (out[20:30] == 7.0).all() and (out[55:] == 7.0).all()
+    pool.close()
 
 
 def test_decode_long_flat_and_sharp(torch, kv4, il):
