@@ -45,7 +45,7 @@ struct TcSmem {
     static constexpr int kTops = kValueScales + 2 * kScaleBytes, kRaw = kTops + 2 * kTcRows * 4;
     static constexpr int kBars = kRaw + kBlockTiles * kv4::tile_bytes(D);
     static constexpr int kBytes = kBars + 16 + 1024;  // aligned by hand
-    static_assert(kTcRows * 4 <= kStage && 2 * kTcRows * 4 <= kGroups * kQGroup, "what threads of a row tell each other");
+    static_assert(kBlockTiles * kv4::half_tile_bytes(D) <= kStage, "the first raw keys lie in a stage");
     static constexpr int kTmem = D == 128 ? 256 : 128;  // columns: S, then O (a power of two)
 };
 enum { kTcS = 0, kTcDone, kTcBars };
@@ -64,6 +64,17 @@ __device__ __forceinline__ void tmem_wait16(std::uint32_t (&r)[16]) {
                    "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                  :
                  : "memory");
+}
+
+// One lane of a converged warp, the same for all of its lanes.
+__device__ __forceinline__ bool elect_one() {
+    std::uint32_t chosen;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(chosen));
+    return chosen != 0;
 }
 
 template <typename QT, int D>
@@ -126,33 +137,44 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
         tc::tmem_relinquish();
     }
     // Warp w brings the keys of tile w of a block, warp 4 + w the values of the
-    // block before. Its block id is asked for a block ahead.
+    // block before, block after block; the next one's id is asked for a block
+    // ahead. Tiles within a pool block are counted, not divided for.
     const std::int32_t* table = p.tables + static_cast<std::size_t>(seq) * p.max_blocks;
-    auto id_of = [&](int b) {
-        return table[min(static_cast<std::uint32_t>((from + max(b, 0)) * kBlockTiles + (warp & 3)) / p.tiles_per_block, p.max_blocks - 1)];
-    };
-    std::int32_t next_id = id_of(warp < 4 ? 0 : -1);
-    auto fetch = [&](int key_block) {
-        const int b = warp < 4 ? key_block : key_block - 1, tile = (from + b) * kBlockTiles + (warp & 3);
-        if (b >= 0 && b < blocks && tile < tiles) {
+    std::uint32_t tile = static_cast<std::uint32_t>(from * kBlockTiles + (warp & 3));
+    std::uint32_t in_block = tile % p.tiles_per_block, pool_block = tile / p.tiles_per_block;
+    const std::uint32_t block_step = kBlockTiles / p.tiles_per_block, tile_step = kBlockTiles % p.tiles_per_block;
+    const std::uint32_t stop = min(static_cast<std::uint32_t>(tiles), static_cast<std::uint32_t>((from + blocks) * kBlockTiles));
+    std::int32_t next_id = table[min(pool_block, p.max_blocks - 1)];
+    auto fetch = [&](std::uint32_t raw) {
+        if (tile < stop) {
             std::int32_t block = next_id;
             if (block < 0 || static_cast<std::uint64_t>(block) >= p.num_blocks) {
                 if (lane == 0) flag_error(p.error_word, kErrBadBlock);
                 block = 0;  // never dereferenced outside the pool
             }
-            const std::uint64_t index = (static_cast<std::uint64_t>(block) * p.kv_heads + kv_head) * p.tiles_per_block +
-                                        static_cast<std::uint32_t>(tile) % p.tiles_per_block;
+            const std::uint64_t index = (static_cast<std::uint64_t>(block) * p.kv_heads + kv_head) * p.tiles_per_block + in_block;
             constexpr int kHalf = kv4::half_tile_bytes(D);
             const unsigned char* src = p.arena + index * kTile + (warp < 4 ? 0 : kHalf) + lane * 16;
-            const std::uint32_t to = at + L::kRaw + warp * kHalf + lane * 16;
+            const std::uint32_t to = raw + warp * kHalf + lane * 16;
 #pragma unroll
             for (int c = 0; c < kHalf; c += 512) {
                 if (c + 512 <= kHalf || lane * 16 < kHalf - c) cp_async16(to + c, src + c);
             }
         }
-        cp_async_commit();
-        next_id = id_of(b + 1);
+        tile += kBlockTiles;
+        in_block += tile_step;
+        pool_block += block_step;
+        if (in_block >= p.tiles_per_block) in_block -= p.tiles_per_block, ++pool_block;
+        next_id = table[min(pool_block, p.max_blocks - 1)];
     };
+    // The first keys come into a stage that is not used yet, so that two blocks
+    // are on their way at once.
+    constexpr int kFirst = L::kV + L::kStage;
+    if (warp < 4) fetch(at + kFirst);
+    cp_async_commit();
+    fetch(at + L::kRaw);
+    cp_async_commit();
+
     // Widens a code row's 16 bytes (four words) of keys or values.
     constexpr int kItems = kTcKeys * kUnits / 4;
     const int item = threadIdx.x % kItems, index = item / (kUnits / 4), part16 = item % (kUnits / 4);
@@ -197,9 +219,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
         if (part16 == 0) scales[token] = __uint_as_float((exponent - 14u) << 23);
     };
     // The raw keys become block `key_block`, the raw values the one before.
-    auto widen = [&](int key_block) {
+    auto widen = [&](int key_block, int raw) {
         const int value_block = key_block - 1;
-        const unsigned char* tile = smem + L::kRaw + token / kv4::kTileTokens * kv4::half_tile_bytes(D);
+        const unsigned char* tile = smem + raw + token / kv4::kTileTokens * kv4::half_tile_bytes(D);
         if (key_block < blocks && (kItems == kTcThreads || threadIdx.x < kItems)) {
             widen_row(tile, smem + L::kK + (key_block & 1) * L::kStage,
                       reinterpret_cast<float*>(smem + L::kKeyScales + (key_block & 1) * L::kScaleBytes),
@@ -214,22 +236,21 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
         }
         fence_proxy_async_shared();
     };
-    fetch(0);
-
-    // ---- queries: a row a thread of the first half, scaled by a power of two
-    // (exact) into f16's range, in the codes' order.
+    // ---- queries: half a row a thread, scaled by a power of two (exact) into
+    // f16's range, in the codes' order.
     const int row = threadIdx.x % kTcRows, half = threadIdx.x / kTcRows;
     const int limit = row < live ? static_cast<int>(start + token_of(row) + 1) : 0;
-    float* told = reinterpret_cast<float*>(smem + L::kV + L::kStage);  // a stage not used yet
-    if (half == 0) {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const QT*>(p.queries) + row_of(min(row, live - 1)) * D);
-        uint4 raw[kUnits];
+    float* tops = reinterpret_cast<float*>(smem + L::kTops);
+    std::uint32_t query_exponent;
+    {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const QT*>(p.queries) + row_of(min(row, live - 1)) * D + half * (D / 2));
+        uint4 raw[kUnits / 2];
         float most = 0.0f;
         bool bad = false;
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) raw[u] = row < live ? src[u] : make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < kUnits / 2; ++u) raw[u] = row < live ? src[u] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
+        for (int u = 0; u < kUnits / 2; ++u) {
             float x[8];
             widen16(raw[u], x, QT{});
 #pragma unroll
@@ -239,51 +260,51 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
             }
         }
         if (bad) flag_error(p.error_word, kErrNonFinite);
-        const int exponent = max(15, static_cast<int>(__float_as_uint(most) >> 23));
-        const float up = most > 0.0f ? __uint_as_float(static_cast<std::uint32_t>(min(254, 268 - exponent)) << 23) : 1.0f;
-        told[row] = p.scale_log2 * __uint_as_float(static_cast<std::uint32_t>(exponent - 14) << 23);
+        tops[threadIdx.x] = most;
+        cp_async_wait_group<1>();
+        __syncthreads();
+        most = fmaxf(tops[row], tops[row + kTcRows]);
+        query_exponent = max(15u, __float_as_uint(most) >> 23);
+        const float up = most > 0.0f ? __uint_as_float(min(254u, 268u - query_exponent) << 23) : 1.0f;
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
+        for (int u = 0; u < kUnits / 2; ++u) {
             float x[8];
             widen16(raw[u], x, QT{});
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] *= up;
-            *reinterpret_cast<uint4*>(smem + L::kQ + (u / 8) * L::kQGroup + row * 128 + ((u % 8 ^ (row & 7)) << 4)) =
+            const int unit = half * (kUnits / 2) + u;
+            *reinterpret_cast<uint4*>(smem + L::kQ + (unit / 8) * L::kQGroup + row * 128 + ((unit % 8 ^ (row & 7)) << 4)) =
                 make_uint4(f16_pair(x[0], x[4]), f16_pair(x[1], x[5]), f16_pair(x[2], x[6]), f16_pair(x[3], x[7]));
         }
-        fence_proxy_async_shared();
     }
+    const float factor = p.scale_log2 * __uint_as_float((query_exponent - 14u) << 23);
+    widen(0, kFirst);
     cp_async_wait_group<0>();
-    __syncthreads();
-    widen(0);
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
-    const std::uint32_t tmem = tmem_at, my = tmem + (static_cast<std::uint32_t>((warp & 3) * 32) << 16);
+    // The same in all lanes, and known to be.
+    const std::uint32_t tmem = __shfl_sync(0xffffffffu, tmem_at, 0), at0 = __shfl_sync(0xffffffffu, at, 0);
+    const bool issuer = __shfl_sync(0xffffffffu, warp, 0) == 0;
+    const std::uint32_t my = tmem + (static_cast<std::uint32_t>((warp & 3) * 32) << 16);
     const tc::Waiter wait{&abort, p.error_word};
-    const float factor = told[row];
     // S of block b.
     auto scores = [&](int b) {
 #pragma unroll
         for (int k = 0; k < kGroups; ++k) {
-            const std::uint64_t q = tc::sw128_desc(at + L::kQ + k * L::kQGroup, 16, 1024);
-            const std::uint64_t key = tc::sw128_desc(at + L::kK + (b & 1) * L::kStage + k * L::kKeyGroup, 16, 1024);
+            const std::uint64_t q = tc::sw128_desc(at0 + L::kQ + k * L::kQGroup, 16, 1024);
+            const std::uint64_t key = tc::sw128_desc(at0 + L::kK + (b & 1) * L::kStage + k * L::kKeyGroup, 16, 1024);
 #pragma unroll
             for (int i = 0; i < 4; ++i) tc::mma_f16(tmem, q + 2 * i, key + 2 * i, tc::idesc_f16(0, 0, 0, kTcKeys), k > 0 || i > 0);
         }
         tc::mma_commit(&bars[kTcS]);
     };
-    if (threadIdx.x == 0) scores(0);
-    __syncwarp();
-    fetch(1);
-    cp_async_wait_group<0>();
-    __syncthreads();
-    widen(1);
+    if (issuer && elect_one()) scores(0);
+    widen(1, L::kRaw);
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars[kTcS]);
 
     const int clear = static_cast<int>(start + token_of(0) + 1);  // keys that all rows see
-    float* tops = reinterpret_cast<float*>(smem + L::kTops);
     float m = kNoScore;
     float2 l2 = make_float2(0.0f, 0.0f);
     for (int b = 0; b < blocks; ++b) {
@@ -320,7 +341,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
         const float* units = reinterpret_cast<const float*>(smem + L::kValueScales + (b & 1) * L::kScaleBytes) + 32 * half;
         std::uint32_t weights[16];
         float2 sum;
-        float most;
+        float most = 0.0f;
         auto weigh = [&] {
             sum = make_float2(0.0f, 0.0f);
             most = 0.0f;
@@ -337,10 +358,11 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
                 }
             }
         };
-        weigh();
-        const bool rescale = __syncthreads_or(most > 32768.0f);
+        if (b > 0) weigh();
+        const bool rescale = __syncthreads_or(b == 0 || most > 32768.0f);
         if (*reinterpret_cast<volatile int*>(&abort)) break;  // set before the barrier only: the same for all
-        fetch(b + 2);
+        fetch(at + L::kRaw);
+        cp_async_commit();
         if (rescale) {
             float top = kNoScore;
 #pragma unroll
@@ -373,10 +395,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
         tc::tmem_store_wait();
         tc::tc_fence_before();
         __syncthreads();  // the weights and the raw tiles are there
-        if (threadIdx.x == 0) {
+        if (issuer && elect_one()) {
             tc::tc_fence_after();
             // V is MN-major, 64 dims an atom.
-            const std::uint64_t v = tc::sw128_desc(at + L::kV + (b & 1) * L::kStage, L::kKeyGroup, 1024);
+            const std::uint64_t v = tc::sw128_desc(at0 + L::kV + (b & 1) * L::kStage, L::kKeyGroup, 1024);
 #pragma unroll
             for (int i = 0; i < kTcKeys / 16; ++i) {
                 tc::mma_f16_tmem_a(tmem + kTcKeys, tmem + 8 * i, v + 128 * i, tc::idesc_f16(0, 0, 1, D), b > 0 || i > 0);
@@ -385,7 +407,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
             else tc::mma_commit(&bars[kTcS]);
         }
         __syncwarp();
-        widen(b + 2);
+        widen(b + 2, L::kRaw);
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[kTcS]);
     }
