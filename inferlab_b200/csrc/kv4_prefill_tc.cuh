@@ -46,6 +46,7 @@ struct TcSmem {
     static constexpr int kBars = kRaw + kBlockTiles * kv4::tile_bytes(D);
     static constexpr int kBytes = kBars + 16 + 1024;  // aligned by hand
     static_assert(kBlockTiles * kv4::half_tile_bytes(D) <= kStage, "the first raw keys lie in a stage");
+    static_assert(kTcRows * D * 4 <= kV - kQ && 2 * kTcRows * 4 <= kStage, "the output lies over queries and keys");
     static constexpr int kTmem = D == 128 ? 256 : 128;  // columns: S, then O (a power of two)
 };
 enum { kTcS = 0, kTcDone, kTcBars };
@@ -66,6 +67,11 @@ __device__ __forceinline__ void tmem_wait16(std::uint32_t (&r)[16]) {
                  : "memory");
 }
 
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // One lane of a converged warp, the same for all of its lanes.
 __device__ __forceinline__ bool elect_one() {
     std::uint32_t chosen;
@@ -181,7 +187,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
     // Eight lanes that store at once hold rows whose numbers differ by an odd
     // number across 4, so that their swizzled chunks differ.
     const int token = (index & ~7) + ((index & 7) >> 1 ^ (index & 1) * 5), slot = token % kv4::kTileTokens;
-    auto widen_row = [&](const unsigned char* tile, unsigned char* to, float* scales, bool seen, auto unit_of) {
+    // Word 4 part16 + j holds the dims of unit (base ^ bits(j)) % 8 of group(j)
+    // (kv4.cuh's order): where that is in a swizzled row.
+    const int key_at = token * 128 + (((part16 << (D == 128 ? 0 : 1)) ^ (token & 7)) << 4);
+    const int value_at = token * 128 + (((part16 << (D == 128 ? 1 : 2)) ^ (D == 128 ? (slot & 2) << 1 : 0) ^ (token & 7)) << 4);
+    auto widen_row = [&](const unsigned char* tile, unsigned char* to, float* scales, bool seen, auto values_too) {
+        constexpr bool kValue = decltype(values_too)::value;
         const uint4 x = *reinterpret_cast<const uint4*>(tile + slot * (D / 2) + part16 * 16);
         const std::uint32_t word[4] = {x.x, x.y, x.z, x.w};
         float2 pair[kGroups];
@@ -211,9 +222,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
         };
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int unit = unit_of(4 * part16 + j), k = kGroups == 1 ? 0 : unit_of(j) / 8;  // the group is the same in all parts
+            const int bits = kValue ? (D == 128 ? j >> 1 : j) : (j & 1) << 2 | (D == 128 ? 0 : j >> 1);
+            const int k = D == 128 ? (kValue ? j & 1 : j >> 1) : 0;
             const std::uint32_t high = word[j] >> 8;
-            *reinterpret_cast<uint4*>(to + k * L::kKeyGroup + token * 128 + ((unit % 8 ^ (token & 7)) << 4)) =
+            *reinterpret_cast<uint4*>(to + k * L::kKeyGroup + ((kValue ? value_at : key_at) ^ bits << 4)) =
                 make_uint4(values(word[j], false, k), values(word[j], true, k), values(high, false, k), values(high, true, k));
         }
         if (part16 == 0) scales[token] = __uint_as_float((exponent - 14u) << 23);
@@ -226,13 +238,13 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
             widen_row(tile, smem + L::kK + (key_block & 1) * L::kStage,
                       reinterpret_cast<float*>(smem + L::kKeyScales + (key_block & 1) * L::kScaleBytes),
                       (from + key_block) * kTcKeys + token < longest,
-                      [](int w) { return ((w % (D / 32)) << 2) + w / (D / 32); });
+                      std::false_type{});
         }
         if (value_block >= 0 && value_block < blocks && (kItems == kTcThreads || threadIdx.x >= kItems)) {
             widen_row(tile + kBlockTiles * kv4::half_tile_bytes(D), smem + L::kV + (value_block & 1) * L::kStage,
                       reinterpret_cast<float*>(smem + L::kValueScales + (value_block & 1) * L::kScaleBytes),
                       (from + value_block) * kTcKeys + token < longest,
-                      [&](int w) { return (w % kGroups) * 8 + (w / kGroups ^ (D == 128 ? ((slot >> 1) & 1) * 4 : 0)); });
+                      std::true_type{});
         }
         fence_proxy_async_shared();
     };
@@ -368,7 +380,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float2 unit = *reinterpret_cast<const float2*>(units + 2 * i);
-                top = fmax3(top, __fadd_rn(s[i].x, __log2f(unit.x)), __fadd_rn(s[i].y, __log2f(unit.y)));
+                top = fmax3(top, __fadd_rn(s[i].x, lg2(unit.x)), __fadd_rn(s[i].y, lg2(unit.y)));
             }
             tops[threadIdx.x] = top;
             __syncthreads();
@@ -414,7 +426,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
     // ---- the row's output, or its sums for the merge; half of the dims a thread.
     if (!tc::warp_ok(wait(&bars[kTcS], blocks & 1))) l2 = make_float2(0.0f, 0.0f);
     tc::tc_fence_after();
-    float* sums = reinterpret_cast<float*>(smem + L::kQ);
+    float* sums = reinterpret_cast<float*>(smem + L::kV);
     sums[threadIdx.x] = l2.x + l2.y;
     __syncthreads();
     const bool whole = splits == 1;
@@ -423,10 +435,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
         const bool good = isfinite(l) && l > 0.0f;
         if (whole && !good && row < live) flag_error(p.error_word, kErrNormalizer);
         const float inv = !whole ? 1.0f : good ? 1.0f / l : 0.0f;
-        // A split's sums: o [row][D], then m and l per row (padded).
+        // Through shared memory (over Q and K, 16-byte chunks swizzled by the row),
+        // so that a row leaves in one piece; a split's sums are o [row][D], then
+        // m and l per row (padded).
         float* part = p.ws_part + (static_cast<std::size_t>(work) * p.max_splits + split) * (kTcRows * (D + 4));
         if (!whole && half == 0) *reinterpret_cast<float2*>(part + kTcRows * D + 2 * row) = make_float2(m, l);
-        QT* out = static_cast<QT*>(p.out) + row_of(min(row, live - 1)) * D;
+        auto staged = [&](int r, int chunk) { return reinterpret_cast<float4*>(smem + L::kQ + r * D * 4 + ((chunk ^ (r & 7)) << 4)); };
 #pragma unroll
         for (int c0 = 0; c0 < D / 2; c0 += 16) {
             const int c1 = half * (D / 2) + c0;
@@ -434,19 +448,19 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
             tmem_load16(my + kTcKeys + c1, o);
             tmem_wait16(o);
 #pragma unroll
-            for (int u = 0; u < 16; u += 8) {
-                float x[8];
+            for (int u = 0; u < 16; u += 4) {
+                float x[4];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(o[u + 2 * (i & 3) + (i >> 2)]) * inv;
-                if (row >= live) continue;
-                if (whole) {
-                    store_row4(out + c1 + u, make_float4(x[0], x[1], x[2], x[3]));
-                    store_row4(out + c1 + u + 4, make_float4(x[4], x[5], x[6], x[7]));
-                } else {
-                    store_row4(part + row * D + c1 + u, make_float4(x[0], x[1], x[2], x[3]));
-                    store_row4(part + row * D + c1 + u + 4, make_float4(x[4], x[5], x[6], x[7]));
-                }
+                for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(o[(u & 8) + 2 * i + (u >> 2 & 1)]) * inv;
+                *staged(row, (c1 + u) / 4) = make_float4(x[0], x[1], x[2], x[3]);
             }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < live * D / 4; i += kTcThreads) {
+            const int r = i / (D / 4);
+            const float4 x = *staged(r, i % (D / 4));
+            if (whole) store_row4(static_cast<QT*>(p.out) + row_of(r) * D + 4 * i % D, x);
+            else store_row4(part + 4 * i, x);
         }
     }
     if (threadIdx.x == 0) {
@@ -463,13 +477,16 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
     if (splits == 1) return;
     if (!last_of(p.ws_count + work, splits, ticket)) return;
     const float* parts = p.ws_part + static_cast<std::size_t>(work) * p.max_splits * (kTcRows * (D + 4));
-    for (int i = threadIdx.x; i < live * D / 4; i += blockDim.x) {
+    bool all_good = true;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < live * D / 4; i += kTcThreads) {
         const int r = i / (D / 4);
         bool good;
         const float4 x = merge_parts<kTcRows * (D + 4), kTcRows * D>(parts, splits, r, i, good);
-        if (!good) flag_error(p.error_word, kErrNormalizer);
+        all_good &= good;
         store_row4(static_cast<QT*>(p.out) + row_of(r) * D + 4 * i % D, x);
     }
+    if (!all_good) flag_error(p.error_word, kErrNormalizer);
 }
 
 }  // namespace
