@@ -142,6 +142,16 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
         tc::tmem_alloc(&tmem_at, L::kTmem);
         tc::tmem_relinquish();
     }
+    // The queries come as they are to where they go; 16-byte chunks of 64 dims of
+    // a row, swizzled.
+    const int row = threadIdx.x % kTcRows, half = threadIdx.x / kTcRows;
+    auto query_at = [&](int r, int unit) { return L::kQ + (unit / 8) * L::kQGroup + r * 128 + ((unit % 8 ^ (r & 7)) << 4); };
+#pragma unroll
+    for (int i = 0; i < kTcRows * kUnits / kTcThreads; ++i) {
+        const int r = (threadIdx.x + i * kTcThreads) / kUnits, unit = threadIdx.x % kUnits;
+        cp_async16(at + query_at(r, unit), static_cast<const QT*>(p.queries) + row_of(min(r, live - 1)) * D + unit * 8);
+    }
+    cp_async_commit();
     // Warp w brings the keys of tile w of a block, warp 4 + w the values of the
     // block before, block after block; the next one's id is asked for a block
     // ahead. Tiles within a pool block are counted, not divided for.
@@ -250,17 +260,17 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
     };
     // ---- queries: half a row a thread, scaled by a power of two (exact) into
     // f16's range, in the codes' order.
-    const int row = threadIdx.x % kTcRows, half = threadIdx.x / kTcRows;
     const int limit = row < live ? static_cast<int>(start + token_of(row) + 1) : 0;
     float* tops = reinterpret_cast<float*>(smem + L::kTops);
     std::uint32_t query_exponent;
+    cp_async_wait_group<1>();
+    __syncthreads();
     {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const QT*>(p.queries) + row_of(min(row, live - 1)) * D + half * (D / 2));
         uint4 raw[kUnits / 2];
         float most = 0.0f;
         bool bad = false;
 #pragma unroll
-        for (int u = 0; u < kUnits / 2; ++u) raw[u] = row < live ? src[u] : make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < kUnits / 2; ++u) raw[u] = row < live ? *reinterpret_cast<const uint4*>(smem + query_at(row, half * (kUnits / 2) + u)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int u = 0; u < kUnits / 2; ++u) {
             float x[8];
@@ -273,7 +283,6 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
         }
         if (bad) flag_error(p.error_word, kErrNonFinite);
         tops[threadIdx.x] = most;
-        cp_async_wait_group<1>();
         __syncthreads();
         most = fmaxf(tops[row], tops[row + kTcRows]);
         query_exponent = max(15u, __float_as_uint(most) >> 23);
@@ -284,8 +293,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
             widen16(raw[u], x, QT{});
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] *= up;
-            const int unit = half * (kUnits / 2) + u;
-            *reinterpret_cast<uint4*>(smem + L::kQ + (unit / 8) * L::kQGroup + row * 128 + ((unit % 8 ^ (row & 7)) << 4)) =
+            *reinterpret_cast<uint4*>(smem + query_at(row, half * (kUnits / 2) + u)) =
                 make_uint4(f16_pair(x[0], x[4]), f16_pair(x[1], x[5]), f16_pair(x[2], x[6]), f16_pair(x[3], x[7]));
         }
     }
