@@ -710,14 +710,21 @@ Kv4Plan plan_kv4(const InferlabCudaKvPool& p, std::uint32_t num_seqs, std::uint3
     Kv4Plan plan{};
     const std::uint64_t rows = static_cast<std::uint64_t>(q_heads / p.kv_heads) * max_count;
     if (rows > 0x7FFFFFFFull) throw std::runtime_error("4-bit attention batch is too large");
-    // Many rows per kv-head share the widened codes. fp32 results need two-part
-    // weights and take the rows kernel.
-    if (max_count > 1 && rows > 24) {
-        plan.kind = query_dtype == kFp32 ? Kv4Plan::kRows : Kv4Plan::kTensor;
-        plan.columns = plan.kind == Kv4Plan::kRows ? kRowTile : kTcRows;
-        const std::uint64_t row_tiles = (rows + plan.columns - 1) / plan.columns;
-        const std::uint64_t row_units = checked_mul(checked_mul(num_seqs, p.kv_heads, "4-bit attention batch is too large"),
-                                                    row_tiles, "4-bit attention batch is too large");
+    // Many rows per kv-head share the widened codes. 16-bit queries from 64 rows
+    // on: 64 segments on contexts of 1200 tokens take 180, 184 and 215 us with 48,
+    // 64 and 128 rows on the tensor cores, 134, 175 and 342 in column tiles; 4 on
+    // 8000 tokens 68, 71 and 81 against 65, 78 and 134. fp32 results need
+    // weights in two parts and take the row kernel from 128 rows on, where its
+    // tiles fill the GPU: 64 fresh prompts of 32 tokens 40 us against 108, 64
+    // segments on 1200 tokens 398 against 379, one prompt of 32 tokens 13 against
+    // 10.
+    const bool tensor = query_dtype != kFp32;
+    const std::uint64_t row_tile = tensor ? kTcRows : kRowTile, row_tiles = (rows + row_tile - 1) / row_tile;
+    const std::uint64_t row_units = checked_mul(checked_mul(num_seqs, p.kv_heads, "4-bit attention batch is too large"),
+                                                row_tiles, "4-bit attention batch is too large");
+    if (max_count > 1 && (tensor ? rows >= 64 : rows >= 128 && row_units >= 148)) {
+        plan.kind = tensor ? Kv4Plan::kTensor : Kv4Plan::kRows;
+        plan.columns = static_cast<std::uint32_t>(row_tile);
         plan.column_tiles = static_cast<std::uint32_t>(row_tiles);
         // Up to 4096 CTAs (nine waves of three an SM) if all contexts were
         // max_context_len long: the lengths are the device's and most are shorter.

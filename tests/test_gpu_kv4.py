@@ -363,7 +363,7 @@ def check_attention(torch, kv4, il, kind, q_kind, heads, q_heads, dim, block, st
             continue
         keys, values = kv4.read_rows(arena, tables[i], int(totals[i]), dim)
         out, reach, size = kv4.attend(rounded[at:at + n], keys, values, int(first))
-        many = not decode and q_kind != "f32" and q_heads // heads * int(counts.max()) > 24
+        many = not decode and q_kind != "f32" and q_heads // heads * int(counts.max()) >= 64
         within(got[at:at + n], out, attention_bound(q_kind, out, reach, size, dim, f16_cache=many))
         at += n
     pool.close()
