@@ -100,8 +100,8 @@ __device__ __forceinline__ float rotated(const RowT* head, std::uint32_t d, cons
 constexpr int kRowThreads = 256;
 
 // Any shape: one CTA per token row, elements (8-dim units in a 4-bit pool)
-// spread over its threads. The row is checked before any of it is written,
-// and the second pass finds it in L1.
+// spread over its threads. K and V are checked before any of them is written,
+// and the second pass finds them in L1; Q goes out either way.
 template <typename RowT, typename PoolT, typename OutT, bool kFourBit>
 __global__ void __launch_bounds__(kRowThreads) rotary_append_kernel(const AppendParams p) {
     const std::size_t row = blockIdx.x;
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kRowThreads) rotary_append_kernel(const Append
             }
             if (pass == 0 && __syncthreads_or(any_bad)) {
                 if (threadIdx.x == 0) flag_error(p.error_word, kErrNonFinite);
-                return;
+                break;
             }
         }
     } else {
@@ -171,11 +171,9 @@ __global__ void __launch_bounds__(kRowThreads) rotary_append_kernel(const Append
             bad |= !isfinite(Storage<PoolT>::to_float(Storage<PoolT>::from_float(k)));
             bad |= !isfinite(Storage<PoolT>::to_float(Storage<PoolT>::from_float(Storage<RowT>::to_float(value_row[i]))));
         }
-        if (__syncthreads_or(bad)) {
-            if (threadIdx.x == 0) flag_error(p.error_word, kErrNonFinite);
-            return;
-        }
-        for (std::size_t i = threadIdx.x; i < width; i += blockDim.x) {
+        const bool rejected = __syncthreads_or(bad);
+        if (rejected && threadIdx.x == 0) flag_error(p.error_word, kErrNonFinite);
+        for (std::size_t i = threadIdx.x; i < width && !rejected; i += blockDim.x) {
             const std::uint32_t head = i / d, dim = i % d;
             const std::size_t dst =
                 ((static_cast<std::size_t>(place.block) * p.kv_heads + head) * p.block_tokens + place.slot) * d + dim;
