@@ -179,6 +179,8 @@ int inferlab_cuda_pool_synchronize(InferlabCudaKvPool* pool, void* stream, uint3
  * sequence row_sequences[r]: block block_tables[seq * max_blocks_per_seq +
  * pos / block_tokens], slot pos % block_tokens. Non-finite values are
  * rejected ("attention input must be finite"); the row is not written.
+ * A 4-bit pool takes the rows quantised from their values rounded to its row
+ * type; a group whose scale or zero f16 cannot hold counts as not finite.
  * All arrays are device memory.
  */
 int inferlab_cuda_kv_append(InferlabCudaKvPool* pool, const void* key_rows, const void* value_rows,
@@ -228,8 +230,8 @@ typedef struct InferlabCudaRotaryAppend {
  * behind the table of angles, is reported through the pool's error word and
  * skipped whole. K/V values that the pool cannot hold as finite numbers (for
  * a 4-bit pool, as a group with finite f16 scale and zero) are reported
- * ("attention input must be finite") and that row is skipped whole. q_out must
- * not overlap the input rows. Two rows of one call with the same sequence and
+ * ("attention input must be finite") and neither K nor V of that row is
+ * written; its Q is. Q is not checked. q_out must not overlap the input rows. Two rows of one call with the same sequence and
  * position leave an unspecified one of the two, in a 4-bit pool possibly a
  * mixture. No counterpart in the reference (its positions are learned vectors).
  */
@@ -295,7 +297,8 @@ int inferlab_cuda_output_project(InferlabCudaKvPool* pool, const void* attention
  * Copies the first `tokens` positions of one sequence into contiguous
  * [tokens][kv_heads][head_dim] arrays of the pool's type, bit for bit: the
  * device form of PagedKvPool::materialize (worker/cpp/inferlab_runtime.cpp:
- * 769-803). block_table holds ceil(tokens / block_tokens) device int32 ids.
+ * 769-803). A 4-bit pool gives the values its codes stand for, rounded to the
+ * row type. block_table holds ceil(tokens / block_tokens) device int32 ids.
  */
 int inferlab_cuda_kv_gather(InferlabCudaKvPool* pool, const int32_t* block_table, uint64_t tokens,
                             void* keys_out, void* values_out, void* stream, char* error,
@@ -493,13 +496,17 @@ int inferlab_cuda_paged_prefill(InferlabCudaKvPool* pool, const void* queries, u
  * segment of count 0 has no rows.
  * queries and out are [..][q_heads][head_dim] of query_dtype: the pool's row
  * type, or fp32 (queries rounded to the row type on load, as the reference's
- * 16-bit modes do). Scores, softmax statistics and sums are fp32.
+ * 16-bit modes do). Scores, softmax statistics and sums are fp32. For a 16-bit
+ * out the weights are rounded to f16, and segments of many rows (64 or more per
+ * kv-head) read keys and values as f16 in units of a power of two per token;
+ * an fp32 out keeps codes and pairs exact and the weights in two f16 parts.
  * max_context_len bounds every context (start + count for segments); a context
  * over it, over the table's width, or negative is reported through the pool's
  * error word and its rows are zero. Long contexts are split across CTAs and
  * merged in split order inside the launch. workspace:
  * inferlab_cuda_kv4_workspace_size bytes, initialised once with
- * inferlab_cuda_paged_decode_workspace_init; launches that may overlap (other
+ * inferlab_cuda_paged_decode_workspace_init. Batches of any shapes may use one
+ * in turn that is large enough for each; launches that may overlap (other
  * streams, graphs replayed side by side) need one each.
  */
 size_t inferlab_cuda_kv4_workspace_size(const InferlabCudaKvPool* pool, uint32_t num_seqs,

@@ -52,6 +52,11 @@ constexpr int kStep = 2;               // tiles a warp takes at once
 constexpr float kHeadroom = 10.0f;     // log2: the largest scaled weight starts at 2^10 (below)
 constexpr float kNoScore = -3.0e38f;   // running maximum before any key
 constexpr std::uint32_t kMaxSplits = 256;
+// The split counters lie at the front of a workspace and are zero between
+// launches; behind them are the partials of whatever batch ran last. So the
+// region is the same for all batches. More units than this fill the GPU many
+// times over and are not split.
+constexpr std::uint32_t kMaxSplitUnits = 16384;
 
 struct Kv4Params {
     const unsigned char* arena;
@@ -731,12 +736,13 @@ Kv4Plan plan_kv4(const InferlabCudaKvPool& p, std::uint32_t num_seqs, std::uint3
         const std::uint64_t all = (max_context_len + kv4::kTileTokens - 1) / kv4::kTileTokens;
         std::uint64_t per = p.decode_blocks_per_split;
         if (per == 0) per = std::max<std::uint64_t>(64, checked_mul(row_units, all, "4-bit attention batch is too large") / 4096);
+        if (row_units > kMaxSplitUnits) per = all;
         per = (std::max<std::uint64_t>(per, (all + kMaxSplits - 1) / kMaxSplits) + kBlockTiles - 1) / kBlockTiles * kBlockTiles;
         plan.tiles_per_split = static_cast<int>(per);
         plan.max_splits = static_cast<std::uint32_t>((all + per - 1) / per);
         if (row_units > 0x7FFFFFFFull / plan.max_splits) throw std::runtime_error("4-bit attention batch is too large");
         if (plan.max_splits > 1) {
-            plan.counter_bytes = (row_units * 4 + 255) & ~std::size_t(255);
+            plan.counter_bytes = kMaxSplitUnits * 4;
             plan.part_bytes = checked_mul(row_units * plan.max_splits, plan.columns * (p.head_dim + 4) * 4, "4-bit attention batch is too large");
         }
         return plan;
@@ -767,13 +773,14 @@ Kv4Plan plan_kv4(const InferlabCudaKvPool& p, std::uint32_t num_seqs, std::uint3
         const std::uint64_t splits = (tiles + per_split - 1) / per_split;
         per_split = (tiles + splits - 1) / splits;
     }
+    if (units > kMaxSplitUnits) per_split = tiles;
     per_split = std::max<std::uint64_t>(per_split, (tiles + kMaxSplits - 1) / kMaxSplits);
     plan.tiles_per_split = static_cast<int>(per_split);
     plan.max_splits = static_cast<std::uint32_t>((tiles + per_split - 1) / per_split);
     if (units > 0x7FFFFFFFull / plan.max_splits) throw std::runtime_error("4-bit attention batch is too large");
     plan.column_tiles = static_cast<std::uint32_t>(column_tiles);
     if (plan.max_splits > 1) {
-        plan.counter_bytes = (units * 4 + 255) & ~std::size_t(255);
+        plan.counter_bytes = kMaxSplitUnits * 4;
         plan.part_bytes = checked_mul(units * plan.max_splits, plan.columns * (p.head_dim + 4) * 4, "4-bit attention batch is too large");
     }
     return plan;

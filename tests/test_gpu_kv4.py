@@ -254,6 +254,18 @@ def test_append_rotary_far_positions_and_bad_rows(torch, il, kv4):
             with pytest.raises(il.AttentionError, match="^attention input must be finite$"):
                 pool.synchronize()
             assert torch.equal(arena()[..., 5, :, :, :] if bits is None else arena()[5], was[..., 5, :, :, :] if bits is None else was[5])
+            # so in rows that no 16-byte load reaches; Q leaves either way
+            odd = torch.zeros((2, 6 * 64 + 1), device="cuda:0")
+            odd[:, 1:] = bad.flatten(1)
+            odd = odd[:, 1:].unflatten(1, (6, 64))
+            outs = [torch.full((2, 2, 64), 9.0, device="cuda:0") for _ in range(2)]
+            for source, out in zip((bad, odd), outs):
+                pool.append_rotary(source[:, :2], source[:, 2:4], source[:, 4:], angles, i32(torch, [0, 1]), i32(torch, [3, 4]), tables,
+                                   q_out=out)
+                with pytest.raises(il.AttentionError, match="^attention input must be finite$"):
+                    pool.synchronize()
+            assert torch.equal(arena()[..., 5, :, :, :] if bits is None else arena()[5], was[..., 5, :, :, :] if bits is None else was[5])
+            assert torch.equal(outs[0], outs[1]) and not (outs[0] == 9).any()
         # a 4-bit group whose scale f16 cannot hold
         if bits:
             wide = rows.clone()
@@ -264,6 +276,32 @@ def test_append_rotary_far_positions_and_bad_rows(torch, il, kv4):
                 pool.synchronize()
             assert torch.equal(arena(), was)
         pool.close()
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+def test_append_rotary_rejects_what_the_row_type_cannot_hold(torch, il, shift):
+    """fp32 rows over 16-bit pools: 65520 is the first number that f16 rounds to infinity, and a rotation can reach it. `shift` 1:
+    rows that no 16-byte load reaches."""
+    turn = torch.tensor([[0.6] * 32 + [0.8] * 32] * 8, device="cuda:0")
+    for kind, bits, value, angles, ok in ((1, None, 65519.0, None, True), (1, None, 65520.0, None, False), (1, 4, 70000.0, None, False),
+                                          (2, None, 70000.0, None, True), (2, None, 3.4e38, None, False), (1, None, 60000.0, turn, False),
+                                          (1, None, 40000.0, turn, True), (2, 4, 4e5, None, True), (2, 4, 6e5, None, False)):
+        for which in (0, 1):
+            if angles is not None and which == 1:
+                continue  # values are not rotated
+            pool = il.CudaKvPool(0, kind, 4, 16, 2, 64, kv_bits=bits)
+            flat = torch.zeros((1, 4 * 64 + shift), device="cuda:0")
+            rows = flat[:, shift:].unflatten(1, (4, 64))
+            rows[0, 2 * which + 1, 3] = value
+            rows[0, 2 * which + 1, 35] = -value
+            pool.append_rotary(None, rows[:, :2], rows[:, 2:], angles, i32(torch, [0]), i32(torch, [5]), i32(torch, [[2]]))
+            if ok:
+                pool.synchronize()
+            else:
+                with pytest.raises(il.AttentionError, match="^attention input must be finite$"):
+                    pool.synchronize()
+                assert not (pool.arena if bits else torch.stack([pool.key_arena, pool.value_arena])).any()
+            pool.close()
 
 
 def test_append_rotary_refusals(torch, il):
@@ -665,6 +703,93 @@ def test_repeated_and_captured_calls_agree(torch, il, kv4):
         back = pool.decode(q, table, lens, 900, stream=torch.cuda.default_stream())
     torch.cuda.synchronize()
     assert torch.equal(elsewhere, first) and torch.equal(back, first)
+    pool.synchronize()
+    pool.close()
+
+
+def test_batches_of_all_shapes_share_a_workspace(torch, il, kv4):
+    """Split decodes and prefills of few and many rows in turn on one workspace: each as on a workspace of its own."""
+    rng = np.random.default_rng(21)
+    lengths = np.array([1500, 700, 1, 64, 333, 80, 1200, 16] * 6)
+    tables, blocks = deal(rng, lengths, 16)
+    pool = filled_pool(torch, il, random_arena(kv4, rng, blocks, 2, 16, 128), "bf16", 16, 128)
+    pool.set_decode_split(4)
+    table, lens = i32(torch, tables), i32(torch, lengths)
+    calls = []
+    for kind in (torch.bfloat16, torch.float32):
+        for seqs in (1, 3, 48):
+            q = torch.randn((seqs, 8, 128), device="cuda:0").to(kind)
+            calls.append((seqs, 1, lambda ws, q=q, n=seqs: pool.decode(q, table[:n], lens[:n], 1500, workspace=ws)))
+            for count in (5, 40):
+                q = torch.randn((seqs * count, 8, 128), device="cuda:0").to(kind)
+                counts = torch.minimum(lens[:seqs], lens.new_tensor(count))
+                at = (torch.arange(seqs, device="cuda:0", dtype=torch.int32) * count).contiguous()
+                out = torch.zeros_like(q)
+                calls.append((seqs, count, lambda ws, q=q, n=seqs, c=count, k=counts, at=at: pool.prefill(
+                    q, table[:n], (lens[:n] - k).contiguous(), k, at, c, out=torch.zeros_like(q), max_context_len=1500, workspace=ws)))
+    alone = []
+    for seqs, count, call in calls:
+        alone.append(call(pool.make_workspace(seqs, 8, 1500, max_query_count=count)))
+    shared = pool.make_workspace(48, 8, 1500, max_query_count=40)
+    for _ in range(2):
+        for i in list(range(len(calls))) + list(rng.permutation(len(calls))):
+            assert torch.equal(calls[i][2](shared), alone[i])
+            assert torch.equal(calls[i][2](None), alone[i])
+    pool.synchronize()
+    # too small a workspace, or one that no 16-byte load can read, is refused
+    need = pool.workspace_size(48, 8, 1500, 40)
+    with pytest.raises(il.AttentionError, match="workspace is too small"):
+        calls[5][2](torch.zeros(256, dtype=torch.uint8, device="cuda:0"))
+    with pytest.raises(il.AttentionError, match="workspace must be 16-byte aligned"):
+        calls[5][2](torch.zeros(need + 64, dtype=torch.uint8, device="cuda:0")[8:])
+    flat = torch.zeros(8 * 128 + 1, device="cuda:0", dtype=torch.bfloat16)
+    with pytest.raises(il.AttentionError, match="must be 16-byte aligned"):
+        pool.decode(flat[1:].view(1, 8, 128), table[:1], lens[:1], 1500)
+    none = torch.zeros((0, 8, 128), device="cuda:0", dtype=torch.bfloat16)
+    assert pool.decode(none, table[:0], lens[:0], 1500).shape == none.shape
+    assert pool.prefill(none, table[:1], lens[:1], lens[:1] * 0, lens[:1] * 0, 40, max_context_len=1500).shape == none.shape
+    pool.synchronize()
+    pool.close()
+
+
+@pytest.mark.parametrize("q_kind", ["bf16", "f32"])
+def test_prefill_of_many_rows_captured_and_side_by_side(torch, il, kv4, q_kind):
+    """The same bits eagerly, from two graphs replayed side by side, and on another stream."""
+    rng = np.random.default_rng(31)
+    lengths = np.array([900, 130, 333, 640])
+    tables, blocks = deal(rng, lengths, 16)
+    pool = filled_pool(torch, il, random_arena(kv4, rng, blocks, 16, 16, 64), "bf16", 16, 64)
+    pool.set_decode_split(8)
+    counts = np.array([130, 130, 1, 77])
+    args = (i32(torch, tables), i32(torch, lengths - counts), i32(torch, counts), i32(torch, [0, 130, 260, 261]), 130)
+    q = torch.randn((338, 32, 64), device="cuda:0").to(kind_of(torch, q_kind))
+
+    def call(out=None, stream=None):
+        return pool.prefill(q, *args, out=out, stream=stream, max_context_len=900)
+
+    first = call()
+    for _ in range(3):
+        assert torch.equal(call(), first)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    outs, graphs = [torch.zeros_like(q), torch.zeros_like(q)], []
+    torch.cuda.synchronize()
+    for out in outs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(out)
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+            elsewhere = call()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], first) and torch.equal(outs[1], first) and torch.equal(elsewhere, first)
+    back = call(stream=side)
+    torch.cuda.synchronize()
+    assert torch.equal(back, first)
     pool.synchronize()
     pool.close()
 
