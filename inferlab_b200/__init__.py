@@ -4,7 +4,8 @@ Drop-in for the reference's kernels/attention_cpu + paged KV cache:
   * run_attention: the worker's attention facade (worker/src/lib.rs:743-819)
     over the C entry inferlab_attention_forward, executed on the GPU;
   * CudaKvPool: the HBM block pool with append / gather / paged decode /
-    paged prefill kernels that follow the reference's block tables;
+    paged prefill kernels that follow the reference's block tables, with
+    elements of 32 or 16 bits or groups in 4, and a rotary append;
   * PageManager: the block ownership model (reference counts, prefixes,
     copy on write, eviction, InferlabPagedCacheStats) kept on the host.
 All compute is in libinferlab_attention_cuda.so (built by

@@ -1,7 +1,9 @@
-// kv4_rows.cuh - attention of many query rows per kv-head over a 4-bit pool
+// kv4_rows.cuh - attention of many fp32 query rows per kv-head over a 4-bit pool
 // (prompt chunks and prompts): the codes of a 64-token block are widened once
 // in shared memory for 64 query rows, instead of once per 8 columns in
-// registers (kv4_attention.cu, whose arithmetic this follows).
+// registers (kv4_attention.cu, whose arithmetic this follows, weights in two f16
+// parts). 16-bit queries take the tensor cores (kv4_prefill_tc.cuh), whose f16
+// keys and values would not do for an fp32 result.
 //
 // One CTA of four warps takes 64 rows (token-major, the heads of a token
 // together) of a (sequence, kv-head), a warp 16 of them. Per block: the four
@@ -13,9 +15,10 @@
 // 0 4 1 5 2 6 3 7, which the contraction of Q and K does not see and O undoes
 // when it is stored. The pairs (scale, zero - 8 scale) and (scale, zero) are
 // widened to fp32 beside them and applied to scores and weights.
-// Bound by the mma.sync rate (1024 multiply-adds a clock and SM): 32 mma per 16
-// rows, 16 tokens and 128 dims take 256 clocks of an SM's quarter, beside ~230
-// other instructions.
+// Bound by shared memory and latency: 16 rows, 16 tokens and 128 dims take 48 mma
+// (384 clocks of an SM's quarter), 16 ldmatrix and ~230 other instructions of the
+// three warps that a quarter holds. 64 fresh prompts of 128 tokens, 32 heads over
+// 8 kv-heads: 176 us, 470 in column tiles.
 #pragma once
 
 namespace ilb {
