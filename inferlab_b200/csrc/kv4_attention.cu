@@ -734,11 +734,15 @@ Kv4Plan plan_kv4(const InferlabCudaKvPool& p, std::uint32_t num_seqs, std::uint3
         plan.kind = tensor ? Kv4Plan::kTensor : Kv4Plan::kRows;
         plan.columns = static_cast<std::uint32_t>(row_tile);
         plan.column_tiles = static_cast<std::uint32_t>(row_tiles);
-        // Up to 4096 CTAs (nine waves of three an SM) if all contexts were
-        // max_context_len long: the lengths are the device's and most are shorter.
+        // Up to 1024 CTAs (3.5 waves of two an SM) if all contexts were
+        // max_context_len long; the lengths are the device's and most may be
+        // shorter, but each split costs a CTA's start and end and a merge. 592,
+        // 1024, 2048 and 4096 CTAs: 64 segments of 64 tokens on 1200 263, 263, 379
+        // and 380 us, 128 tokens on 120000 739, 754, 799 and 1011, 4 x 512 on zipf
+        // 8192 381, 274, 263 and 265.
         const std::uint64_t all = (max_context_len + kv4::kTileTokens - 1) / kv4::kTileTokens;
         std::uint64_t per = p.decode_blocks_per_split;
-        if (per == 0) per = std::max<std::uint64_t>(64, checked_mul(row_units, all, "4-bit attention batch is too large") / 4096);
+        if (per == 0) per = std::max<std::uint64_t>(64, checked_mul(row_units, all, "4-bit attention batch is too large") / 1024);
         if (row_units > kMaxSplitUnits) per = all;
         per = (std::max<std::uint64_t>(per, (all + kMaxSplits - 1) / kMaxSplits) + kBlockTiles - 1) / kBlockTiles * kBlockTiles;
         plan.tiles_per_split = static_cast<int>(per);

@@ -304,6 +304,27 @@ def test_append_rotary_rejects_what_the_row_type_cannot_hold(torch, il, shift):
             pool.close()
 
 
+@pytest.mark.parametrize("bits", [None, 4])
+def test_no_rows_and_rows_behind_the_last(torch, il, bits):
+    """Calls of no rows write nothing; so do padded rows among others, in the pool and in q_out."""
+    pool = il.CudaKvPool(0, 2, 6, 16, 2, 64, kv_bits=bits)
+    tables = i32(torch, [[1, 2], [3, 4]])
+    none = torch.zeros((0, 2, 64), device="cuda:0")
+    assert pool.append_rotary(none, none, none, None, i32(torch, []), i32(torch, []), tables).shape == none.shape
+    keys, values = pool.gather_rows(i32(torch, []), i32(torch, []), tables)
+    assert keys.shape == values.shape == none.shape
+    rows = torch.randn((5, 6, 64), device="cuda:0")
+    angles = torch.from_numpy(angles_of(32, 64)).to("cuda:0")
+    out = torch.full((5, 2, 64), 9.0, device="cuda:0")
+    pool.append_rotary(rows[:, :2], rows[:, 2:4], rows[:, 4:], angles, i32(torch, [0, -1, 1, -1, -1]), i32(torch, [17, 5, 31, -7, 1 << 30]), tables,
+                       q_out=out)
+    pool.synchronize()
+    assert [(out[r] == 9).all().item() for r in range(5)] == [False, True, False, True, True]
+    written = (pool.arena if bits else torch.stack([pool.key_arena, pool.value_arena], 1)).flatten(1).any(1)
+    assert written.nonzero().flatten().tolist() == [2, 4]
+    pool.close()
+
+
 def test_append_rotary_refusals(torch, il):
     pool = il.CudaKvPool(0, 2, 8, 16, 2, 64, kv_bits=4)
     rows = torch.randn((4, 8, 64), device="cuda:0")
