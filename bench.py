@@ -379,6 +379,13 @@ def compare(got, ref, rtol, atol=0.0, row_atol=0.0) -> dict:
             "elements": int(err.size)}
 
 
+def cpu_reference_built():
+    """Whether the reference's CPU kernel was built from its sources (oracle/Makefile)."""
+    from oracle import oracle
+
+    return oracle.ref_lib() is not None
+
+
 def cpu_baseline_decode(sample, bytes_per_step_sample, q_heads, dtype, seconds, what):
     """The reference CPU kernel (page gather + one inferlab_attention_forward
     per q-head, OnlineTiled tile 16) on a host sample of the timed workload,
@@ -450,7 +457,7 @@ def measure_decode(args, dist, world, rank, device, peaks, peak_kind, workload):
     # append new rows to the pool.
     sample = None
     want_cpu = rank == 0 and world == 1 and not args.no_cpu_baseline
-    if want_cpu:
+    if want_cpu and cpu_reference_built():
         from inferlab_b200 import workloads as wl
 
         seqs = (list(range(num_seqs)) if workload == "decode_fp32"
@@ -504,6 +511,8 @@ def measure_decode(args, dist, world, rank, device, peaks, peak_kind, workload):
                 + ", ".join(str(int(c)) for c in sample[3]) + ")")
         line["cpu_baseline"] = cpu_baseline_decode(sample, sample_bytes, batch.q_heads,
                                                    batch.pool.dtype, args.cpu_seconds, what)
+    elif want_cpu:
+        line["cpu_baseline"] = {"unavailable": "oracle/_ref/libref.so is not built"}
     return line
 
 
@@ -685,8 +694,10 @@ def measure_prefill(args, dist, world, rank, device, peaks, peak_kind):
                              tflops=achieved),
     }
     if rank == 0 and world == 1 and not args.no_cpu_baseline:
-        line["cpu_baseline"] = cpu_baseline_prefill(pool, batch, out.cpu().numpy(),
-                                                    min(args.cpu_seconds, 8.0))
+        line["cpu_baseline"] = (cpu_baseline_prefill(pool, batch, out.cpu().numpy(),
+                                                     min(args.cpu_seconds, 8.0))
+                                if cpu_reference_built() else
+                                {"unavailable": "oracle/_ref/libref.so is not built"})
     pool.close()
     return line
 
