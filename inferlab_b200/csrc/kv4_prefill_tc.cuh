@@ -149,14 +149,20 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
         tc::tmem_alloc(&tmem_at, L::kTmem);
         tc::tmem_relinquish();
     }
+    // A thread's row, and where it is in queries and out. A warp's 16 rows of a
+    // copy are its own half of the 32 it owns, so that their places are known
+    // without a division each.
+    const int row = threadIdx.x % kTcRows, half = threadIdx.x / kTcRows;
+    const std::uint32_t row_at = static_cast<std::uint32_t>(row_of(min(row, live - 1)) - static_cast<std::size_t>(offset) * p.q_heads);
+    auto copied_row = [&](int i, int lanes) { return 16 * half + i * (32 / lanes) + lane / lanes; };  // within the warp's 32
+    auto place_of = [&](int r) { return static_cast<std::size_t>(offset) * p.q_heads + __shfl_sync(0xffffffffu, row_at, r); };
     // The queries come as they are to where they go; 16-byte chunks of 64 dims of
     // a row, swizzled.
-    const int row = threadIdx.x % kTcRows, half = threadIdx.x / kTcRows;
     auto query_at = [&](int r, int unit) { return L::kQ + (unit / 8) * L::kQGroup + r * 128 + ((unit % 8 ^ (r & 7)) << 4); };
 #pragma unroll
-    for (int i = 0; i < kTcRows * kUnits / kTcThreads; ++i) {
-        const int r = (threadIdx.x + i * kTcThreads) / kUnits, unit = threadIdx.x % kUnits;
-        cp_async16(at + query_at(r, unit), static_cast<const QT*>(p.queries) + row_of(min(r, live - 1)) * D + unit * 8);
+    for (int i = 0; i < kUnits / 2; ++i) {
+        const int r = copied_row(i, kUnits), unit = lane % kUnits;
+        cp_async16(at + query_at(32 * (warp & 3) + r, unit), static_cast<const QT*>(p.queries) + place_of(r) * D + unit * 8);
     }
     cp_async_commit();
     // Warp w brings the keys of tile w of a block, warp 4 + w the values of the
@@ -471,11 +477,14 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
             }
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < live * D / 4; i += kTcThreads) {
-            const int r = i / (D / 4);
-            const float4 x = *staged(r, i % (D / 4));
-            if (whole) store_row4(static_cast<QT*>(p.out) + row_of(r) * D + 4 * i % D, x);
-            else store_row4(part + 4 * i, x);
+#pragma unroll 4
+        for (int i = 0; i < D / 8; ++i) {
+            const int own = copied_row(i, D / 4), r = 32 * (warp & 3) + own, chunk = lane % (D / 4);
+            const std::size_t place = place_of(own);
+            if (r >= live) continue;
+            const float4 x = *staged(r, chunk);
+            if (whole) store_row4(static_cast<QT*>(p.out) + place * D + 4 * chunk, x);
+            else store_row4(part + r * D + 4 * chunk, x);
         }
     }
     if (threadIdx.x == 0) {
