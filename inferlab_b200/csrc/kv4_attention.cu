@@ -78,6 +78,8 @@ struct Kv4Params {
     std::uint32_t max_count;           // query tokens a sequence may have
     long long total_queries;
     std::uint32_t column_tiles, max_splits;
+    std::uint32_t per_seq;             // kv-heads x column (or row) tiles
+    bool by_length;                    // longest contexts first
     int tiles_per_split;
     float scale_log2;
     std::uint32_t* ws_count;  // [unit]
@@ -134,6 +136,52 @@ __device__ __forceinline__ void load_pairs(const unsigned char* at, float2 (&pai
 // t, r = 2t + 1 token 7 - t. Rows 2t of all t (what four lanes read of V at
 // once) and rows r of neighbouring r (K) then fall on different banks.
 __device__ __forceinline__ int slot_of_row(int r) { return r & 1 ? 7 - (r >> 1) : r >> 1; }
+
+// What a CTA works on: a split of a sequence's keys, and which of its kv-heads
+// and tiles. Up to 32 sequences come in the order of their lengths, which the
+// device knows, all of a long one's CTAs before a shorter one's: the short ones
+// fill what the long ones leave (4 chunks of 512 tokens on contexts of 32 to 8192:
+// 268 -> 215 us; a decode of 32 contexts: 41 -> 37.5). More sequences, or contexts
+// in one piece, come with their last splits first, which only long contexts have;
+// row tiles (kRowTiles: rest = tile x kv-heads + kv-head) then before the
+// sequences, those with the most keys first (8 prompts of 1 to 1024 tokens: 66
+// us, 82 sequence by sequence).
+struct Work {
+    std::uint32_t seq, split, rest;
+};
+template <bool kRowTiles>
+__device__ __forceinline__ Work work_of(const Kv4Params& p) {
+    Work w;
+    if (!p.by_length) {
+        const std::uint32_t units = p.num_seqs * p.per_seq, unit = blockIdx.x % units;
+        w.split = p.max_splits - 1 - blockIdx.x / units;
+        if constexpr (kRowTiles) {
+            const std::uint32_t pairs = p.num_seqs * p.kv_heads, pair = unit % pairs;
+            w.seq = pair / p.kv_heads;
+            w.rest = unit / pairs * p.kv_heads + pair % p.kv_heads;
+        } else {
+            w.seq = unit / p.per_seq;
+            w.rest = unit % p.per_seq;
+        }
+        return w;
+    }
+    const int lane = threadIdx.x & 31;
+    std::uint32_t length = 0, rank = 0;  // 1 more than the context; 0 for no sequence
+    if (lane < static_cast<int>(p.num_seqs)) {
+        length = 1 + (p.context_lens != nullptr ? static_cast<std::uint32_t>(p.context_lens[lane])
+                                                : static_cast<std::uint32_t>(p.starts[lane]) + static_cast<std::uint32_t>(p.counts[lane]));
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const std::uint32_t other = __shfl_sync(0xffffffffu, length, i);
+        rank += other > length || (other == length && i < lane);
+    }
+    const std::uint32_t each = p.per_seq * p.max_splits, at = blockIdx.x % each;
+    w.seq = __ffs(__ballot_sync(0xffffffffu, rank == blockIdx.x / each)) - 1;
+    w.split = at / p.per_seq;
+    w.rest = at % p.per_seq;
+    return w;
+}
 
 // Whether this CTA is the last of `splits` to come here; what the others wrote
 // before is then visible. Returns the counter to zero.
@@ -225,11 +273,10 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t4 = lane & 3;
-    const std::uint32_t split = blockIdx.x % p.max_splits;
-    const std::uint32_t unit = blockIdx.x / p.max_splits;
-    const std::uint32_t column_tile = unit % p.column_tiles;
-    const std::uint32_t kv_head = unit / p.column_tiles % p.kv_heads;
-    const std::uint32_t seq = unit / p.column_tiles / p.kv_heads;
+    const Work work = work_of<false>(p);
+    const std::uint32_t seq = work.seq, split = work.split;
+    const std::uint32_t column_tile = work.rest % p.column_tiles, kv_head = work.rest / p.column_tiles;
+    const std::uint32_t unit = seq * p.per_seq + work.rest;
     const int b0 = static_cast<int>(split) * p.tiles_per_split;
 
     // Block ids of the split's first tiles are asked for at once, beside the
@@ -738,8 +785,8 @@ Kv4Plan plan_kv4(const InferlabCudaKvPool& p, std::uint32_t num_seqs, std::uint3
         // max_context_len long; the lengths are the device's and most may be
         // shorter, but each split costs a CTA's start and end and a merge. 592,
         // 1024, 2048 and 4096 CTAs: 64 segments of 64 tokens on 1200 263, 263, 379
-        // and 380 us, 128 tokens on 120000 739, 754, 799 and 1011, 4 x 512 on zipf
-        // 8192 381, 274, 263 and 265.
+        // and 380 us, 128 tokens on 120000 739, 715, 799 and 1011, 4 x 512 on zipf
+        // 8192 307, 215, 227 and 252.
         const std::uint64_t all = (max_context_len + kv4::kTileTokens - 1) / kv4::kTileTokens;
         std::uint64_t per = p.decode_blocks_per_split;
         if (per == 0) per = std::max<std::uint64_t>(64, checked_mul(row_units, all, "4-bit attention batch is too large") / 1024);
@@ -829,13 +876,15 @@ void run_kv4(InferlabCudaKvPool& p, Kv4Params k, std::uint32_t query_dtype, std:
     k.max_context = static_cast<int>(std::min<long long>(max_context_len, static_cast<long long>(k.max_blocks) * p.block_tokens));
     k.column_tiles = plan.column_tiles;
     k.max_splits = plan.max_splits;
+    k.per_seq = p.kv_heads * plan.column_tiles;
+    k.by_length = num_seqs > 1 && num_seqs <= 32 && plan.max_splits > 1;
     k.tiles_per_split = plan.tiles_per_split;
     k.scale_log2 = kLog2e / std::sqrt(static_cast<float>(p.head_dim));
     k.ws_count = static_cast<std::uint32_t*>(workspace);
     k.ws_part = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + plan.counter_bytes);
     k.error_word = p.error_word;
     k.num_seqs = num_seqs;
-    const unsigned grid = static_cast<unsigned>(num_seqs * p.kv_heads * plan.column_tiles * plan.max_splits);
+    const unsigned grid = num_seqs * k.per_seq * plan.max_splits;
     auto launch = [&](auto row_type, auto query_type) {
         using RowT = decltype(row_type);
         using QT = decltype(query_type);

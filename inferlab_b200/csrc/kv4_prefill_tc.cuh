@@ -104,12 +104,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
     __shared__ int abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    // Row tiles of all segments and heads, those with the most keys first, each
-    // cut into splits of its keys.
-    const std::uint32_t pairs = p.num_seqs * p.kv_heads;
-    const std::uint32_t split = blockIdx.x % p.max_splits, work = blockIdx.x / p.max_splits;
-    const std::uint32_t row_tile = p.column_tiles - 1 - work / pairs;
-    const std::uint32_t kv_head = work % pairs % p.kv_heads, seq = work % pairs / p.kv_heads;
+    // The row tiles with the most keys come first.
+    const Work place = work_of<true>(p);
+    const std::uint32_t seq = place.seq, split = place.split, work = seq * p.per_seq + place.rest;
+    const std::uint32_t row_tile = p.column_tiles - 1 - place.rest / p.kv_heads, kv_head = place.rest % p.kv_heads;
     const bool first_split = split == 0;
     const std::int32_t s_ = p.starts[seq], c_ = p.counts[seq], o_ = p.offsets[seq];
     const std::uint32_t start = static_cast<std::uint32_t>(s_), count = static_cast<std::uint32_t>(c_),
