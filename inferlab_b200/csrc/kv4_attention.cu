@@ -138,11 +138,11 @@ __device__ __forceinline__ void load_pairs(const unsigned char* at, float2 (&pai
 __device__ __forceinline__ int slot_of_row(int r) { return r & 1 ? 7 - (r >> 1) : r >> 1; }
 
 // What a CTA works on: a split of a sequence's keys, and which of its kv-heads
-// and tiles. Up to 32 sequences come in the order of their lengths, which the
-// device knows, all of a long one's CTAs before a shorter one's: the short ones
-// fill what the long ones leave (4 chunks of 512 tokens on contexts of 32 to 8192:
-// 268 -> 215 us; a decode of 32 contexts: 41 -> 37.5). More sequences, or contexts
-// in one piece, come with their last splits first, which only long contexts have;
+// and tiles. By length (the host says for which batches), sequences come in the
+// order of their contexts, which the device knows, all of a long one's CTAs before
+// a shorter one's: the short ones fill what the long ones leave (4 chunks of 512
+// tokens on contexts of 32 to 8192: 268 -> 215 us; a decode of 32 contexts: 41 ->
+// 37.5). Otherwise the last splits come first, which only long contexts have;
 // row tiles (kRowTiles: rest = tile x kv-heads + kv-head) then before the
 // sequences, those with the most keys first (8 prompts of 1 to 1024 tokens: 66
 // us, 82 sequence by sequence).
@@ -166,18 +166,32 @@ __device__ __forceinline__ Work work_of(const Kv4Params& p) {
         return w;
     }
     const int lane = threadIdx.x & 31;
-    std::uint32_t length = 0, rank = 0;  // 1 more than the context; 0 for no sequence
-    if (lane < static_cast<int>(p.num_seqs)) {
-        length = 1 + (p.context_lens != nullptr ? static_cast<std::uint32_t>(p.context_lens[lane])
-                                                : static_cast<std::uint32_t>(p.starts[lane]) + static_cast<std::uint32_t>(p.counts[lane]));
-    }
+    auto length_of = [&](std::uint32_t seq) -> std::uint32_t {  // 1 more than the context; 0 for no sequence
+        if (seq >= p.num_seqs) return 0;
+        return 1 + (p.context_lens != nullptr ? static_cast<std::uint32_t>(p.context_lens[seq])
+                                              : static_cast<std::uint32_t>(p.starts[seq]) + static_cast<std::uint32_t>(p.counts[seq]));
+    };
+    // Ranks of sequences lane and 32 + lane; of equal ones the first comes first.
+    const std::uint32_t low = length_of(lane), high = length_of(32 + lane);
+    std::uint32_t low_rank = 0, high_rank = 0;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-        const std::uint32_t other = __shfl_sync(0xffffffffu, length, i);
-        rank += other > length || (other == length && i < lane);
+        const std::uint32_t other = __shfl_sync(0xffffffffu, low, i);
+        low_rank += other > low || (other == low && i < lane);
+        high_rank += other >= high;
+    }
+    if (p.num_seqs > 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const std::uint32_t other = __shfl_sync(0xffffffffu, high, i);
+            low_rank += other > low;
+            high_rank += other > high || (other == high && i < lane);
+        }
     }
     const std::uint32_t each = p.per_seq * p.max_splits, at = blockIdx.x % each;
-    w.seq = __ffs(__ballot_sync(0xffffffffu, rank == blockIdx.x / each)) - 1;
+    const std::uint32_t rank = blockIdx.x / each;
+    const std::uint32_t in_low = __ballot_sync(0xffffffffu, low_rank == rank), in_high = __ballot_sync(0xffffffffu, high_rank == rank);
+    w.seq = in_low != 0 ? __ffs(in_low) - 1 : 31 + __ffs(in_high);
     w.split = at / p.per_seq;
     w.rest = at % p.per_seq;
     return w;
@@ -877,7 +891,13 @@ void run_kv4(InferlabCudaKvPool& p, Kv4Params k, std::uint32_t query_dtype, std:
     k.column_tiles = plan.column_tiles;
     k.max_splits = plan.max_splits;
     k.per_seq = p.kv_heads * plan.column_tiles;
-    k.by_length = num_seqs > 1 && num_seqs <= 32 && plan.max_splits > 1;
+    // Split contexts of more than 32 sequences even out without (64 x 4096..32768:
+    // 279 us, 312 by length), whole ones only where the CTAs are not all resident
+    // at once (64 x 5 drafted tokens: 78 us, 70 by length; row tiles have an order
+    // of their own).
+    k.by_length = num_seqs > 1 && (plan.max_splits > 1 ? num_seqs <= 32
+                                                       : plan.kind == Kv4Plan::kColumns && num_seqs <= 64 &&
+                                                             static_cast<std::uint64_t>(num_seqs) * k.per_seq > 592);
     k.tiles_per_split = plan.tiles_per_split;
     k.scale_log2 = kLog2e / std::sqrt(static_cast<float>(p.head_dim));
     k.ws_count = static_cast<std::uint32_t*>(workspace);

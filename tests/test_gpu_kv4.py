@@ -546,6 +546,34 @@ def test_prefill_of_many_rows_reports_what_it_cannot_read(torch, kv4, il, q_kind
     pool.close()
 
 
+@pytest.mark.parametrize("seqs", [2, 31, 32, 33, 63, 64, 65])
+@pytest.mark.parametrize("split", [0, 2])
+def test_batches_in_any_order_of_lengths(torch, kv4, il, seqs, split):
+    """Ascending, equal and mixed lengths, empty sequences among them; more CTAs than run at once, whole and split."""
+    rng = np.random.default_rng(seqs)
+    for lengths in (np.arange(seqs) + 6, np.full(seqs, 20), rng.integers(0, 90, seqs)):
+        counts = np.minimum(lengths, 5)
+        check_attention(torch, kv4, il, "bf16", "bf16", 4, 32, 64, 16, lengths - counts, counts, split=split, poison=False)
+        check_attention(torch, kv4, il, "bf16", "f32", 4, 32, 64, 16, lengths - 1, np.ones_like(lengths), decode=True, split=split, poison=False)
+    # a bad length among them: its rows are zero, the others' as before
+    tables, blocks = deal(rng, np.full(seqs, 40), 16)
+    pool = filled_pool(torch, il, random_arena(kv4, rng, blocks, 4, 16, 64), "bf16", 16, 64)
+    pool.set_decode_split(split)
+    q = torch.randn((seqs, 32, 64), device="cuda:0")
+    good = host(pool.decode(q, i32(torch, tables), i32(torch, np.full(seqs, 40)), 40))
+    pool.synchronize()
+    for bad in (-1, -2, -(1 << 31), 41, (1 << 31) - 1):
+        lens = np.full(seqs, 40)
+        lens[seqs // 2] = bad
+        out = host(pool.decode(q, i32(torch, tables), i32(torch, lens), 40))
+        with pytest.raises(il.AttentionError, match="^paged KV context length is invalid$"):
+            pool.synchronize()
+        assert not out[seqs // 2].any()
+        rest = np.arange(seqs) != seqs // 2
+        assert np.array_equal(out[rest], good[rest])
+    pool.close()
+
+
 def test_decode_long_flat_and_sharp(torch, kv4, il):
     """20,000 keys: queries of zero weigh all alike, large ones pick a few."""
     rng = np.random.default_rng(8)
