@@ -23,13 +23,13 @@
 // tokens on contexts up to 8192.
 // Two CTAs an SM: one's softmax runs beside the other's MMAs (half of the 512
 // TMEM columns and 110 KB of shared memory each).
-// Bound by instruction issue (54% of the slots, 16% of the tensor pipe): a block
+// Bound by instruction issue (54% of the slots, 18% of the tensor pipe): a block
 // costs its eight warps ~700 instructions each, 250 of them the widening, and
 // 4300 clocks, of which the other CTA uses the gaps. 4 chunks of 512 tokens on
-// contexts up to 8192, 32 heads over 8 kv-heads: 264 us, 302 TFLOP/s. A CTA's
+// contexts up to 8192, 32 heads over 8 kv-heads: 212 us, 376 TFLOP/s. A CTA's
 // queries, first keys and outputs cost as much as four blocks, so short prompts
-// come off worse (8 of 1 to 1024 tokens, 16 heads: 68 us). A second S in TMEM,
-// issued a block ahead, changed nothing (264 and 70 us).
+// come off worse (8 of 1 to 1024 tokens, 16 heads: 63 us). A second S in TMEM,
+// issued a block ahead, changed nothing.
 #pragma once
 
 #include "tc_common.cuh"
