@@ -325,7 +325,10 @@ int inferlab_cuda_pool_set_decode_split(InferlabCudaKvPool* pool, uint32_t block
 
 /*
  * Zeroes the counters at the front of a decode workspace. Needed once per
- * workspace before its first use; the decode kernel leaves them at zero.
+ * workspace before its first use; the decode kernel leaves them at zero. In
+ * inferlab_cuda_paged_decode they take num_seqs * kv_heads words, rounded up to
+ * 256 bytes, and partials follow: before a batch of more sequences than the
+ * last ones on the same workspace, zero it again.
  */
 int inferlab_cuda_paged_decode_workspace_init(void* workspace, size_t workspace_bytes,
                                               void* stream, char* error, size_t error_capacity);

@@ -63,6 +63,9 @@ def _require(tensor: torch.Tensor, name: str, dtype, device: int) -> torch.Tenso
     return tensor
 
 
+_COUNTER_FRONT = 65536  # bytes of split counters that a pool's own workspace starts with
+
+
 def _expect(tensor, name: str, dtype, device: int) -> int:
     """_require for the per-token calls, whose time is the host's: one pass over what a good
     tensor satisfies, the messages only for others. Returns the address."""
@@ -415,16 +418,26 @@ class CudaKvPool:
         stream run in order and may share it, decodes on two streams would race
         on its split counters and partials. A workspace outgrown on a stream is
         replaced only after that stream has finished with it (record_stream)."""
-        need = self.workspace_size(num_seqs, q_heads, max_context_len)
+        # A batch's split counters lie in front of its partials and take as much
+        # as it has sequences. Behind the same front all batches' partials begin
+        # at one place, and no batch finds another's where its counters are.
+        counters = (num_seqs * self.kv_heads * 4 + 255) // 256 * 256
+        front = max(_COUNTER_FRONT, counters)
+        need = self.workspace_size(num_seqs, q_heads, max_context_len) - counters + front
         key = _stream_handle(self.device, stream).value
+        if front != _COUNTER_FRONT:
+            key = (key, front)
         ws = self._workspaces.get(key)
         if ws is None or ws.numel() < need:
+            used = stream if stream is not None else torch.cuda.current_stream(self.device)
             if ws is not None:
-                ws.record_stream(stream if stream is not None
-                                 else torch.cuda.current_stream(self.device))
-            ws = self.make_workspace(num_seqs, q_heads, max_context_len, stream)
+                ws.record_stream(used)
+            ws = torch.empty(need, dtype=torch.uint8, device=f"cuda:{self.device}")
+            error = _lib.error_buffer()
+            _check(self._lib.inferlab_cuda_paged_decode_workspace_init(
+                _vp(ws), need, _stream_handle(self.device, stream), error, len(error)), error)
             self._workspaces[key] = ws
-        return ws
+        return ws[front - counters:]
 
     def decode(self, queries: torch.Tensor, block_tables: torch.Tensor,
                context_lens: torch.Tensor, max_context_len: int | None = None,
