@@ -132,6 +132,15 @@ __device__ __forceinline__ void load_pairs(const unsigned char* at, float2 (&pai
     pairs[0] = __half22float2(*reinterpret_cast<const __half2*>(&raw.x));
     pairs[1] = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
 }
+// What m may be for a score and the log2 of what its weight is multiplied by:
+// `kHeadroom` below their sum, rounded up and never above the score. From 2^24
+// on, fp32 scores are so far apart that the headroom itself is rounded: rounded
+// down, m would let 2^(score - m) times that factor leave f16's range (scores
+// around 2^28); rounded up it may be lost, and the weight is then 1 and what is
+// kept as f16 the factor itself.
+__device__ __forceinline__ float score_with_room(float score, float factor_log2) {
+    return __fadd_ru(score, fminf(factor_log2 - kHeadroom, 0.0f));
+}
 // Token slot (0..7) that sits in row r of an 8-token mma half: r = 2t is token
 // t, r = 2t + 1 token 7 - t. Rows 2t of all t (what four lanes read of V at
 // once) and rows r of neighbouring r (K) then fall on different banks.
@@ -573,7 +582,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) kv4_attention_kernel(const Kv4
                         float scale = 9.5367431640625e-07f;  // 2^-20
 #pragma unroll
                         for (int k = 0; k < kPairs; ++k) scale = fmaxf(scale, vp[u][h][k].x);
-                        top = fmaxf(top, s[u][2 * h + c] + (__log2f(scale) - kHeadroom));
+                        top = fmaxf(top, score_with_room(s[u][2 * h + c], __log2f(scale)));
                     }
                 }
                 if constexpr (kFour) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));  // the column's twin

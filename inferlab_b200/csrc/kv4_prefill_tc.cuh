@@ -224,8 +224,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
             if (!seen) pair[k] = make_float2(0.0f, 0.0f);  // slots behind the last key may hold anything
             most = fmax3(most, fabsf(fmaf(-8.0f, pair[k].x, pair[k].y)), fabsf(fmaf(7.0f, pair[k].x, pair[k].y)));
         }
-        // 2^e: the largest value becomes 2^14 to 2^15, one below 2^-20 less.
-        const std::uint32_t exponent = max(107u, __float_as_uint(most) >> 23);
+        // 2^e: the largest value becomes 2^14 to 2^15, one below 2^-10 less (the
+        // f16 pairs are multiples of 2^-24, so nothing is lost): where large
+        // scores leave m no room a weight is kept as 2^e, which f16 must hold.
+        const std::uint32_t exponent = max(117u, __float_as_uint(most) >> 23);
         const float down = __uint_as_float((268u - exponent) << 23);
         __half2 scale[kGroups], zero[kGroups];
 #pragma unroll
@@ -399,11 +401,11 @@ __global__ void __launch_bounds__(kTcThreads, 2) kv4_prefill_tc_kernel(const Kv4
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float2 unit = *reinterpret_cast<const float2*>(units + 2 * i);
-                top = fmax3(top, __fadd_rn(s[i].x, lg2(unit.x)), __fadd_rn(s[i].y, lg2(unit.y)));
+                top = fmax3(top, score_with_room(s[i].x, lg2(unit.x)), score_with_room(s[i].y, lg2(unit.y)));
             }
             tops[threadIdx.x] = top;
             __syncthreads();
-            const float next = fmaxf(m, fmaxf(tops[row], tops[row + kTcRows]) - kHeadroom), alpha = ex2_ftz(m - next);
+            const float next = fmaxf(m, fmaxf(tops[row], tops[row + kTcRows])), alpha = ex2_ftz(m - next);
             m = next;
             l2 = kv4::mul2(l2, make_float2(alpha, alpha));
             if (b > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {

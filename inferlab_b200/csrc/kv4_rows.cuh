@@ -335,8 +335,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) kv4_rows_kernel(const Kv4Pa
                         for (int k = 0; k < kGroups; ++k) {
                             scale = make_float2(fmaxf(scale.x, vs[h][k].x), fmaxf(scale.y, vs[h][k].y));
                         }
-                        top = fmaxf(top, s[h][r].x + (__log2f(scale.x) - kHeadroom));
-                        top = fmaxf(top, s[h][r].y + (__log2f(scale.y) - kHeadroom));
+                        top = fmaxf(top, score_with_room(s[h][r].x, __log2f(scale.x)));
+                        top = fmaxf(top, score_with_room(s[h][r].y, __log2f(scale.y)));
                     }
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
