@@ -515,6 +515,27 @@ int inferlab_cuda_paged_prefill(InferlabCudaKvPool* pool, const void* queries, u
 size_t inferlab_cuda_kv4_workspace_size(const InferlabCudaKvPool* pool, uint32_t num_seqs,
                                         uint32_t q_heads, uint32_t max_query_count,
                                         uint32_t max_context_len);
+
+/*
+ * What a call of this shape launches, for sizing a workspace before there is a
+ * pool and for tests; needs no device. max_query_count 1: _kv4_decode.
+ * tiles_per_split: inferlab_cuda_pool_set_decode_split's value, 0 for the
+ * planner's choice (which keeps a batch of several sequences to 32768 CTAs, or
+ * one per sequence, kv-head and tile of rows where those are more).
+ */
+typedef struct InferlabCudaKv4Plan {
+    uint32_t kernel;             /* 0: tiles of 4 or 8 rows; 1: of 64 rows (fp32 queries); 2: of 128 rows (16-bit) */
+    uint32_t tile_rows;          /* query rows (tokens x heads of a kv-head) a CTA works on */
+    uint32_t max_splits;         /* CTAs a context of max_context_len is split across */
+    uint32_t reserved;
+    uint64_t tokens_per_split;
+    uint64_t ctas;
+    uint64_t workspace_bytes;    /* for this type of query */
+} InferlabCudaKv4Plan;
+int inferlab_cuda_kv4_plan(uint32_t kv_heads, uint32_t head_dim, uint32_t num_seqs, uint32_t q_heads,
+                           uint32_t query_dtype, uint32_t max_query_count, uint32_t max_context_len,
+                           uint32_t tiles_per_split, InferlabCudaKv4Plan* plan, char* error,
+                           size_t error_capacity);
 int inferlab_cuda_kv4_decode(InferlabCudaKvPool* pool, const void* queries, uint32_t query_dtype,
                              const int32_t* block_tables, uint32_t max_blocks_per_seq,
                              const int32_t* context_lens, uint32_t num_seqs, uint32_t q_heads,

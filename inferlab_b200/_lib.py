@@ -93,6 +93,20 @@ class InferlabCudaRotaryAppend(ctypes.Structure):
     ]
 
 
+class InferlabCudaKv4Plan(ctypes.Structure):
+    """What an attention call over a 4-bit pool launches (inferlab_cuda_kv4_plan)."""
+
+    _fields_ = [
+        ("kernel", ctypes.c_uint32),
+        ("tile_rows", ctypes.c_uint32),
+        ("max_splits", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+        ("tokens_per_split", ctypes.c_uint64),
+        ("ctas", ctypes.c_uint64),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
 class InferlabPagedCacheStats(ctypes.Structure):
     """worker/cpp/inferlab_runtime.h:7-31."""
 
@@ -149,6 +163,8 @@ SIGNATURES = {
         c_vp, c_err, c_sz]),
     "inferlab_cuda_kv4_workspace_size": (c_sz, [
         c_vp, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32]),
+    "inferlab_cuda_kv4_plan": (ctypes.c_int, [ctypes.c_uint32] * 8 + [
+        ctypes.POINTER(InferlabCudaKv4Plan), c_err, c_sz]),
     "inferlab_cuda_kv4_decode": (ctypes.c_int, [
         c_vp, c_vp, ctypes.c_uint32, c_vp, ctypes.c_uint32, c_vp, ctypes.c_uint32,
         ctypes.c_uint32, ctypes.c_uint32, c_vp, c_vp, c_sz, c_vp, c_err, c_sz]),

@@ -60,6 +60,7 @@ constexpr std::uint32_t kMaxSplits = 256;
 // region is the same for all batches. More units than this fill the GPU many
 // times over and are not split.
 constexpr std::uint32_t kMaxSplitUnits = 16384;
+constexpr std::uint32_t kMaxSplitCtas = 32768;  // of split batches, where the planner chooses
 
 struct Kv4Params {
     const unsigned char* arena;
@@ -846,6 +847,14 @@ Kv4Plan plan_kv4(const InferlabCudaKvPool& p, std::uint32_t num_seqs, std::uint3
             // even that out themselves.
             per_split = std::max<std::uint64_t>(total / 1184, units >= 296 ? 128 : 16);
             per_split = std::min<std::uint64_t>(per_split, 256 * std::max<std::uint64_t>(1, column_tiles / 4));
+            // But not more than kMaxSplitCtas, most of which find no keys where
+            // the bound is one long context's: 512 sequences x 8 kv-heads of 1000
+            // tokens, one of 131072, in 4096 x 8, 16, 32 CTAs 264, 295, 432 us;
+            // 2048 of 300 tokens in 16384 x 2, 8, 32 328, 532, 1354 us (one of
+            // 131072 among them 611, 562, 1398) and 69 MB, 277 MB, 1.1 GB of
+            // partials; 1024 of 500, one of 32768, in 8192 x 2, 4, 8 225, 244, 313.
+            const std::uint64_t most = std::max<std::uint64_t>(1, kMaxSplitCtas / units);
+            per_split = std::max<std::uint64_t>(per_split, (tiles + most - 1) / most);
         }
         const std::uint64_t splits = (tiles + per_split - 1) / per_split;
         per_split = (tiles + splits - 1) / splits;
@@ -973,6 +982,38 @@ extern "C" std::size_t inferlab_cuda_kv4_workspace_size(const InferlabCudaKvPool
     } catch (...) {
         return 0;  // the call itself reports why
     }
+}
+
+extern "C" int inferlab_cuda_kv4_plan(std::uint32_t kv_heads, std::uint32_t head_dim,
+                                      std::uint32_t num_seqs, std::uint32_t q_heads,
+                                      std::uint32_t query_dtype, std::uint32_t max_query_count,
+                                      std::uint32_t max_context_len, std::uint32_t tiles_per_split,
+                                      InferlabCudaKv4Plan* plan, char* error,
+                                      std::size_t error_capacity) {
+    return ilb::protect(error, error_capacity, [&] {
+        if (plan == nullptr) throw std::runtime_error("4-bit attention plan output pointer is null");
+        *plan = InferlabCudaKv4Plan{};
+        if (kv_heads == 0 || q_heads == 0 || q_heads % kv_heads != 0) {
+            throw std::runtime_error("4-bit attention q_heads must be a positive multiple of kv_heads");
+        }
+        if (head_dim != 64 && head_dim != 128) throw std::runtime_error("4-bit paged KV head_dim must be 64 or 128");
+        if (num_seqs == 0 || max_query_count == 0 || max_context_len == 0 || max_context_len > 0x7FFFFF00u) {
+            throw std::runtime_error("4-bit attention bounds must be positive");
+        }
+        if (query_dtype > ilb::kBf16) throw std::runtime_error("4-bit attention query dtype must be FP32 or the pool's row type");
+        if (tiles_per_split > 1024) throw std::runtime_error("paged decode split length must be at most 1024 blocks");
+        InferlabCudaKvPool shape;
+        shape.kv_heads = kv_heads;
+        shape.head_dim = head_dim;
+        shape.decode_blocks_per_split = tiles_per_split;
+        const auto p = ilb::plan_kv4(shape, num_seqs, q_heads, max_query_count, max_context_len, query_dtype);
+        plan->kernel = p.kind == ilb::Kv4Plan::kColumns ? 0 : p.kind == ilb::Kv4Plan::kRows ? 1 : 2;
+        plan->tile_rows = p.columns;
+        plan->max_splits = p.max_splits;
+        plan->tokens_per_split = static_cast<std::uint64_t>(p.tiles_per_split) * ilb::kv4::kTileTokens;
+        plan->ctas = static_cast<std::uint64_t>(num_seqs) * kv_heads * p.column_tiles * p.max_splits;
+        plan->workspace_bytes = p.counter_bytes + p.part_bytes;
+    });
 }
 
 extern "C" int inferlab_cuda_kv4_decode(InferlabCudaKvPool* pool, const void* queries,
