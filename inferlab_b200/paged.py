@@ -117,7 +117,8 @@ class CudaKvPool:
         self.row_bytes = info.block_bytes // info.block_tokens * (1 if kv_bits == 4 else 2)
         self._key_ptr = info.key_arena
         self._value_ptr = info.value_arena
-        self._workspaces: dict = {}
+        self._workspaces: dict = {}  # by stream
+        self._fitting: dict = {}  # (stream, batch shape) -> the part of a workspace that fits it
         self._views: dict = {}  # weak: a view keeps the pool, not the pool its views
         self._kv4_workspaces: dict = {}  # (stream, batch shape) -> a workspace that fits it
 
@@ -409,35 +410,50 @@ class CudaKvPool:
         blocks (0: the planner chooses, the default). A tuning and test knob
         (inferlab_cuda_pool_set_decode_split)."""
         self._kv4_workspaces.clear()
+        self._fitting.clear()
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_pool_set_decode_split(
             self._handle, int(blocks_per_split), error, len(error)), error)
 
     def _cached_workspace(self, num_seqs, q_heads, max_context_len, stream):
-        """The pool's own decode workspace, kept per stream: decodes on one
+        """The pool's own decode workspace, one per stream: decodes on one
         stream run in order and may share it, decodes on two streams would race
-        on its split counters and partials. A workspace outgrown on a stream is
-        replaced only after that stream has finished with it (record_stream)."""
+        on its split counters and partials. Returned is the part of it that this
+        batch shape uses."""
+        raw = _raw_stream(self.device, stream)
+        shape = (raw, num_seqs, q_heads, max_context_len)
+        known = self._fitting.get(shape)
+        if known is not None:
+            return known
         # A batch's split counters lie in front of its partials and take as much
         # as it has sequences. Behind the same front all batches' partials begin
         # at one place, and no batch finds another's where its counters are.
         counters = (num_seqs * self.kv_heads * 4 + 255) // 256 * 256
-        front = max(_COUNTER_FRONT, counters)
-        need = self.workspace_size(num_seqs, q_heads, max_context_len) - counters + front
-        key = _stream_handle(self.device, stream).value
-        if front != _COUNTER_FRONT:
-            key = (key, front)
-        ws = self._workspaces.get(key)
-        if ws is None or ws.numel() < need:
-            used = stream if stream is not None else torch.cuda.current_stream(self.device)
-            if ws is not None:
-                ws.record_stream(used)
-            ws = torch.empty(need, dtype=torch.uint8, device=f"cuda:{self.device}")
-            error = _lib.error_buffer()
-            _check(self._lib.inferlab_cuda_paged_decode_workspace_init(
-                _vp(ws), need, _stream_handle(self.device, stream), error, len(error)), error)
-            self._workspaces[key] = ws
-        return ws[front - counters:]
+        partials = self.workspace_size(num_seqs, q_heads, max_context_len) - counters
+        front, ws = self._workspaces.get(raw, (0, None))
+        if ws is None or front < counters or ws.numel() - front < partials:
+            # An outgrown one goes, and with it what was known to fit it. Both
+            # parts only grow, the front in powers of two.
+            room = 0 if ws is None else ws.numel() - front
+            front = max(front, _COUNTER_FRONT, 1 << (counters - 1).bit_length())
+            ws = self._zeroed(front + max(room, partials), front, stream)
+            self._workspaces[raw] = front, ws
+            self._fitting.clear()
+        if len(self._fitting) > 1024:
+            self._fitting.clear()
+        self._fitting[shape] = ws = ws[front - counters:]
+        return ws
+
+    def _zeroed(self, size: int, front: int, stream) -> torch.Tensor:
+        """A workspace whose first `front` bytes are zero, allocated on the stream that uses it, so
+        that its memory is reused only behind that stream's work."""
+        used = stream if stream is not None else torch.cuda.current_stream(self.device)
+        with torch.cuda.stream(used):
+            ws = torch.empty(size, dtype=torch.uint8, device=f"cuda:{self.device}")
+        error = _lib.error_buffer()
+        _check(self._lib.inferlab_cuda_paged_decode_workspace_init(
+            _vp(ws), front, ctypes.c_void_p(used.cuda_stream), error, len(error)), error)
+        return ws
 
     def decode(self, queries: torch.Tensor, block_tables: torch.Tensor,
                context_lens: torch.Tensor, max_context_len: int | None = None,
