@@ -63,7 +63,7 @@ def _require(tensor: torch.Tensor, name: str, dtype, device: int) -> torch.Tenso
     return tensor
 
 
-_COUNTER_FRONT = 65536  # bytes of split counters that a pool's own workspace starts with
+_COUNTER_FRONT = 65536  # bytes of split counters: all of a 4-bit batch's, a wide pool's at first
 
 
 def _expect(tensor, name: str, dtype, device: int) -> int:
@@ -117,10 +117,9 @@ class CudaKvPool:
         self.row_bytes = info.block_bytes // info.block_tokens * (1 if kv_bits == 4 else 2)
         self._key_ptr = info.key_arena
         self._value_ptr = info.value_arena
-        self._workspaces: dict = {}  # by stream
+        self._workspaces: dict = {}  # by stream: bytes of its front, and the workspace
         self._fitting: dict = {}  # (stream, batch shape) -> the part of a workspace that fits it
         self._views: dict = {}  # weak: a view keeps the pool, not the pool its views
-        self._kv4_workspaces: dict = {}  # (stream, batch shape) -> a workspace that fits it
 
     # -- lifetime -----------------------------------------------------------
     def close(self) -> None:
@@ -409,50 +408,52 @@ class CudaKvPool:
         """Fixes later decodes' split length at blocks_per_split 16-token
         blocks (0: the planner chooses, the default). A tuning and test knob
         (inferlab_cuda_pool_set_decode_split)."""
-        self._kv4_workspaces.clear()
         self._fitting.clear()
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_pool_set_decode_split(
             self._handle, int(blocks_per_split), error, len(error)), error)
 
-    def _cached_workspace(self, num_seqs, q_heads, max_context_len, stream):
-        """The pool's own decode workspace, one per stream: decodes on one
-        stream run in order and may share it, decodes on two streams would race
-        on its split counters and partials. Returned is the part of it that this
-        batch shape uses."""
-        raw = _raw_stream(self.device, stream)
-        shape = (raw, num_seqs, q_heads, max_context_len)
-        known = self._fitting.get(shape)
-        if known is not None:
-            return known
-        # A batch's split counters lie in front of its partials and take as much
-        # as it has sequences. Behind the same front all batches' partials begin
-        # at one place, and no batch finds another's where its counters are.
-        counters = (num_seqs * self.kv_heads * 4 + 255) // 256 * 256
-        partials = self.workspace_size(num_seqs, q_heads, max_context_len) - counters
-        front, ws = self._workspaces.get(raw, (0, None))
-        if ws is None or front < counters or ws.numel() - front < partials:
-            # An outgrown one goes, and with it what was known to fit it. Both
-            # parts only grow, the front in powers of two.
-            room = 0 if ws is None else ws.numel() - front
-            front = max(front, _COUNTER_FRONT, 1 << (counters - 1).bit_length())
-            ws = self._zeroed(front + max(room, partials), front, stream)
-            self._workspaces[raw] = front, ws
-            self._fitting.clear()
+    def _own_workspace(self, raw, stream, num_seqs, q_heads, max_query_count, max_context_len):
+        """The part that a batch shape uses of the pool's own workspace, of which there is one per
+        stream: calls on one stream run in order and may share it, calls on two streams would race
+        on its split counters and partials. A capture gets one of its own, zeroed by the graph, so
+        that graphs replayed side by side share none and none outlives what it was captured with."""
+        shape = (raw, num_seqs, q_heads, max_query_count, max_context_len)
+        if stream is None and not torch.cuda.is_current_stream_capturing():
+            known = self._fitting.get(shape)
+            if known is not None:
+                return known
+        # A batch's split counters lie in front of its partials; a wide pool's take as much as it
+        # has sequences, a 4-bit pool's always the same. Behind one front all batches' partials
+        # begin at one place, and no batch finds another's where its counters are.
+        counters = (_COUNTER_FRONT if self.kv_bits == 4
+                    else (num_seqs * self.kv_heads * 4 + 255) // 256 * 256)
+        partials = max(0, self.workspace_size(num_seqs, q_heads, max_context_len,
+                                              max_query_count) - counters)
+        used = stream if stream is not None else torch.cuda.current_stream(self.device)
+        with torch.cuda.stream(used):  # the allocation belongs to that stream
+            if torch.cuda.is_current_stream_capturing():
+                return self._zeroed(counters + partials, counters, used)
+            front, ws = self._workspaces.get(raw, (0, None))
+            if ws is None or front < counters or ws.numel() - front < partials:
+                # An outgrown one goes, and with it what was known to fit it. Both
+                # parts only grow, the front in powers of two.
+                room = 0 if ws is None else ws.numel() - front
+                front = max(front, _COUNTER_FRONT, 1 << (counters - 1).bit_length())
+                ws = self._zeroed(front + max(room, partials), front, used)
+                self._workspaces[raw] = front, ws
+                self._fitting.clear()
         if len(self._fitting) > 1024:
             self._fitting.clear()
         self._fitting[shape] = ws = ws[front - counters:]
         return ws
 
     def _zeroed(self, size: int, front: int, stream) -> torch.Tensor:
-        """A workspace whose first `front` bytes are zero, allocated on the stream that uses it, so
-        that its memory is reused only behind that stream's work."""
-        used = stream if stream is not None else torch.cuda.current_stream(self.device)
-        with torch.cuda.stream(used):
-            ws = torch.empty(size, dtype=torch.uint8, device=f"cuda:{self.device}")
+        """A workspace whose first `front` bytes the (current) stream makes zero."""
+        ws = torch.empty(max(16, size), dtype=torch.uint8, device=f"cuda:{self.device}")
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_paged_decode_workspace_init(
-            _vp(ws), front, ctypes.c_void_p(used.cuda_stream), error, len(error)), error)
+            _vp(ws), front, ctypes.c_void_p(stream.cuda_stream), error, len(error)), error)
         return ws
 
     def decode(self, queries: torch.Tensor, block_tables: torch.Tensor,
@@ -479,7 +480,8 @@ class CudaKvPool:
             out = torch.empty_like(queries)
         _require(out, "out", torch.float32, dev)
         if workspace is None:
-            workspace = self._cached_workspace(num_seqs, q_heads, max_context_len, stream)
+            workspace = self._own_workspace(_raw_stream(dev, stream), stream, num_seqs, q_heads, 1,
+                                            max_context_len)
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_paged_decode(
             self._handle, _vp(queries), _vp(block_tables), block_tables.shape[1],
@@ -558,7 +560,8 @@ class CudaKvPool:
             l = torch.empty_like(m)
             o = torch.empty_like(queries)
         if workspace is None:
-            workspace = self._cached_workspace(num_seqs, q_heads, max_context_len, stream)
+            workspace = self._own_workspace(_raw_stream(dev, stream), stream, num_seqs, q_heads, 1,
+                                            max_context_len)
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_paged_decode_partials(
             self._handle, _vp(queries), _vp(block_tables), block_tables.shape[1],
@@ -622,29 +625,6 @@ class CudaKvPool:
                 raise AttentionError("4-bit attention output must be shaped like the queries")
         return KV_FP32 if dtype is torch.float32 else self.dtype, queries_at, out_at, out
 
-    def _kv4_workspace(self, raw, stream, *shape):
-        """The pool's workspace of the stream, for a batch shape (num_seqs, q_heads,
-        max_query_count, max_context_len). A capture gets its own, so that two graphs that are
-        replayed side by side never share one."""
-        if stream is None and not torch.cuda.is_current_stream_capturing():
-            known = self._kv4_workspaces.get((raw, *shape))
-            if known is not None:
-                return known
-        num_seqs, q_heads, queries, context = shape
-        used = stream if stream is not None else torch.cuda.current_stream(self.device)
-        with torch.cuda.stream(used):  # the allocation belongs to that stream
-            if torch.cuda.is_current_stream_capturing():
-                return self.make_workspace(num_seqs, q_heads, context, used, queries)
-            ws = self._workspaces.get(raw)
-            if ws is None or ws.numel() < self.workspace_size(num_seqs, q_heads, context, queries):
-                ws = self.make_workspace(num_seqs, q_heads, context, used, queries)
-                self._workspaces[raw] = ws
-                self._kv4_workspaces.clear()  # nothing keeps the outgrown one
-            if len(self._kv4_workspaces) > 1024:
-                self._kv4_workspaces.clear()
-            self._kv4_workspaces[(raw, *shape)] = ws
-            return ws
-
     def _kv4_decode(self, queries, block_tables, context_lens, max_context_len, out, workspace,
                     stream):
         dev = self.device
@@ -661,7 +641,7 @@ class CudaKvPool:
             max_context_len = max(1, int(context_lens.max().item()))
         raw = _raw_stream(dev, stream)
         if workspace is None:
-            workspace = self._kv4_workspace(raw, stream, num_seqs, q_heads, 1, max_context_len)
+            workspace = self._own_workspace(raw, stream, num_seqs, q_heads, 1, max_context_len)
         workspace_at = _expect(workspace, "workspace", torch.uint8, dev)
         error = _lib.call_error_buffer()
         if self._lib.inferlab_cuda_kv4_decode(
@@ -690,7 +670,7 @@ class CudaKvPool:
             max_context_len = min(table_shape[1] * self.block_tokens, 0x7fffff00)
         raw = _raw_stream(dev, stream)
         if workspace is None:
-            workspace = self._kv4_workspace(raw, stream, segments, q_heads, max_query_count,
+            workspace = self._own_workspace(raw, stream, segments, q_heads, max_query_count,
                                             max_context_len)
         workspace_at = _expect(workspace, "workspace", torch.uint8, dev)
         error = _lib.call_error_buffer()
