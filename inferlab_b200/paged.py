@@ -157,8 +157,10 @@ class CudaKvPool:
             raise AttentionError("a 4-bit pool has one packed arena (arena)")
         known = self._views.get(ptr)
         view = None if known is None else known()
-        if view is None:
-            shape = (self.num_blocks, self.kv_heads, self.block_tokens, self.head_dim)
+        shape = (self.num_blocks, self.kv_heads, self.block_tokens, self.head_dim)
+        # A holder may have turned it into another view in place.
+        if view is None or view.shape != shape or not view.is_contiguous() or \
+                view.data_ptr() != ptr or view.requires_grad:
             view = torch.as_tensor(_DeviceView(ptr, shape, _TYPESTR[self.dtype], self),
                                    device=f"cuda:{self.device}")
             if self.dtype == KV_BF16:
@@ -168,7 +170,8 @@ class CudaKvPool:
 
     @property
     def key_arena(self) -> torch.Tensor:
-        """A torch view of the key arena (no copy; it keeps the pool alive, until close())."""
+        """A torch view of the key arena (no copy; it keeps the pool alive, until close()). While one
+        is held the same tensor is returned again, unless it was reshaped in place."""
         return self._arena(self._key_ptr)
 
     @property
