@@ -145,10 +145,10 @@ class PeerExchange:
         import torch
 
         from . import _lib
-        from .paged import _check, _stream_handle, _vp
+        from .paged import _check, _made, _stream_handle, _vp
 
         if out is None:
-            out = torch.empty((self.rows, self.head_dim), dtype=torch.float32, device=packed.device)
+            out = _made((self.rows, self.head_dim), torch.float32, self.device, stream)
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_peer_exchange_combine(
             self._handle, _vp(packed), _vp(out), _stream_handle(self.device, stream), error,
@@ -163,11 +163,11 @@ class PeerExchange:
         import torch
 
         from . import _lib
-        from .paged import _check, _stream_handle, _vp
+        from .paged import _check, _made, _stream_handle, _vp
 
         num_seqs, q_heads, hd = queries.shape
         if out is None:
-            out = torch.empty((num_seqs, q_heads, hd), dtype=torch.float32, device=queries.device)
+            out = _made((num_seqs, q_heads, hd), torch.float32, self.device, stream)
         ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_paged_decode_exchange(

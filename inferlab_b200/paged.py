@@ -39,6 +39,27 @@ def _stream_handle(device: int, stream) -> ctypes.c_void_p:
     return ctypes.c_void_p(stream.cuda_stream)
 
 
+def _torch_stream(device: int, stream) -> torch.cuda.Stream:
+    """The stream a call runs on (default: the current one) as torch's own."""
+    if stream is None:
+        return torch.cuda.current_stream(device)
+    if isinstance(stream, torch.cuda.Stream):
+        return stream
+    return torch.cuda.ExternalStream(stream.cuda_stream, device=device)
+
+
+def _made(shape, dtype, device: int, stream) -> torch.Tensor:
+    """Memory that a call fills on `stream`, allocated there: the current stream may still use what
+    its own allocations reuse. It is then read on the current stream, as a rule, behind `stream`."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=f"cuda:{device}")
+    here = torch.cuda.current_stream(device)
+    with torch.cuda.stream(_torch_stream(device, stream)):
+        made = torch.empty(shape, dtype=dtype, device=f"cuda:{device}")
+    made.record_stream(here)
+    return made
+
+
 class _DeviceView:
     """Exposes a raw device range through __cuda_array_interface__. The tensor made from it keeps
     it, and so `owner`, whose memory it is, alive."""
@@ -265,7 +286,7 @@ class CudaKvPool:
             if queries.shape[0] != rows:
                 raise AttentionError("paged KV append shapes do not match the pool")
             if q_out is None:
-                q_out = torch.empty(queries.shape, dtype=dtype, device=queries.device)
+                q_out = _made(queries.shape, dtype, dev, stream)
             out_dtype = q_out.dtype
             out_at = _expect(q_out, "q_out", out_dtype, dev)
             if q_out.shape != queries.shape or \
@@ -309,7 +330,7 @@ class CudaKvPool:
                 block_tables.dim() != 2:
             raise AttentionError("projection shapes do not match the pool")
         if q_out is None:
-            q_out = torch.empty((tokens, q_heads, self.head_dim), dtype=dtype, device=f"cuda:{dev}")
+            q_out = _made((tokens, q_heads, self.head_dim), dtype, dev, stream)
         _require(q_out, "q_out", dtype, dev)
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_qkv_project_append(
@@ -341,7 +362,7 @@ class CudaKvPool:
             if residual.shape != (tokens, out_dim):
                 raise AttentionError("projection shapes do not match")
         if out is None:
-            out = torch.empty((tokens, out_dim), dtype=torch.float32, device=f"cuda:{dev}")
+            out = _made((tokens, out_dim), torch.float32, dev, stream)
         _require(out, "out", torch.float32, dev)
         a_dtype = KV_FP32 if attention.dtype == torch.float32 else self.dtype
         error = _lib.error_buffer()
@@ -358,8 +379,8 @@ class CudaKvPool:
         if block_table.numel() != (tokens + self.block_tokens - 1) // self.block_tokens:
             raise AttentionError("paged KV block table length is inconsistent")
         shape = (tokens, self.kv_heads, self.head_dim)
-        keys = torch.empty(shape, dtype=TORCH_DTYPES[self.dtype], device=f"cuda:{dev}")
-        values = torch.empty_like(keys)
+        keys = _made(shape, TORCH_DTYPES[self.dtype], dev, stream)
+        values = _made(shape, TORCH_DTYPES[self.dtype], dev, stream)
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_kv_gather(
             self._handle, _vp(block_table), tokens, _vp(keys), _vp(values),
@@ -378,8 +399,8 @@ class CudaKvPool:
         rows = row_sequences.numel()
         if positions.numel() != rows or block_tables.dim() != 2:
             raise AttentionError("paged KV gather shapes do not match")
-        keys, values = torch.empty((2, rows, self.kv_heads, self.head_dim),
-                                   dtype=TORCH_DTYPES[self.dtype], device=positions.device).unbind()
+        keys, values = _made((2, rows, self.kv_heads, self.head_dim), TORCH_DTYPES[self.dtype], dev,
+                             stream).unbind()
         error = _lib.call_error_buffer()
         if self._lib.inferlab_cuda_kv_gather_rows(
                 self._handle, sequences_at, positions_at, rows, tables_at, block_tables.shape[0],
@@ -401,7 +422,7 @@ class CudaKvPool:
         """A zero-initialised decode workspace for this batch shape (max_query_count: the prefill
         of a 4-bit pool)."""
         size = max(16, self.workspace_size(num_seqs, q_heads, max_context_len, max_query_count))
-        ws = torch.empty(size, dtype=torch.uint8, device=f"cuda:{self.device}")
+        ws = _made(size, torch.uint8, self.device, stream)
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_paged_decode_workspace_init(
             _vp(ws), size, _stream_handle(self.device, stream), error, len(error)), error)
@@ -433,7 +454,7 @@ class CudaKvPool:
                     else (num_seqs * self.kv_heads * 4 + 255) // 256 * 256)
         partials = max(0, self.workspace_size(num_seqs, q_heads, max_context_len,
                                               max_query_count) - counters)
-        used = stream if stream is not None else torch.cuda.current_stream(self.device)
+        used = _torch_stream(self.device, stream)
         with torch.cuda.stream(used):  # the allocation belongs to that stream
             if torch.cuda.is_current_stream_capturing():
                 return self._zeroed(counters + partials, counters, used)
@@ -480,7 +501,7 @@ class CudaKvPool:
         if max_context_len is None:
             max_context_len = int(context_lens.max().item())
         if out is None:
-            out = torch.empty_like(queries)
+            out = _made(queries.shape, torch.float32, dev, stream)
         _require(out, "out", torch.float32, dev)
         if workspace is None:
             workspace = self._own_workspace(_raw_stream(dev, stream), stream, num_seqs, q_heads, 1,
@@ -559,9 +580,9 @@ class CudaKvPool:
             l = flat[rows:2 * rows].view(num_seqs, q_heads)
             o = flat[2 * rows:].view(num_seqs, q_heads, hd)
         else:
-            m = torch.empty((num_seqs, q_heads), dtype=torch.float32, device=f"cuda:{dev}")
-            l = torch.empty_like(m)
-            o = torch.empty_like(queries)
+            m = _made((num_seqs, q_heads), torch.float32, dev, stream)
+            l = _made((num_seqs, q_heads), torch.float32, dev, stream)
+            o = _made(queries.shape, torch.float32, dev, stream)
         if workspace is None:
             workspace = self._own_workspace(_raw_stream(dev, stream), stream, num_seqs, q_heads, 1,
                                             max_context_len)
@@ -601,7 +622,7 @@ class CudaKvPool:
         if hd != self.head_dim:
             raise AttentionError("paged prefill head_dim does not match the pool")
         if out is None:
-            out = torch.empty((total, q_heads, hd), dtype=torch.float32, device=f"cuda:{dev}")
+            out = _made((total, q_heads, hd), torch.float32, dev, stream)
         _require(out, "out", torch.float32, dev)
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_paged_prefill(
@@ -611,7 +632,7 @@ class CudaKvPool:
             len(error)), error)
         return out
 
-    def _kv4_operands(self, queries, out):
+    def _kv4_operands(self, queries, out, stream):
         """The query / output type code, the addresses, and the output of a 4-bit attention call."""
         dtype = queries.dtype
         if dtype is not torch.float32 and dtype is not TORCH_DTYPES[self.dtype]:
@@ -620,7 +641,7 @@ class CudaKvPool:
         if queries.dim() != 3 or queries.shape[2] != self.head_dim:
             raise AttentionError("4-bit attention shapes do not match the pool")
         if out is None:
-            out = torch.empty_like(queries)
+            out = _made(queries.shape, dtype, self.device, stream)
             out_at = out.data_ptr()
         else:
             out_at = _expect(out, "out", dtype, self.device)
@@ -631,7 +652,7 @@ class CudaKvPool:
     def _kv4_decode(self, queries, block_tables, context_lens, max_context_len, out, workspace,
                     stream):
         dev = self.device
-        query_type, queries_at, out_at, out = self._kv4_operands(queries, out)
+        query_type, queries_at, out_at, out = self._kv4_operands(queries, out, stream)
         tables_at = _expect(block_tables, "block_tables", torch.int32, dev)
         lens_at = _expect(context_lens, "context_lens", torch.int32, dev)
         num_seqs, q_heads, _ = queries.shape
@@ -656,7 +677,7 @@ class CudaKvPool:
     def _kv4_prefill(self, queries, block_tables, query_starts, query_counts, query_offsets,
                      max_query_count, out, stream, max_context_len, workspace):
         dev = self.device
-        query_type, queries_at, out_at, out = self._kv4_operands(queries, out)
+        query_type, queries_at, out_at, out = self._kv4_operands(queries, out, stream)
         segments = query_starts.numel()
         tables_at = _expect(block_tables, "block_tables", torch.int32, dev)
         starts_at = _expect(query_starts, "query_starts", torch.int32, dev)
@@ -695,7 +716,7 @@ def lse_combine(part_m: torch.Tensor, part_l: torch.Tensor, part_o: torch.Tensor
     for name, t in (("part_m", part_m), ("part_l", part_l), ("part_o", part_o)):
         _require(t, name, torch.float32, dev)
     if out is None:
-        out = torch.empty(part_o.shape[1:], dtype=torch.float32, device=part_o.device)
+        out = _made(part_o.shape[1:], torch.float32, dev, stream)
     error = _lib.error_buffer()
     _check(_lib.lib().inferlab_cuda_lse_combine(
         _vp(part_m), _vp(part_l), _vp(part_o), parts, rows, hd, _vp(out),
@@ -712,7 +733,7 @@ def lse_combine_packed(packed: torch.Tensor, parts: int, rows: int, head_dim: in
     if packed.numel() != parts * rows * (head_dim + 2):
         raise AttentionError("packed partials buffer has the wrong size")
     if out is None:
-        out = torch.empty((rows, head_dim), dtype=torch.float32, device=packed.device)
+        out = _made((rows, head_dim), torch.float32, dev, stream)
     error = _lib.error_buffer()
     _check(_lib.lib().inferlab_cuda_lse_combine_packed(
         _vp(packed), parts, rows, head_dim, _vp(out), _stream_handle(dev, stream), error,
