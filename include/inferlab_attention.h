@@ -315,7 +315,7 @@ size_t inferlab_cuda_paged_decode_workspace_size(const InferlabCudaKvPool* pool,
  * Fixes the decode split length of this pool's later decode calls at
  * blocks_per_split 16-token blocks (1..1024; 0 restores the planner's own
  * choice, the default). The planner still caps a split at 256 blocks and a
- * context at 64 splits. A tuning and test setting with no counterpart in the
+ * context at 64 splits (a 4-bit pool's: at 256 splits). A tuning and test setting with no counterpart in the
  * reference (its decode is one host call per sequence); workspace sizes
  * follow it, so query inferlab_cuda_paged_decode_workspace_size after
  * changing it. Not synchronised with decode calls on other host threads.
@@ -324,11 +324,12 @@ int inferlab_cuda_pool_set_decode_split(InferlabCudaKvPool* pool, uint32_t block
                                         char* error, size_t error_capacity);
 
 /*
- * Zeroes the counters at the front of a decode workspace. Needed once per
- * workspace before its first use; the decode kernel leaves them at zero. In
- * inferlab_cuda_paged_decode they take num_seqs * kv_heads words, rounded up to
- * 256 bytes, and partials follow: before a batch of more sequences than the
- * last ones on the same workspace, zero it again.
+ * Zeroes a decode workspace. Needed once per workspace before its first use,
+ * for its first 64 KB at least, which hold the split counters; the decode
+ * kernels leave them at zero. Batches of any sizes may use a workspace in turn
+ * that is large enough for each (one of more than 16384 sequences x kv_heads
+ * has its counters zeroed on every call); launches that may overlap need one
+ * each.
  */
 int inferlab_cuda_paged_decode_workspace_init(void* workspace, size_t workspace_bytes,
                                               void* stream, char* error, size_t error_capacity);

@@ -9,8 +9,8 @@ struct InferlabCudaRotaryAppend;
 
 namespace ilb {
 
-// Bytes of decode workspace a batch of this shape needs, and how many of its
-// leading bytes are the split counters that must be zero before a launch.
+// Bytes of workspace launch_paged_decode needs for a batch of this shape, and how
+// many of its leading bytes are the split counters that must be zero before it.
 std::size_t decode_workspace_bytes(const InferlabCudaKvPool& pool, std::uint32_t num_seqs,
                                    std::uint32_t q_heads, std::uint32_t max_context_len);
 std::size_t decode_counter_bytes(const InferlabCudaKvPool& pool, std::uint32_t num_seqs);
@@ -26,8 +26,8 @@ void check_decode_arguments(const InferlabCudaKvPool& pool, const float* queries
                             const std::int32_t* context_lens, std::uint32_t num_seqs,
                             std::uint32_t q_heads, std::uint32_t max_context_len);
 
-// Launches the decode kernel with the given workspace; the pool's device must
-// be current.
+// Launches the decode kernel with the given workspace, whose counters the caller
+// has zeroed for this batch; the pool's device must be current.
 void launch_paged_decode(InferlabCudaKvPool& pool, const float* queries,
                          const std::int32_t* block_tables, std::uint32_t max_blocks,
                          const std::int32_t* context_lens, std::uint32_t num_seqs,

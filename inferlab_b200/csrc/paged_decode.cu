@@ -855,10 +855,25 @@ DecodePlan plan_decode(std::uint32_t num_seqs, std::uint32_t kv_heads,
     return DecodePlan{bps, max_splits};
 }
 
+// A caller keeps a workspace for batches of many sizes. Its split counters lie in
+// front, zero between launches, and behind them the partials of whatever batch ran
+// last, so the front is the same for all batches; one whose counters need more has
+// them zeroed on every call. Callers in this library that zero the counters
+// themselves (`zeroed`) need no more room than they take.
+constexpr std::size_t kCounterFront = 65536;
+
+std::size_t counter_bytes_for(std::uint32_t num_seqs, std::uint32_t kv_heads) {
+    return (static_cast<std::size_t>(num_seqs) * kv_heads * 4 + 255) & ~std::size_t(255);
+}
+std::size_t front_bytes_for(std::uint32_t num_seqs, std::uint32_t kv_heads, bool zeroed) {
+    const std::size_t counters = counter_bytes_for(num_seqs, kv_heads);
+    return zeroed ? counters : std::max(counters, kCounterFront);
+}
+
 std::size_t workspace_bytes_for(std::uint32_t num_seqs, std::uint32_t q_heads,
                                 std::uint32_t kv_heads, std::uint32_t head_dim,
-                                const DecodePlan& plan) {
-    const std::size_t counters = (static_cast<std::size_t>(num_seqs) * kv_heads * 4 + 255) & ~std::size_t(255);
+                                const DecodePlan& plan, bool zeroed) {
+    const std::size_t counters = front_bytes_for(num_seqs, kv_heads, zeroed);
     const std::size_t slots = static_cast<std::size_t>(num_seqs) * q_heads * plan.max_splits;
     const std::size_t ml = (slots * 2 * 4 + 255) & ~std::size_t(255);
     return counters + ml + slots * head_dim * 4;
@@ -987,7 +1002,7 @@ void run_decode(InferlabCudaKvPool& p, const float* queries, const std::int32_t*
                 std::uint32_t max_blocks, const std::int32_t* context_lens, std::uint32_t num_seqs,
                 std::uint32_t q_heads, std::uint32_t max_context_len, float* out, float* part_m,
                 float* part_l, float* part_o, void* workspace, std::size_t workspace_bytes,
-                cudaStream_t stream, const ExchangeView* xview = nullptr) {
+                bool zeroed, cudaStream_t stream, const ExchangeView* xview = nullptr) {
     const std::uint32_t group = q_heads / p.kv_heads;
     std::size_t smem = 0;
     DecodeKernel kernel = select_decode(p, group, smem, xview != nullptr);
@@ -1053,7 +1068,7 @@ void run_decode(InferlabCudaKvPool& p, const float* queries, const std::int32_t*
         throw std::runtime_error("paged decode queries must be 16-byte aligned");
     }
     const DecodePlan plan = full_plan(p, num_seqs, q_heads, max_context_len);
-    const std::size_t need = workspace_bytes_for(num_seqs, q_heads, p.kv_heads, p.head_dim, plan);
+    const std::size_t need = workspace_bytes_for(num_seqs, q_heads, p.kv_heads, p.head_dim, plan, zeroed);
     if (plan.max_splits > 1 && (workspace == nullptr || workspace_bytes < need)) {
         throw std::runtime_error("paged decode workspace is too small");
     }
@@ -1078,8 +1093,10 @@ void run_decode(InferlabCudaKvPool& p, const float* queries, const std::int32_t*
     d.part_o = part_o;
     if (workspace != nullptr) {
         auto* base = static_cast<unsigned char*>(workspace);
-        const std::size_t counters =
-            (static_cast<std::size_t>(num_seqs) * p.kv_heads * 4 + 255) & ~std::size_t(255);
+        const std::size_t counters = front_bytes_for(num_seqs, p.kv_heads, zeroed);
+        if (plan.max_splits > 1 && !zeroed && counters > kCounterFront) {
+            cuda_check(cudaMemsetAsync(workspace, 0, counters, stream), "cudaMemsetAsync split counters");
+        }
         const std::size_t slots = static_cast<std::size_t>(num_seqs) * q_heads * plan.max_splits;
         const std::size_t ml = (slots * 2 * 4 + 255) & ~std::size_t(255);
         d.ws_count = reinterpret_cast<std::uint32_t*>(base);
@@ -1113,7 +1130,7 @@ namespace ilb {
 std::size_t decode_workspace_bytes(const InferlabCudaKvPool& pool, std::uint32_t num_seqs,
                                    std::uint32_t q_heads, std::uint32_t max_context_len) {
     const auto plan = full_plan(pool, num_seqs, q_heads, max_context_len);
-    return workspace_bytes_for(num_seqs, q_heads, pool.kv_heads, pool.head_dim, plan);
+    return workspace_bytes_for(num_seqs, q_heads, pool.kv_heads, pool.head_dim, plan, true);
 }
 
 std::size_t decode_scratch_bytes(const InferlabCudaKvPool& pool, std::uint32_t num_seqs,
@@ -1122,11 +1139,11 @@ std::size_t decode_scratch_bytes(const InferlabCudaKvPool& pool, std::uint32_t n
     if (select_decode(pool, q_heads / pool.kv_heads, smem) == nullptr) return 0;
     const auto plan = full_plan(pool, num_seqs, q_heads, max_context_len);
     if (plan.max_splits <= 1) return 0;
-    return workspace_bytes_for(num_seqs, q_heads, pool.kv_heads, pool.head_dim, plan);
+    return workspace_bytes_for(num_seqs, q_heads, pool.kv_heads, pool.head_dim, plan, true);
 }
 
 std::size_t decode_counter_bytes(const InferlabCudaKvPool& pool, std::uint32_t num_seqs) {
-    return (static_cast<std::size_t>(num_seqs) * pool.kv_heads * 4 + 255) & ~std::size_t(255);
+    return counter_bytes_for(num_seqs, pool.kv_heads);
 }
 
 void check_decode_arguments(const InferlabCudaKvPool& pool, const float* queries,
@@ -1143,7 +1160,7 @@ void launch_paged_decode(InferlabCudaKvPool& pool, const float* queries,
                          std::uint32_t q_heads, std::uint32_t max_context_len, float* out,
                          void* workspace, std::size_t workspace_bytes, cudaStream_t stream) {
     run_decode(pool, queries, block_tables, max_blocks, context_lens, num_seqs, q_heads,
-               max_context_len, out, nullptr, nullptr, nullptr, workspace, workspace_bytes, stream);
+               max_context_len, out, nullptr, nullptr, nullptr, workspace, workspace_bytes, true, stream);
 }
 
 }  // namespace ilb
@@ -1183,14 +1200,14 @@ extern "C" int inferlab_cuda_paged_decode_exchange(InferlabCudaKvPool* pool, con
         }
         const ilb::DecodePlan plan = ilb::full_plan(p, num_seqs, q_heads, max_context_len);
         const std::size_t need =
-            ilb::workspace_bytes_for(num_seqs, q_heads, p.kv_heads, p.head_dim, plan);
+            ilb::workspace_bytes_for(num_seqs, q_heads, p.kv_heads, p.head_dim, plan, false);
         if (plan.max_splits > 1 && (workspace == nullptr || workspace_bytes < need)) {
             throw std::runtime_error("paged decode workspace is too small");
         }
         const ilb::ExchangeView view = ilb::exchange_take_step(
             exchange, p.device, static_cast<std::uint64_t>(num_seqs) * q_heads, p.head_dim);
         ilb::run_decode(p, queries, block_tables, max_blocks, context_lens, num_seqs, q_heads,
-                        max_context_len, out, nullptr, nullptr, nullptr, workspace, workspace_bytes,
+                        max_context_len, out, nullptr, nullptr, nullptr, workspace, workspace_bytes, false,
                         static_cast<cudaStream_t>(stream), &view);
     });
 }
@@ -1202,7 +1219,7 @@ extern "C" std::size_t inferlab_cuda_paged_decode_workspace_size(const InferlabC
     if (pool == nullptr || pool->kv_bits != 0 || num_seqs == 0 || q_heads == 0 || max_context_len == 0) return 0;
     try {
         const auto plan = ilb::full_plan(*pool, num_seqs, q_heads, max_context_len);
-        return ilb::workspace_bytes_for(num_seqs, q_heads, pool->kv_heads, pool->head_dim, plan);
+        return ilb::workspace_bytes_for(num_seqs, q_heads, pool->kv_heads, pool->head_dim, plan, false);
     } catch (...) {
         return 0;  // the decode call itself reports why
     }
@@ -1248,7 +1265,7 @@ extern "C" int inferlab_cuda_paged_decode(InferlabCudaKvPool* pool, const float*
         if (out == nullptr) throw std::runtime_error("paged decode output pointer is null");
         DeviceGuard guard(p.device);
         run_decode(p, queries, block_tables, max_blocks_per_seq, context_lens, num_seqs, q_heads,
-                   max_context_len, out, nullptr, nullptr, nullptr, workspace, workspace_bytes,
+                   max_context_len, out, nullptr, nullptr, nullptr, workspace, workspace_bytes, false,
                    static_cast<cudaStream_t>(stream));
     });
 }
@@ -1270,7 +1287,7 @@ extern "C" int inferlab_cuda_paged_decode_partials(
         }
         DeviceGuard guard(p.device);
         run_decode(p, queries, block_tables, max_blocks_per_seq, context_lens, num_seqs, q_heads,
-                   max_context_len, nullptr, part_m, part_l, part_o, workspace, workspace_bytes,
+                   max_context_len, nullptr, part_m, part_l, part_o, workspace, workspace_bytes, false,
                    static_cast<cudaStream_t>(stream));
     });
 }

@@ -84,7 +84,7 @@ def _require(tensor: torch.Tensor, name: str, dtype, device: int) -> torch.Tenso
     return tensor
 
 
-_COUNTER_FRONT = 65536  # bytes of split counters: all of a 4-bit batch's, a wide pool's at first
+_COUNTER_FRONT = 65536  # bytes at the front of a workspace that must start at zero
 
 
 def _expect(tensor, name: str, dtype, device: int) -> int:
@@ -138,8 +138,8 @@ class CudaKvPool:
         self.row_bytes = info.block_bytes // info.block_tokens * (1 if kv_bits == 4 else 2)
         self._key_ptr = info.key_arena
         self._value_ptr = info.value_arena
-        self._workspaces: dict = {}  # by stream: bytes of its front, and the workspace
-        self._fitting: dict = {}  # (stream, batch shape) -> the part of a workspace that fits it
+        self._workspaces: dict = {}  # by stream
+        self._fitting: dict = {}  # (stream, batch shape) -> a workspace that fits it
         self._views: dict = {}  # weak: a view keeps the pool, not the pool its views
 
     # -- lifetime -----------------------------------------------------------
@@ -420,7 +420,7 @@ class CudaKvPool:
     def make_workspace(self, num_seqs: int, q_heads: int, max_context_len: int,
                        stream=None, max_query_count: int = 1) -> torch.Tensor:
         """A zero-initialised decode workspace for this batch shape (max_query_count: the prefill
-        of a 4-bit pool)."""
+        of a 4-bit pool) and every smaller one."""
         size = max(16, self.workspace_size(num_seqs, q_heads, max_context_len, max_query_count))
         ws = _made(size, torch.uint8, self.device, stream)
         error = _lib.error_buffer()
@@ -438,46 +438,37 @@ class CudaKvPool:
             self._handle, int(blocks_per_split), error, len(error)), error)
 
     def _own_workspace(self, raw, stream, num_seqs, q_heads, max_query_count, max_context_len):
-        """The part that a batch shape uses of the pool's own workspace, of which there is one per
-        stream: calls on one stream run in order and may share it, calls on two streams would race
-        on its split counters and partials. A capture gets one of its own, zeroed by the graph, so
-        that graphs replayed side by side share none and none outlives what it was captured with."""
+        """A workspace for a batch shape: the pool's own of the stream, as calls on one stream run
+        in order and may share it, calls on two streams would race on its split counters and
+        partials. A capture gets one of its own, zeroed by the graph, so that graphs replayed side
+        by side share none and none outlives what it was captured with."""
         shape = (raw, num_seqs, q_heads, max_query_count, max_context_len)
         if stream is None and not torch.cuda.is_current_stream_capturing():
             known = self._fitting.get(shape)
             if known is not None:
                 return known
-        # A batch's split counters lie in front of its partials; a wide pool's take as much as it
-        # has sequences, a 4-bit pool's always the same. Behind one front all batches' partials
-        # begin at one place, and no batch finds another's where its counters are.
-        counters = (_COUNTER_FRONT if self.kv_bits == 4
-                    else (num_seqs * self.kv_heads * 4 + 255) // 256 * 256)
-        partials = max(0, self.workspace_size(num_seqs, q_heads, max_context_len,
-                                              max_query_count) - counters)
+        need = self.workspace_size(num_seqs, q_heads, max_context_len, max_query_count)
         used = _torch_stream(self.device, stream)
         with torch.cuda.stream(used):  # the allocation belongs to that stream
             if torch.cuda.is_current_stream_capturing():
-                return self._zeroed(counters + partials, counters, used)
-            front, ws = self._workspaces.get(raw, (0, None))
-            if ws is None or front < counters or ws.numel() - front < partials:
-                # An outgrown one goes, and with it what was known to fit it. Both
-                # parts only grow, the front in powers of two.
-                room = 0 if ws is None else ws.numel() - front
-                front = max(front, _COUNTER_FRONT, 1 << (counters - 1).bit_length())
-                ws = self._zeroed(front + max(room, partials), front, used)
-                self._workspaces[raw] = front, ws
-                self._fitting.clear()
+                return self._zeroed(need, used)
+            ws = self._workspaces.get(raw)
+            if ws is None or ws.numel() < need:
+                ws = self._zeroed(need, used)
+                self._workspaces[raw] = ws
+                self._fitting.clear()  # nothing keeps the outgrown one
         if len(self._fitting) > 1024:
             self._fitting.clear()
-        self._fitting[shape] = ws = ws[front - counters:]
+        self._fitting[shape] = ws
         return ws
 
-    def _zeroed(self, size: int, front: int, stream) -> torch.Tensor:
-        """A workspace whose first `front` bytes the (current) stream makes zero."""
+    def _zeroed(self, size: int, stream) -> torch.Tensor:
+        """A workspace whose split counters, all in front, the (current) stream makes zero."""
         ws = torch.empty(max(16, size), dtype=torch.uint8, device=f"cuda:{self.device}")
         error = _lib.error_buffer()
         _check(self._lib.inferlab_cuda_paged_decode_workspace_init(
-            _vp(ws), front, ctypes.c_void_p(stream.cuda_stream), error, len(error)), error)
+            _vp(ws), min(ws.numel(), _COUNTER_FRONT), ctypes.c_void_p(stream.cuda_stream), error,
+            len(error)), error)
         return ws
 
     def decode(self, queries: torch.Tensor, block_tables: torch.Tensor,

@@ -60,3 +60,31 @@ def test_a_workspace_that_two_shapes_outgrow_in_turn_settles(torch):
     pool.synchronize()
     assert len(set(held)) == 1
     pool.close()
+
+
+@pytest.mark.parametrize("heads,largest", [(8, 130), (64, 330)])
+@pytest.mark.parametrize("dtype", [0, 2])
+def test_one_workspace_of_the_caller_serves_batches_of_all_sizes(torch, dtype, heads, largest):
+    """In any order, also around 16384 (sequence, kv-head) pairs: the bits are those of a workspace made for the batch."""
+    import inferlab_b200 as il
+
+    gen = torch.Generator(device="cuda:0").manual_seed(8)
+    pool = il.CudaKvPool(0, dtype, 64, 16, heads, 64)
+    pool.key_arena.normal_(generator=gen)
+    pool.value_arena.normal_(generator=gen)
+    pool.set_decode_split(1)
+    sizes = [1, 2, 5, 40, 3, largest, 1, largest * 3 // 4, largest - 1, 17, largest * 4 // 5, largest, 2, largest // 2]
+    tables = torch.randint(0, 64, (largest, 6), device="cuda:0", dtype=torch.int32, generator=gen)
+    lens = torch.randint(1, 97, (largest,), device="cuda:0", dtype=torch.int32, generator=gen)
+    queries = torch.randn((largest, heads, 64), device="cuda:0", generator=gen)
+    shared = pool.make_workspace(largest, heads, 96)
+    for n in sizes:
+        args = queries[:n], tables[:n], lens[:n], 96
+        alone = pool.decode(*args, workspace=pool.make_workspace(n, heads, 96))
+        assert torch.equal(pool.decode(*args, workspace=shared), alone)
+        assert torch.equal(pool.decode(*args), alone)
+        # both kinds of output leave the counters as they found them
+        m, l, o = pool.decode_partials(*args, workspace=shared)
+        assert torch.allclose(o / l[..., None], alone, rtol=1e-5, atol=1e-6)
+    pool.synchronize()
+    pool.close()
