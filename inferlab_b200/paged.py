@@ -140,6 +140,7 @@ class CudaKvPool:
         self._value_ptr = info.value_arena
         self._workspaces: dict = {}  # by stream
         self._fitting: dict = {}  # (stream, batch shape) -> a workspace that fits it
+        self._arena_shape = (self.num_blocks, self.kv_heads, self.block_tokens, self.head_dim)
         self._views: dict = {}  # weak: a view keeps the pool, not the pool its views
 
     # -- lifetime -----------------------------------------------------------
@@ -178,11 +179,10 @@ class CudaKvPool:
             raise AttentionError("a 4-bit pool has one packed arena (arena)")
         known = self._views.get(ptr)
         view = None if known is None else known()
-        shape = (self.num_blocks, self.kv_heads, self.block_tokens, self.head_dim)
         # A holder may have turned it into another view in place.
-        if view is None or view.shape != shape or not view.is_contiguous() or \
+        if view is None or view.shape != self._arena_shape or not view.is_contiguous() or \
                 view.data_ptr() != ptr or view.requires_grad:
-            view = torch.as_tensor(_DeviceView(ptr, shape, _TYPESTR[self.dtype], self),
+            view = torch.as_tensor(_DeviceView(ptr, self._arena_shape, _TYPESTR[self.dtype], self),
                                    device=f"cuda:{self.device}")
             if self.dtype == KV_BF16:
                 view = view.view(TORCH_DTYPES[self.dtype])
@@ -492,7 +492,8 @@ class CudaKvPool:
         if max_context_len is None:
             max_context_len = int(context_lens.max().item())
         if out is None:
-            out = _made(queries.shape, torch.float32, dev, stream)
+            out = (torch.empty_like(queries) if stream is None
+                   else _made(queries.shape, torch.float32, dev, stream))
         _require(out, "out", torch.float32, dev)
         if workspace is None:
             workspace = self._own_workspace(_raw_stream(dev, stream), stream, num_seqs, q_heads, 1,
@@ -632,7 +633,8 @@ class CudaKvPool:
         if queries.dim() != 3 or queries.shape[2] != self.head_dim:
             raise AttentionError("4-bit attention shapes do not match the pool")
         if out is None:
-            out = _made(queries.shape, dtype, self.device, stream)
+            out = (torch.empty_like(queries) if stream is None
+                   else _made(queries.shape, dtype, self.device, stream))
             out_at = out.data_ptr()
         else:
             out_at = _expect(out, "out", dtype, self.device)
