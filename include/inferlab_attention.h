@@ -130,8 +130,12 @@ int inferlab_cuda_pool_create(int32_t device, uint32_t dtype, uint64_t num_block
 /*
  * A pool whose K and V rows are held in 4 bits: every 64 dims of a row share an
  * f16 pair (scale, zero) and a code c in 0..15 stands for zero + (c - 8) *
- * scale, with scale = f16((max - min) / 15), zero = f16(min + 8 * scale), c =
- * clamp(rint((x - zero) / scale) + 8, 0, 15): 4.5 bits a value against 16.
+ * scale: 4.5 bits a value against 16. In fp32, each operation rounded once,
+ *   scale = f16((max - min) / 15), zero = f16(min + 8 * scale),
+ *   c = clamp(rint((x - zero) * (1 / scale)) + 8, 0, 15), 8 where scale is 0
+ * (a product with the rounded reciprocal: a quotient would round ties
+ * elsewhere). f16 ends at 2^-24: a group whose range is below about 1e-6 has
+ * scale 0 and becomes one value, a multiple of 2^-24 where it is that small.
  * `dtype` (INFERLAB_KV_F16 or INFERLAB_KV_BF16) is the row type: rows are
  * rounded to it before they are quantised, read back in it, and queries and
  * outputs of the attention entries are in it (or fp32). block_tokens must be a

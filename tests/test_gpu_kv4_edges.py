@@ -297,3 +297,25 @@ def test_segments_of_at_most_four_rows(torch, kv4, il, dim, heads, group, counts
     counts = np.array(counts)
     assert group * counts.max() <= 4
     check_attention(torch, kv4, il, kind, q_kind, heads, heads * group, dim, 16, starts, counts, seed=split, split=split)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_ties_follow_the_rounded_reciprocal(torch, kv4, il, kind, shift):  # noqa: F811
+    """Rows of steps and half steps: the codes are those of the product with the fp32 reciprocal, as the header says, also where a
+    quotient would round a tie to the other side. `shift` 1: rows that no 16-byte load reaches."""
+    n = np.arange(1, 101, dtype=np.float32)
+    x = kv4.round_to((np.arange(64) % 31 / 2 - 7.5).astype(np.float32) * (n * np.float32(2.0 ** -6))[:, None], kind)
+    codes, scale, zero = kv4.quantise(x)
+    quotient = np.clip(np.rint((x - zero.astype(np.float32)) / scale.astype(np.float32)) + 8, 0, 15)
+    assert (quotient != codes).sum() > 20
+    arena = np.zeros((7, 1, 1, kv4.tile_bytes(64)), np.uint8)
+    pool = filled_pool(torch, il, arena, kind, 16, 64)
+    flat = torch.zeros((100, 64 + shift), device="cuda:0", dtype=kind_of(torch, kind))
+    rows = flat[:, shift:].unsqueeze(1)
+    rows.copy_(torch.from_numpy(x)[:, None])
+    pool.append_rotary(None, rows, rows, None, i32(torch, [0] * 100), i32(torch, range(100)), i32(torch, [list(range(7))]))
+    pool.synchronize()
+    kv4.write_rows(arena, np.arange(100) // 16, np.arange(100) % 16, x[:, None], x[:, None])
+    assert np.array_equal(pool.arena.cpu().numpy(), arena)
+    pool.close()
