@@ -25,15 +25,16 @@
 // The mma computes S^T = K Q^T and O^T = V^T P^T: 16 tokens or dims by 8 query
 // columns. P^T's operand layout is S^T's result transposed (movmatrix).
 //
-// What bounds it: HBM, (D + D / 8) bytes a token and kv-head (144 at D = 128,
-// 23 bytes a clock and SM), and with 67% of the issue slots used the instructions
-// behind them: 64 sequences of 4096 to 32768 tokens x 8 kv-heads, 4 queries each,
-// 1489 MB in 280 us (5.3 TB/s; 324 us where the clock falls under load). One CTA of
-// four warps per (sequence, kv-head, 8 columns, split); every warp streams its
-// own 16-token tiles through a ring in shared memory, so that the warps never
-// wait for each other before the merge. The copies are 16-byte cp.async by all
-// lanes: five instructions a tile, where a bulk copy by one lane with its
-// barrier took ~40 issue slots of ~430.
+// What bounds it: (D + D / 8) bytes a token and kv-head from HBM (144 at D = 128,
+// 23 bytes a clock and SM), and behind them the instructions of four warps a
+// scheduler, which use 67% of its slots and mostly wait on each other's fixed
+// latencies: 64 sequences of 4096 to 32768 tokens x 8 kv-heads, 4 queries each,
+// 1489 MB in 280 to 327 us with the card and its clock under load (5.3 to 4.6
+// TB/s). One CTA of four warps per (sequence, kv-head, 8 columns, split); every
+// warp streams its own 16-token tiles through a ring in shared memory, so that
+// the warps never wait for each other before the merge. The copies are 16-byte
+// cp.async by all lanes: five instructions a tile, where a bulk copy by one lane
+// with its barrier took ~40 issue slots of ~430.
 #include "common.cuh"
 #include "internal.cuh"
 #include "kv4.cuh"
@@ -148,11 +149,9 @@ __device__ __forceinline__ float score_with_room(float score, float factor_log2)
 __device__ __forceinline__ int slot_of_row(int r) { return r & 1 ? 7 - (r >> 1) : r >> 1; }
 
 // What a CTA works on: a split of a sequence's keys, and which of its kv-heads
-// and tiles. By length (the host says for which batches), sequences come in the
+// and tiles. By length (run_kv4 says for which batches), sequences come in the
 // order of their contexts, which the device knows, all of a long one's CTAs before
-// a shorter one's: the short ones fill what the long ones leave (4 chunks of 512
-// tokens on contexts of 32 to 8192: 268 -> 215 us; a decode of 32 contexts: 41 ->
-// 37.5). Otherwise the last splits come first, which only long contexts have;
+// a shorter one's: the short ones fill what the long ones leave. Otherwise the last splits come first, which only long contexts have;
 // row tiles (kRowTiles: rest = tile x kv-heads + kv-head) then before the
 // sequences, those with the most keys first (8 prompts of 1 to 1024 tokens: 66
 // us, 82 sequence by sequence).
@@ -794,9 +793,10 @@ Kv4Plan plan_kv4(const InferlabCudaKvPool& p, std::uint32_t num_seqs, std::uint3
     // 64 and 128 rows on the tensor cores, 134, 175 and 342 in column tiles; 4 on
     // 8000 tokens 68, 71 and 81 against 65, 78 and 134. fp32 results need
     // weights in two parts and take the row kernel from 128 rows on, where its
-    // tiles fill the GPU: 64 fresh prompts of 32 tokens 40 us against 108, 64
-    // segments on 1200 tokens 398 against 379, one prompt of 32 tokens 13 against
-    // 10.
+    // tiles fill the GPU: 64 fresh prompts of 32 tokens 40 us against 108 in column
+    // tiles, one prompt of 32 tokens (not filled) 13 against 10; where they meet,
+    // 64 segments of 32 tokens on 1200, the row kernel is the slower one by 5%, 398
+    // against 379.
     const bool tensor = query_dtype != kFp32;
     const std::uint64_t row_tile = tensor ? kTcRows : kRowTile, row_tiles = (rows + row_tile - 1) / row_tile;
     const std::uint64_t row_units = checked_mul(checked_mul(num_seqs, p.kv_heads, "4-bit attention batch is too large"),
@@ -909,10 +909,19 @@ void run_kv4(InferlabCudaKvPool& p, Kv4Params k, std::uint32_t query_dtype, std:
     k.column_tiles = plan.column_tiles;
     k.max_splits = plan.max_splits;
     k.per_seq = p.kv_heads * plan.column_tiles;
-    // Split contexts of more than 32 sequences even out without (64 x 4096..32768:
-    // 279 us, 312 by length), whole ones only where the CTAs are not all resident
-    // at once (64 x 5 drafted tokens: 78 us, 70 by length; row tiles have an order
-    // of their own).
+    // What decides is how much the lengths differ, which only the device knows, and
+    // the number of sequences stands in for it. us without / by length, 32 heads
+    // over 8 kv-heads x 128, split: a decode of one context of 32768 among short
+    // ones 39 / 33 (8 sequences), 57 / 47 (32), 63 / 56 (64); of zipf lengths 106 /
+    // 106 (16), 131 / 130 (32), 247 / 250 (64); of 4096 to 32768 evenly drawn 47 /
+    // 53 (8), 159 / 174 (32), 270 / 305 (64); of one length 233 / 238 (32). So by
+    // length up to 32 costs even batches up to 13% and gives skewed ones up to 18%,
+    // and more than 32, which are mostly even, do without. Row tiles (128 tokens
+    // each on up to 8192) gain at every size: zipf 826 / 750 (32), 829 / 752 (33),
+    // 1610 / 1431 (64), even 960 / 793, 970 / 808, 1714 / 1517, so from 33 on this
+    // rule leaves them 10 to 20%. Whole contexts only where the CTAs are not all
+    // resident at once (64 x 5 drafted tokens: 78 / 70; row tiles have an order of
+    // their own).
     k.by_length = num_seqs > 1 && (plan.max_splits > 1 ? num_seqs <= 32
                                                        : plan.kind == Kv4Plan::kColumns && num_seqs <= 64 &&
                                                              static_cast<std::uint64_t>(num_seqs) * k.per_seq > 592);

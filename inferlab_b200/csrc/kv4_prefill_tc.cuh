@@ -23,13 +23,14 @@
 // tokens on contexts up to 8192.
 // Two CTAs an SM: one's softmax runs beside the other's MMAs (half of the 512
 // TMEM columns and 110 KB of shared memory each).
-// Bound by instruction issue (54% of the slots, 18% of the tensor pipe): a block
-// costs its eight warps ~700 instructions each, 250 of them the widening, and
-// 4300 clocks, of which the other CTA uses the gaps. 4 chunks of 512 tokens on
-// contexts up to 8192, 32 heads over 8 kv-heads: 212 us, 376 TFLOP/s. A CTA's
-// queries, first keys and outputs cost as much as four blocks, so short prompts
-// come off worse (8 of 1 to 1024 tokens, 16 heads: 63 us). A second S in TMEM,
-// issued a block ahead, changed nothing.
+// Bound by latency: 54% of the issue slots, 18% of the tensor pipe and 2% of DRAM
+// are used. A block is one chain (S, softmax, weights to TMEM, O) with two or three
+// barriers of the CTA; it costs the eight warps ~700 instructions each, 250 of them
+// the widening, and 4300 clocks, of which only the other CTA uses the gaps. 4
+// chunks of 512 tokens on contexts up to 8192, 32 heads over 8 kv-heads: 212 us,
+// 376 TFLOP/s. A CTA's queries, first keys and outputs cost as much as four
+// blocks, so short prompts come off worse (8 of 1 to 1024 tokens, 16 heads: 63
+// us). A second S in TMEM, issued a block ahead, changed nothing.
 #pragma once
 
 #include "tc_common.cuh"

@@ -17,8 +17,10 @@
 // widened to fp32 beside them and applied to scores and weights.
 // Bound by shared memory and latency: 16 rows, 16 tokens and 128 dims take 48 mma
 // (384 clocks of an SM's quarter), 16 ldmatrix and ~230 other instructions of the
-// three warps that a quarter holds. 64 fresh prompts of 128 tokens, 32 heads over
-// 8 kv-heads: 176 us, 470 in column tiles.
+// three warps that a quarter holds; 168 registers, 76 bytes of them spilled at D =
+// 128. 64 fresh prompts of 128 tokens, 32 heads over 8 kv-heads: 176 us, 470 in
+// column tiles; 4 chunks of 512 tokens on contexts up to 8192 850 us, 8 prompts of
+// 1 to 1024 tokens of 16 heads 125 (16-bit queries: 212 and 63).
 #pragma once
 
 namespace ilb {
@@ -57,7 +59,6 @@ __device__ __forceinline__ void ldmatrix4_trans(std::uint32_t (&r)[4], std::uint
 template <typename RowT, int D>
 __global__ void __launch_bounds__(kRowWarps * 32, 3) kv4_rows_kernel(const Kv4Params p) {
     using L = RowSmem<D>;
-    using QT = float;
     constexpr int kTile = kv4::tile_bytes(D);
     constexpr int kGroups = D / kv4::kGroup;
     constexpr int kUnits = D / 8;  // words of a token's row
@@ -87,7 +88,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) kv4_rows_kernel(const Kv4Pa
     };
     if (!valid) {
         for (int i = threadIdx.x; first_split && i < live * D; i += blockDim.x) {
-            static_cast<QT*>(p.out)[row_of(i / D) * D + i % D] = Storage<QT>::from_float(0.0f);
+            static_cast<float*>(p.out)[row_of(i / D) * D + i % D] = 0.0f;
         }
         return;
     }
@@ -135,14 +136,13 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) kv4_rows_kernel(const Kv4Pa
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int row = 16 * warp + 8 * h + g;
-        const QT* src = static_cast<const QT*>(p.queries) + row_of(min(row, live - 1)) * D + 8 * t4;
+        const float* src = static_cast<const float*>(p.queries) + row_of(min(row, live - 1)) * D + 8 * t4;
         float x[D / 32][8], most = 0.0f;
         bool bad = false;
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) {
-            constexpr int kPer = 16 / sizeof(QT);
 #pragma unroll
-            for (int c = 0; c < 8 / kPer; ++c) widen16(reinterpret_cast<const uint4*>(src + 32 * w)[c], &x[w][c * kPer], QT{});
+            for (int c = 0; c < 2; ++c) widen16(reinterpret_cast<const uint4*>(src + 32 * w)[c], &x[w][4 * c], 0.0f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 x[w][i] = row < live ? Storage<RowT>::to_float(Storage<RowT>::from_float(x[w][i])) : 0.0f;
@@ -371,10 +371,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) kv4_rows_kernel(const Kv4Pa
                     for (int r = 0; r < 2; ++r) {
                         const float w0 = scaled[h][k][r].x, w1 = scaled[h][k][r].y;
                         a[2 * h + r] = f16_pair(w0, w1);
-                        {
-                            const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&a[2 * h + r]));
-                            a2[2 * h + r] = f16_pair(w0 - t.x, w1 - t.y);
-                        }
+                        const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&a[2 * h + r]));
+                        a2[2 * h + r] = f16_pair(w0 - t.x, w1 - t.y);
                     }
                 }
 #pragma unroll
@@ -384,10 +382,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) kv4_rows_kernel(const Kv4Pa
                     ldmatrix4_trans(vf, at + L::kValue + token * L::kRow + ((unit ^ (token & 7)) << 4));
                     mma_f16(o[u], a[0], a[1], a[2], a[3], vf[0], vf[1]);
                     mma_f16(o[u + 1], a[0], a[1], a[2], a[3], vf[2], vf[3]);
-                    {
-                        mma_f16(o[u], a2[0], a2[1], a2[2], a2[3], vf[0], vf[1]);
-                        mma_f16(o[u + 1], a2[0], a2[1], a2[2], a2[3], vf[2], vf[3]);
-                    }
+                    mma_f16(o[u], a2[0], a2[1], a2[2], a2[3], vf[0], vf[1]);
+                    mma_f16(o[u + 1], a2[0], a2[1], a2[2], a2[3], vf[2], vf[3]);
                 }
             }
         }
@@ -441,7 +437,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) kv4_rows_kernel(const Kv4Pa
             *reinterpret_cast<float4*>(part + 16 * warp * D + 4 * i) = x;
             continue;
         }
-        store_row4(static_cast<QT*>(p.out) + row_of(row) * D + 4 * i % D, x);
+        store_row4(static_cast<float*>(p.out) + row_of(row) * D + 4 * i % D, x);
     }
     if (splits == 1) return;
     if (!last_of(p.ws_count + work, splits, ticket)) return;
@@ -451,7 +447,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) kv4_rows_kernel(const Kv4Pa
         bool ok;
         const float4 x = merge_parts<kPart, kRowTile * D>(parts, splits, row, i, ok);
         if (!ok) flag_error(p.error_word, kErrNormalizer);
-        store_row4(static_cast<QT*>(p.out) + row_of(row) * D + 4 * i % D, x);
+        store_row4(static_cast<float*>(p.out) + row_of(row) * D + 4 * i % D, x);
     }
 }
 

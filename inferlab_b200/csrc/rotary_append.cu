@@ -309,10 +309,12 @@ __device__ __forceinline__ void store4(T* at, const float (&x)[4]) {
 //   Q (blockIdx.y 1): a thread takes four dims and their partners, so nothing is
 //     loaded or widened twice, and asks for several heads' at once.
 // Everything of a row is asked for in one round of loads behind its sequence and
-// position. Bound by HBM: 8192 rows of 32 + 8 + 8 bf16 heads x 128 move 12 KB in
-// and 8 KB (+ 2.3 KB a row in 4 bits) out each; what it needs for that is rows
-// in flight: as one CTA of 256 threads and 64 registers 51 us, split in two and
-// Q by eight dims (70 registers) 48.
+// position, and what it is short of is rows in flight: 8192 rows of 16 + 16 + 16
+// fp32 heads x 128 into an f16 pool take 57 us (90% of the copy rate), of 32 + 8 +
+// 8 bf16 heads into 4 bits, 12 KB in and 8 + 2.3 KB out each, 51 (28 at that
+// rate; 59% of the issue slots and a third of DRAM used, warps wait for their
+// rows). As one CTA of 256 threads and 64 registers, or with Q by eight dims (70
+// registers), a tenth more.
 template <typename RowT, typename PoolT, typename OutT, bool kFourBit, bool kNeighbours, int kPasses>
 __global__ void __launch_bounds__(kRowThreads) rotary_append_vector_kernel(const AppendParams p) {
     const std::size_t row = blockIdx.x;
@@ -529,9 +531,10 @@ struct GatherParams {
 };
 
 // The common shapes of a gather: units of 8 dims, 16-byte accesses; a 4-bit
-// pool's unit is one word of codes and its group's pair. Bound by HBM as the
-// append is (8192 rows of 8 + 8 heads x 128: 12 us in 128 threads a row, 15 in
-// 256).
+// pool's unit is one word of codes and its group's pair. Bound by a short CTA's
+// chain of loads (place, table, tile): 8192 rows of 8 + 8 heads x 128 of a 4-bit
+// pool 14 us (7 at the copy rate; 256 threads a row a quarter more), of 16 + 16
+// heads of an f16 pool 28 (20).
 constexpr int kGatherThreads = 128;
 template <typename T, bool kFourBit>
 __global__ void __launch_bounds__(kGatherThreads) gather_rows_vector_kernel(const GatherParams p) {
