@@ -328,6 +328,13 @@ int inferlab_cuda_pool_set_decode_split(InferlabCudaKvPool* pool, uint32_t block
                                         char* error, size_t error_capacity);
 
 /*
+ * 1 while `stream` is being captured into a graph, else 0. A call captured with a
+ * workspace writes to it at every replay, so a captured call wants one that
+ * nothing else uses or frees.
+ */
+int inferlab_cuda_stream_is_capturing(void* stream);
+
+/*
  * Zeroes a decode workspace. Needed once per workspace before its first use,
  * for its first 64 KB at least, which hold the split counters; the decode
  * kernels leave them at zero. Batches of any sizes may use a workspace in turn

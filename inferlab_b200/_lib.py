@@ -174,6 +174,7 @@ SIGNATURES = {
         c_vp, c_err, c_sz]),
     "inferlab_cuda_kv_gather": (ctypes.c_int, [
         c_vp, c_vp, ctypes.c_uint64, c_vp, c_vp, c_vp, c_err, c_sz]),
+    "inferlab_cuda_stream_is_capturing": (ctypes.c_int, [c_vp]),
     "inferlab_cuda_paged_decode_workspace_size": (c_sz, [
         c_vp, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32]),
     "inferlab_cuda_paged_decode_workspace_init": (ctypes.c_int, [c_vp, c_sz, c_vp, c_err, c_sz]),

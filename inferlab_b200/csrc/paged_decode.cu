@@ -1237,6 +1237,15 @@ extern "C" int inferlab_cuda_pool_set_decode_split(InferlabCudaKvPool* pool,
     });
 }
 
+extern "C" int inferlab_cuda_stream_is_capturing(void* stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &status) != cudaSuccess) {
+        cudaGetLastError();  // the legacy stream while another one captures: not itself captured
+        return 0;
+    }
+    return status != cudaStreamCaptureStatusNone;
+}
+
 extern "C" int inferlab_cuda_paged_decode_workspace_init(void* workspace,
                                                          std::size_t workspace_bytes,
                                                          void* stream, char* error,

@@ -51,13 +51,32 @@ def _torch_stream(device: int, stream) -> torch.cuda.Stream:
 def _made(shape, dtype, device: int, stream) -> torch.Tensor:
     """Memory that a call fills on `stream`, allocated there: the current stream may still use what
     its own allocations reuse. It is then read on the current stream, as a rule, behind `stream`."""
-    if stream is None:
-        return torch.empty(shape, dtype=dtype, device=f"cuda:{device}")
-    here = torch.cuda.current_stream(device)
-    with torch.cuda.stream(_torch_stream(device, stream)):
-        made = torch.empty(shape, dtype=dtype, device=f"cuda:{device}")
+    if stream is None or stream.cuda_stream == torch._C._cuda_getCurrentRawStream(device):
+        return torch.empty(shape, dtype=dtype, device=device)
+    here, there = torch.cuda.current_stream(device), _torch_stream(device, stream)
+    near = torch.cuda.current_device() == device
+    with _On(there, here) if near else torch.cuda.stream(there):
+        made = torch.empty(shape, dtype=dtype, device=device)
     made.record_stream(here)
     return made
+
+
+class _On:
+    """torch.cuda.stream for two streams of the current device, of which `here` is current: what the
+    general form costs is as much as a call."""
+
+    def __init__(self, stream, here):
+        self.stream, self.here = stream, here
+
+    def __enter__(self):
+        s = self.stream
+        torch._C._cuda_setStream(stream_id=s.stream_id, device_index=s.device_index,
+                                 device_type=s.device_type)
+
+    def __exit__(self, *exc):
+        s = self.here
+        torch._C._cuda_setStream(stream_id=s.stream_id, device_index=s.device_index,
+                                 device_type=s.device_type)
 
 
 class _DeviceView:
@@ -443,14 +462,16 @@ class CudaKvPool:
         partials. A capture gets one of its own, zeroed by the graph, so that graphs replayed side
         by side share none and none outlives what it was captured with."""
         shape = (raw, num_seqs, q_heads, max_query_count, max_context_len)
-        if stream is None and not torch.cuda.is_current_stream_capturing():
+        capturing = (torch.cuda.is_current_stream_capturing() if stream is None
+                     else self._lib.inferlab_cuda_stream_is_capturing(raw) != 0)
+        if not capturing:
             known = self._fitting.get(shape)
             if known is not None:
                 return known
         need = self.workspace_size(num_seqs, q_heads, max_context_len, max_query_count)
         used = _torch_stream(self.device, stream)
         with torch.cuda.stream(used):  # the allocation belongs to that stream
-            if torch.cuda.is_current_stream_capturing():
+            if capturing:
                 return self._zeroed(need, used)
             ws = self._workspaces.get(raw)
             if ws is None or ws.numel() < need:

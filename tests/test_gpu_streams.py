@@ -59,3 +59,99 @@ def test_outputs_belong_to_the_stream_given(bits, handle_only):
     assert stream_of(torch, again) == side.cuda_stream
     pool.synchronize()
     pool.close()
+
+
+def test_calls_leave_the_current_stream_and_device_alone():
+    """Also where an allocation on the stream given fails."""
+    import torch
+
+    import inferlab_b200 as il
+    from inferlab_b200.paged import _made
+
+    pool = il.CudaKvPool(0, 2, 64, 16, 2, 64)
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    q = torch.randn((1, 2, 64), device="cuda:0")
+    table = torch.zeros((1, 4), dtype=torch.int32, device="cuda:0")
+    lens = torch.ones(1, dtype=torch.int32, device="cuda:0")
+    torch.cuda.synchronize()
+    for here in (torch.cuda.default_stream(), other):
+        with torch.cuda.stream(here):
+            for stream in (None, side, here, torch.cuda.default_stream()):
+                pool.decode(q, table, lens, 1, stream=stream)
+                assert torch.cuda.current_stream() == here and torch.cuda.current_device() == 0
+            with pytest.raises(RuntimeError):
+                _made((-1,), torch.float32, 0, side)
+            assert torch.cuda.current_stream() == here
+    torch.cuda.synchronize()
+    pool.synchronize()
+    pool.close()
+
+
+def test_a_stream_under_capture_is_known():
+    import torch
+
+    from inferlab_b200 import _lib
+
+    lib = _lib.lib()
+    side = torch.cuda.Stream()
+    x = torch.zeros(4, device="cuda:0")
+    assert lib.inferlab_cuda_stream_is_capturing(None) == 0
+    assert lib.inferlab_cuda_stream_is_capturing(side.cuda_stream) == 0
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        here = torch.cuda.current_stream()
+        assert lib.inferlab_cuda_stream_is_capturing(here.cuda_stream) == 1
+        assert lib.inferlab_cuda_stream_is_capturing(side.cuda_stream) == 0
+        side.wait_stream(here)
+        assert lib.inferlab_cuda_stream_is_capturing(side.cuda_stream) == 1
+        here.wait_stream(side)
+        x += 1
+    assert lib.inferlab_cuda_stream_is_capturing(side.cuda_stream) == 0
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool((x == 1).all())
+    del graph
+
+
+@pytest.mark.parametrize("bits", [None, 4])
+def test_a_captured_call_on_a_forked_stream(bits):
+    """Inside a capture, with the stream given and without, each call has a workspace of its own."""
+    import torch
+
+    import inferlab_b200 as il
+
+    gen = torch.Generator(device="cuda:0").manual_seed(1)
+    pool = il.CudaKvPool(0, 2, 64, 16, 2, 64, kv_bits=bits)
+    rows = torch.randn((1024, 4, 64), device="cuda:0", generator=gen)
+    at = torch.arange(1024, device="cuda:0", dtype=torch.int32)
+    pool.append_rotary(None, rows[:, :2], rows[:, 2:], None, at // 1024, at, torch.arange(64, device="cuda:0", dtype=torch.int32)[None])
+    pool.set_decode_split(2)
+    q = torch.randn((8, 4, 64), device="cuda:0", generator=gen)
+    table = torch.randint(0, 64, (8, 16), device="cuda:0", dtype=torch.int32, generator=gen)
+    lens = torch.randint(100, 257, (8,), device="cuda:0", dtype=torch.int32, generator=gen)
+    want = pool.decode(q, table, lens, 256)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        side.wait_stream(torch.cuda.default_stream())
+        assert torch.equal(pool.decode(q, table, lens, 256), want)
+    torch.cuda.synchronize()
+    outs = [torch.zeros_like(q) for _ in range(3)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        pool.decode(q, table, lens, 256, out=outs[0], stream=side)
+        pool.decode(q, table, lens, 256, out=outs[1])
+        made = pool.decode(q, table, lens, 256, stream=side)
+        here.wait_stream(side)
+        outs[2].copy_(made)
+    for _ in range(5):
+        graph.replay()
+        pool.decode(q, table, lens, 256, stream=side)
+    torch.cuda.synchronize()
+    for out in outs:
+        assert torch.equal(out, want)
+    pool.synchronize()
+    del graph
+    pool.close()
