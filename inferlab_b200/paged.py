@@ -45,6 +45,8 @@ def _torch_stream(device: int, stream) -> torch.cuda.Stream:
         return torch.cuda.current_stream(device)
     if isinstance(stream, torch.cuda.Stream):
         return stream
+    if stream.cuda_stream in (0, 1):  # both name the legacy stream
+        return torch.cuda.default_stream(device)
     return torch.cuda.ExternalStream(stream.cuda_stream, device=device)
 
 

@@ -76,7 +76,8 @@ def test_calls_leave_the_current_stream_and_device_alone():
     torch.cuda.synchronize()
     for here in (torch.cuda.default_stream(), other):
         with torch.cuda.stream(here):
-            for stream in (None, side, here, torch.cuda.default_stream()):
+            handles = [types.SimpleNamespace(cuda_stream=n) for n in (0, 1, 2, side.cuda_stream)]
+            for stream in (None, side, here, torch.cuda.default_stream(), *handles):
                 pool.decode(q, table, lens, 1, stream=stream)
                 assert torch.cuda.current_stream() == here and torch.cuda.current_device() == 0
             with pytest.raises(RuntimeError):
